@@ -35,6 +35,7 @@ enum {
 #define OFB_TYPE_F16 1
 #define OFB_TYPE_Q4_K 12
 #define OFB_TYPE_Q6_K 14
+#define OFB_TYPE_BF16 30
 
 /* output element types of the dequant entry points */
 #define OFB_OUT_F32 0
@@ -228,6 +229,139 @@ int ofb_matvec(const float *x, int n_tokens, int in_dim, int out_dim, const void
 #define OFB_SAMPLE_SCRATCH(vocab) ((vocab) + 2 * (((vocab) + 1023) / 1024))
 int ofb_sample(const float *logits, int vocab, float temperature, float r, float *scratch, uint32_t *token,
                void *stream);
+
+/* ---- attention cache --------------------------------------------------------
+ * The attention half of a decode step: rotary positions, a paged key/value
+ * cache, attention of one new token over it and eviction from it. The
+ * reference's attention (engine/src/model.c:563-679) runs on the CPU over a
+ * flat f32 cache of 256 positions (engine/src/inference.c:15) and rotates by
+ * one position axis; pages, several axes, accumulated weights and eviction
+ * have no counterpart there.
+ *
+ * One layer's cache. Entry i of sequence b lives in page
+ * p = page_table[b][i / page_size] at slot s = i % page_size; per kv head h its
+ * key and value rows start at element
+ *   p*page_stride + (h*page_size + s)*head_dim
+ * of k and v, and its accumulated weight and order number are element
+ * (p*n_kv_heads + h)*page_size + s of `weight` and `order`. Entries of a
+ * sequence differ between kv heads once an eviction has been made (each head
+ * keeps its own), their number does not. Keys are stored rotated, so attention
+ * does not depend on the place of an entry.
+ *
+ * Only the pages that hold entries below the sequence's length are looked up;
+ * table entries behind them may hold anything, and what is in memory behind
+ * the last entry is neither used nor changed. A page number outside
+ * [0, n_pages) is never followed: such an entry counts as masked (attention),
+ * is dropped (append), or as the lightest (eviction), and OFB_CACHE_EPAGE is
+ * set. No page may belong to two sequences of one call that write it. */
+#define OFB_CACHE_EPAGE 1u  /* a page number outside [0, n_pages) */
+#define OFB_CACHE_ELEN 2u   /* a length above the call's max_len or the table's reach: cut down to it */
+#define OFB_CACHE_EINDEX 4u /* append: a sequence or place outside the table: the row was dropped */
+typedef struct {
+    void *k, *v;               /* device, 16-byte aligned; element type `type` */
+    float *weight;             /* device f32 [n_pages][n_kv_heads][page_size], or NULL */
+    int32_t *order;            /* device int32, laid out like weight, or NULL */
+    const int32_t *page_table; /* device int32 [n_seqs][max_pages] */
+    uint32_t *errors;          /* device word that collects OFB_CACHE_E* bits (never cleared here), or NULL */
+    int64_t page_stride;       /* elements from one page of k (and of v) to the next: a multiple of 8,
+                                  at least n_kv_heads*page_size*head_dim; 0 means exactly that */
+    int32_t type;              /* OFB_TYPE_BF16 or OFB_TYPE_F16 */
+    int32_t n_kv_heads;        /* 1..1024 */
+    int32_t head_dim;          /* 64, 96, 128, 192 or 256 */
+    int32_t page_size;         /* entries per page, 1..65536 */
+    int32_t n_pages;
+    int32_t n_seqs;            /* rows of the page table */
+    int32_t max_pages;         /* columns of the page table */
+} ofb_kv_cache;
+
+/* Rotary positions with up to four axes (time, height, width, ...). The first
+ * rot_dim elements of a head are turned in pairs, the others pass through:
+ *   y[u] = x[u] cos a - x[v] sin a,  y[v] = x[v] cos a + x[u] sin a,
+ *   a = pos[axis(i)][token] * f(i)  for pair i = 0 .. rot_dim/2-1.
+ * section[a] pairs belong to axis a (their sum is rot_dim/2). BLOCKED: axis 0
+ * has the first section[0] pairs, axis 1 the next, and so on. DEALT: pair i
+ * belongs to axis i % n_axes while that axis has pairs left
+ * (i / n_axes < section[axis]), else to axis 0; this deals section[a] pairs to
+ * every axis a >= 1 when section[a] * n_axes <= rot_dim/2 + n_axes - 1 - a
+ * (else the call is refused).
+ * per_axis 0: f(i) = base^(-2i/rot_dim); per_axis 1 (BLOCKED only): axis a's
+ * j-th pair has base^(-j/section[a]). Angles are formed in 64 bits, so far
+ * positions keep their place in the turn. */
+#define OFB_ROPE_HALVES 0   /* pair i: elements i and i + rot_dim/2 */
+#define OFB_ROPE_ADJACENT 1 /* pair i: elements 2i and 2i+1 */
+#define OFB_ROPE_BLOCKED 0
+#define OFB_ROPE_DEALT 1
+typedef struct {
+    int32_t rot_dim;    /* even, 2..256, <= head_dim */
+    int32_t pairing;    /* OFB_ROPE_HALVES / OFB_ROPE_ADJACENT */
+    int32_t order;      /* OFB_ROPE_BLOCKED / OFB_ROPE_DEALT */
+    int32_t n_axes;     /* 1..4 */
+    int32_t per_axis;   /* 0/1 */
+    int32_t section[4]; /* pairs per axis, >= 0 */
+    double base;        /* > 0 */
+} ofb_rope_config;
+
+/* out[t][h] = x[t][h] turned by its token's positions. type OFB_TYPE_F32, BF16
+ * or F16 (arithmetic in f32, rounded once). x and out: row t starts at element
+ * t*x_stride (t*out_stride), its heads are consecutive; out may be x with the
+ * same stride, otherwise they must not overlap. pos: int32 [n_axes][n_tokens],
+ * axis a at a*pos_stride. head_dim 1..1024. */
+int ofb_rope(const ofb_rope_config *rope, const void *x, int type, int n_tokens, int n_heads, int head_dim,
+             int64_t x_stride, const int32_t *pos, int64_t pos_stride, void *out, int64_t out_stride, void *stream);
+
+/* One layer's new tokens enter the cache: token t's key rows are turned (when
+ * `rope` is given) and written with its value rows as entry index[t] of
+ * sequence seq[t], its weight there set to 0 and its order number to
+ * number[t] (index[t] when number is NULL); in the same launch its n_heads
+ * query rows are turned into q_out (q NULL: none). Padding rows have
+ * seq[t] < 0: they write nothing to the cache; their queries are turned all
+ * the same. q, k, v: element type `type` (OFB_TYPE_F32 or the cache's), row t
+ * of q at t*q_stride with its heads consecutive, k and v rows with n_kv_heads
+ * heads likewise (parts of one projection's rows, for instance); q_out like q
+ * and may be q with the same stride. The (seq, index) of a call are distinct:
+ * of two rows for one entry, parts of either may remain. */
+int ofb_rope_append(const ofb_kv_cache *cache, const ofb_rope_config *rope, int type, int n_tokens, int n_heads,
+                    const void *q, int64_t q_stride, const void *k, int64_t k_stride, const void *v,
+                    int64_t v_stride, const int32_t *pos, int64_t pos_stride, const int32_t *seq,
+                    const int32_t *index, const int32_t *number, void *q_out, int64_t q_out_stride, void *stream);
+
+/* Attention of one new token per sequence over its cached entries (its own
+ * among them, appended before), split over the length across the GPU and
+ * joined in a fixed order (results are reproducible):
+ *   out[b][h] = sum_n p_n v_n,  p = softmax over n < lens[b] of scale * q[b][h].k_n
+ * where head h reads kv head h / (n_heads / n_kv_heads). lens: device int32
+ * [n_seqs], n_seqs <= cache->n_seqs rows of the page table in order; a length
+ * of 0 (or below) gives zeros. max_len bounds every length (0: the table's
+ * reach) and sizes the scratch. q and out: type OFB_TYPE_F32 or the cache's,
+ * row b at b*q_stride (b*out_stride), heads consecutive; they must not overlap.
+ * accumulate 1: cache->weight of entry n of kv head g grows by the sum of p_n
+ * over g's query heads. Softmax, sums and weights are f32 and queries and
+ * probabilities are not rounded to the cache's type. scratch:
+ * ofb_attn_scratch_size() bytes of device memory, 16-byte aligned, needing no
+ * initialisation; calls whose GPU work may overlap (other streams, graphs
+ * replayed side by side) need scratch of their own. */
+size_t ofb_attn_scratch_size(const ofb_kv_cache *cache, int n_heads, int n_seqs, int max_len, int accumulate);
+int ofb_attn_decode(const ofb_kv_cache *cache, const void *q, int type, int64_t q_stride, int n_heads, float scale,
+                    const int32_t *lens, int n_seqs, int max_len, int accumulate, void *out, int64_t out_stride,
+                    void *scratch, size_t scratch_bytes, void *stream);
+
+/* Eviction: sequence b's cache is brought down to min(lens[b], keep) entries,
+ * per kv head by itself. Kept are first the entries whose order number is
+ * above (highest order number - recent), then those of the largest accumulated
+ * weight (NaN counts as the lightest, -0 as 0); equals go to the lower place.
+ * Kept entries at or behind place `keep` move, in ascending order, into the
+ * places below it that fall free, also ascending, with their weight and order
+ * number; all other entries stay where they are, and the memory at and behind
+ * `keep` is left as it was. Writes lens_out[b] = min(lens[b], keep) and, when
+ * kept is given, kept[b][h][i] = the place that entry i comes from (-1 for
+ * i >= lens_out[b]; int32 [n_seqs][n_kv_heads][keep]). cache->weight and
+ * cache->order are needed. 0 <= recent <= keep, keep >= 1; max_len as for
+ * ofb_attn_decode, at most OFB_EVICT_MAX_LEN; lens_out must not overlap lens.
+ * scratch as for ofb_attn_decode. */
+#define OFB_EVICT_MAX_LEN 393216
+size_t ofb_kv_evict_scratch_size(const ofb_kv_cache *cache, int n_seqs, int keep);
+int ofb_kv_evict(const ofb_kv_cache *cache, const int32_t *lens, int n_seqs, int max_len, int keep, int recent,
+                 int32_t *lens_out, int32_t *kept, void *scratch, size_t scratch_bytes, void *stream);
 
 /* ---- GGUF -> HBM ------------------------------------------------------------
  * Replaces gguf_open / gguf_read_tensor_bytes (engine/src/gguf.c:408-445,

@@ -1,0 +1,244 @@
+// attn.cu — ofb_attn_decode: the join of the split kernel's parts (attn.cuh)
+// and the entry point.
+//
+// Second launch (programmatic, its CTAs come up as the split kernel's leave):
+// one CTA per query head joins the parts of a head that more than one CTA
+// worked on,
+//   M = max m_i, out = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i,
+// in the order of the parts, so the result does not depend on timing. With
+// `accumulate`, further CTAs add each entry's probability, summed over the
+// query heads of its kv head in their order, to the cache's weight: they read
+// the scores the split kernel left (4 bytes per entry and query head, an
+// eighth of the entry's K and V at 8 heads of 128; forming them again would
+// read all of K a second time).
+#include "attn.cuh"
+
+namespace ofb {
+
+constexpr int AJ_THREADS = 256;
+constexpr int AJ_CHUNK = 512;  // entries of one weight CTA
+
+struct AttnJoinArgs {
+    AttnArgs a;
+    int ctas, d, n_out, chunks;  // CTAs of the split kernel; join CTAs, weight CTAs per (sequence, kv head)
+};
+
+// Where the parts of (sequence b, pass vh) are: CTAs c0..c1 of the split kernel.
+struct PartRange {
+    long long c0, c1, f0, run;
+    __device__ __forceinline__ int64_t slot(int i) const { return 2 * (c0 + i) + ((c0 + i) * run < f0 ? 1 : 0); }
+};
+__device__ __forceinline__ PartRange part_range(const AttnJoinArgs &j, int b, int vh, int nt) {
+    const int nvh = j.a.KVH * j.a.NB;
+    PartRange r;
+    r.run = attn_run((long long)j.a.prefix[j.a.B] * nvh, j.ctas);
+    r.f0 = (long long)j.a.prefix[b] * nvh + (long long)vh * nt;
+    r.c0 = r.f0 / r.run;
+    r.c1 = (r.f0 + nt - 1) / r.run;
+    return r;
+}
+
+// Maximum and sum of exponentials over the parts of row r, by one warp.
+__device__ __forceinline__ float2 warp_ml(const AttnJoinArgs &j, const PartRange &pr, int r, int lane) {
+    const int n = (int)(pr.c1 - pr.c0) + 1;
+    float m = -INFINITY;
+    for (int i = lane; i < n; i += 32) m = fmaxf(m, j.a.part_ml[pr.slot(i) * ATT_R + r].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const float ref = m == -INFINITY ? 0.0f : m;
+    float l = 0.0f;
+    for (int i = lane; i < n; i += 32) {
+        const float2 e = j.a.part_ml[pr.slot(i) * ATT_R + r];
+        l += exp2f(e.x - ref) * e.y;
+    }
+    return make_float2(ref, warp_sum(l));
+}
+
+template <typename IO> __global__ void __launch_bounds__(AJ_THREADS) attn_join_kernel(const __grid_constant__ AttnJoinArgs j) {
+    __shared__ float acc[AJ_THREADS / 32][256 + 4];
+    __shared__ float2 ml[128];
+    const AttnArgs &a = j.a;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    pdl_wait();
+    pdl_trigger();
+    if (blockIdx.x < j.n_out) {
+        const int b = blockIdx.x / a.H, h = blockIdx.x - b * a.H, kvh = h / a.G, g = h - kvh * a.G;
+        const int nt = a.prefix[b + 1] - a.prefix[b];
+        if (!nt) return;
+        const PartRange pr = part_range(j, b, kvh * a.NB + g / ATT_R, nt);
+        if (pr.c0 == pr.c1) return;
+        const int r = g % ATT_R, n = (int)(pr.c1 - pr.c0) + 1;
+        const float2 e = warp_ml(j, pr, r, lane);
+        for (int x0 = 0; x0 < j.d; x0 += 128) {
+            const int x = x0 + lane * 4;
+            if (x >= j.d) continue;
+            float4 s = make_float4(0, 0, 0, 0);
+#pragma unroll 4
+            for (int i = warp; i < n; i += AJ_THREADS / 32) {
+                const int64_t p = pr.slot(i) * ATT_R + r;
+                const float f = exp2f(a.part_ml[p].x - e.x);
+                const float4 y = *reinterpret_cast<const float4 *>(a.part_o + p * j.d + x);
+                s.x += f * y.x, s.y += f * y.y, s.z += f * y.z, s.w += f * y.w;
+            }
+            *reinterpret_cast<float4 *>(&acc[warp][x]) = s;
+        }
+        __syncthreads();
+        const float inv = e.y > 0.0f || e.y != e.y ? 1.0f / e.y : 0.0f;
+        for (int x = tid; x < j.d; x += AJ_THREADS) {
+            float s = 0.0f;
+#pragma unroll
+            for (int w = 0; w < AJ_THREADS / 32; w++) s += acc[w][x];
+            static_cast<IO *>(a.out)[b * a.out_stride + (int64_t)h * j.d + x] = from_f32<IO>(s * inv);
+        }
+        return;
+    }
+    // weights of entries [i0, i0 + AJ_CHUNK) of one (sequence, kv head)
+    const unsigned w = blockIdx.x - j.n_out;
+    const int u = (int)(w / j.chunks), b = u / a.KVH, kvh = u - b * a.KVH, i0 = (int)(w - (unsigned)u * j.chunks) * AJ_CHUNK;
+    const int len = attn_len(a, b);
+    if (i0 >= len) return;
+    const int nt = a.prefix[b + 1] - a.prefix[b];
+    float add[AJ_CHUNK / AJ_THREADS] = {};
+    for (int g0 = 0; g0 < a.G; g0 += 128) {  // ml holds 128 heads at a time
+        const int ng = min(a.G - g0, 128);
+        for (int g = warp; g < ng; g += AJ_THREADS / 32) {
+            const PartRange pr = part_range(j, b, kvh * a.NB + (g0 + g) / ATT_R, nt);
+            const float2 e = pr.c0 == pr.c1 ? a.ml[(int64_t)b * a.H + kvh * a.G + g0 + g] : warp_ml(j, pr, (g0 + g) % ATT_R, lane);
+            if (lane == 0) ml[g] = make_float2(e.x == -INFINITY ? 0.0f : e.x, e.y > 0.0f || e.y != e.y ? 1.0f / e.y : 0.0f);
+        }
+        __syncthreads();
+        const float *z = a.z + ((int64_t)b * a.H + kvh * a.G + g0) * a.z_stride + i0 + tid;
+        for (int g = 0; g < ng; g++, z += a.z_stride) {
+            const float2 e = ml[g];
+#pragma unroll
+            for (int k = 0; k < AJ_CHUNK / AJ_THREADS; k++)
+                if (i0 + k * AJ_THREADS + tid < len) add[k] += exp2f(z[k * AJ_THREADS] - e.x) * e.y;
+        }
+        __syncthreads();
+    }
+#pragma unroll
+    for (int k = 0; k < AJ_CHUNK / AJ_THREADS; k++) {
+        const int i = i0 + k * AJ_THREADS + tid;
+        if (i >= len) continue;
+        const int col = i / a.page_size, page = a.table[(int64_t)b * a.max_pages + col];
+        if (page < 0 || page >= a.n_pages) continue;
+        a.weight[((int64_t)page * a.KVH + kvh) * a.page_size + (i - col * a.page_size)] += add[k];
+    }
+}
+
+struct AttnPlan {
+    AttnVariant v;
+    int max_len, ctas, NB;
+    int64_t z_stride;
+    size_t prefix, ml, part_o, part_ml, z, total;
+};
+
+// Checks the call's sizes and lays out its scratch.
+static int attn_plan(const ofb_kv_cache *c, int n_heads, int n_seqs, int max_len, int accumulate, bool f32, AttnPlan &p) {
+    int st = check_cache(c, "ofb_attn_decode");
+    if (st != OFB_OK) return st;
+    if (n_heads < 1 || n_heads % c->n_kv_heads || n_heads > 65536 || n_seqs < 0 || n_seqs > c->n_seqs || max_len < 0 ||
+        (accumulate != 0 && accumulate != 1)) {
+        set_error("ofb_attn_decode: %d heads over %d kv heads, %d sequences of %d, max_len %d", n_heads, c->n_kv_heads, n_seqs,
+                  c->n_seqs, max_len);
+        return OFB_EINVAL;
+    }
+    if (accumulate && !c->weight) { set_error("ofb_attn_decode: accumulate needs the cache's weight"); return OFB_EINVAL; }
+    if (n_seqs > ATT_MAX_SEQS) { set_error("ofb_attn_decode: %d sequences, %d at most", n_seqs, ATT_MAX_SEQS); return OFB_ETOOLARGE; }
+    const int reach = cache_reach(c);
+    p.max_len = max_len && max_len < reach ? max_len : reach;
+    const int64_t tiles = ((int64_t)p.max_len + ATT_TILE - 1) / ATT_TILE;
+    if (tiles * n_seqs > INT32_MAX) {
+        set_error("ofb_attn_decode: %d sequences of %d entries are too many tiles", n_seqs, p.max_len);
+        return OFB_ETOOLARGE;
+    }
+    const bool bf = c->type == OFB_TYPE_BF16;
+    switch (c->head_dim) {
+    case 64: p.v = attn_variant_64(bf, f32); break;
+    case 96: p.v = attn_variant_96(bf, f32); break;
+    case 128: p.v = attn_variant_128(bf, f32); break;
+    case 192: p.v = attn_variant_192(bf, f32); break;
+    default: p.v = attn_variant_256(bf, f32); break;
+    }
+    p.NB = (n_heads / c->n_kv_heads + ATT_R - 1) / ATT_R;
+    const int64_t runs = (tiles * n_seqs * c->n_kv_heads * p.NB + ATT_W - 1) / ATT_W;
+    const int most = sm_count() * p.v.ctas;
+    p.ctas = runs < 1 ? 1 : runs < most ? (int)runs : most;
+    p.z_stride = tiles * ATT_TILE;
+    size_t at = 0;
+    auto take = [&](size_t bytes) { const size_t o = at; at += (bytes + 255) / 256 * 256; return o; };
+    p.prefix = take((size_t)(n_seqs + 1) * 4);
+    p.ml = take((size_t)n_seqs * n_heads * 8);
+    // sized for a full grid, so that the size grows with n_seqs and max_len
+    p.part_ml = take((size_t)2 * most * ATT_R * 8);
+    p.part_o = take((size_t)2 * most * ATT_R * c->head_dim * 4);
+    p.z = accumulate ? take((size_t)n_seqs * n_heads * p.z_stride * 4) : 0;
+    p.total = at;
+    return OFB_OK;
+}
+
+}  // namespace ofb
+
+using namespace ofb;
+
+extern "C" size_t ofb_attn_scratch_size(const ofb_kv_cache *cache, int n_heads, int n_seqs, int max_len, int accumulate) {
+    AttnPlan p;
+    return attn_plan(cache, n_heads, n_seqs, max_len, accumulate, true, p) == OFB_OK ? p.total : 0;
+}
+
+extern "C" int ofb_attn_decode(const ofb_kv_cache *cache, const void *q, int type, int64_t q_stride, int n_heads,
+                               float scale, const int32_t *lens, int n_seqs, int max_len, int accumulate, void *out,
+                               int64_t out_stride, void *scratch, size_t scratch_bytes, void *stream) {
+    AttnPlan p;
+    int st = attn_plan(cache, n_heads, n_seqs, max_len, accumulate, type == OFB_TYPE_F32, p);
+    if (st != OFB_OK) return st;
+    if (type != OFB_TYPE_F32 && type != cache->type) {
+        set_error("ofb_attn_decode: type %d is neither F32 nor the cache's", type);
+        return OFB_EUNSUPPORTED;
+    }
+    if (!n_seqs) return OFB_OK;
+    const int64_t width = (int64_t)n_heads * cache->head_dim;
+    if (!q || !lens || !out || q == out || misaligned(q, type_size(type)) || misaligned(out, type_size(type)) ||
+        misaligned(lens, 4) || (n_seqs > 1 && (q_stride < width || out_stride < width)) || !(scale == scale)) {
+        set_error("ofb_attn_decode: bad arguments (q stride %lld, out stride %lld)", (long long)q_stride, (long long)out_stride);
+        return OFB_EINVAL;
+    }
+    if (!scratch || misaligned(scratch, 16)) { set_error("ofb_attn_decode: scratch is NULL or not 16-byte aligned"); return OFB_EINVAL; }
+    if (scratch_bytes < p.total) {
+        set_error("ofb_attn_decode: scratch of %zu bytes, %zu needed", scratch_bytes, p.total);
+        return OFB_ETOOLARGE;
+    }
+    uint8_t *w = static_cast<uint8_t *>(scratch);
+    AttnJoinArgs j = {};
+    AttnArgs &a = j.a;
+    a.k = cache->k, a.v = cache->v, a.q = q, a.out = out, a.table = cache->page_table, a.lens = lens;
+    a.page_stride = cache_page_stride(cache), a.q_stride = q_stride, a.out_stride = out_stride;
+    a.B = n_seqs, a.KVH = cache->n_kv_heads, a.G = n_heads / a.KVH, a.NB = p.NB, a.H = n_heads;
+    a.page_size = cache->page_size, a.max_pages = cache->max_pages, a.n_pages = cache->n_pages, a.max_len = p.max_len;
+    a.scale = scale * 1.4426950408889634f;
+    a.errors = cache->errors;
+    a.prefix = reinterpret_cast<int *>(w + p.prefix), a.ml = reinterpret_cast<float2 *>(w + p.ml);
+    a.part_o = reinterpret_cast<float *>(w + p.part_o), a.part_ml = reinterpret_cast<float2 *>(w + p.part_ml);
+    a.z = accumulate ? reinterpret_cast<float *>(w + p.z) : nullptr;
+    a.z_stride = p.z_stride, a.weight = cache->weight;
+    j.ctas = p.ctas, j.d = cache->head_dim;
+    j.n_out = n_seqs * n_heads;
+    j.chunks = (p.max_len + AJ_CHUNK - 1) / AJ_CHUNK;
+    const int64_t blocks = (int64_t)n_seqs * n_heads + (accumulate ? (int64_t)n_seqs * a.KVH * j.chunks : 0);
+    if (blocks > INT32_MAX) { set_error("ofb_attn_decode: too many weight blocks"); return OFB_ETOOLARGE; }
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    // a raised shared-memory limit per kernel and device
+    static size_t attr[20][64];
+    const int vi = (cache->head_dim == 64 ? 0 : cache->head_dim == 96 ? 1 : cache->head_dim == 128 ? 2 : cache->head_dim == 192 ? 3 : 4) * 4 +
+                   (cache->type == OFB_TYPE_BF16 ? 2 : 0) + (type == OFB_TYPE_F32 ? 1 : 0);
+    cudaError_t e = ensure_dyn_smem(p.v.kernel, p.v.smem, attr[vi]);
+    if (e != cudaSuccess) return cuda_status(e, "ofb_attn_decode smem attribute");
+    e = launch_pdl(p.v.kernel, dim3(p.ctas), dim3(ATT_W * 32), p.v.smem, s, a);
+    if (e != cudaSuccess) return cuda_status(e, "ofb_attn_decode launch");
+    if (p.ctas == 1 && !accumulate) return OFB_OK;  // every part is whole
+    const dim3 grid((unsigned)blocks), block(AJ_THREADS);
+    e = type == OFB_TYPE_F32              ? launch_pdl(attn_join_kernel<float>, grid, block, 0, s, j)
+        : cache->type == OFB_TYPE_BF16 ? launch_pdl(attn_join_kernel<__nv_bfloat16>, grid, block, 0, s, j)
+                                       : launch_pdl(attn_join_kernel<__half>, grid, block, 0, s, j);
+    return e == cudaSuccess ? OFB_OK : cuda_status(e, "ofb_attn_decode join launch");
+}

@@ -1,0 +1,442 @@
+// attn.cuh — attention of one new token over the paged cache: the split
+// kernel (attn_d*.cu hold its instances, attn.cu the join and the entry point).
+//
+//   z_n = scale * q.k_n,  p_n = exp(z_n - m) / l,  out = sum_n p_n v_n
+//
+// HBM-bound: 4 * head_dim bytes per cached entry and kv head against
+// 4 * head_dim operations per query head.
+//
+// Work: the entries of each (sequence, kv head) are cut into tiles of 16, and
+// the tiles of all of them, laid end to end, are dealt to the CTAs in equal
+// runs, whatever the lengths. A run holds parts of one or more (sequence, kv
+// head)s; a part that is not whole goes to the scratch (sums, maximum, sum of
+// exponentials) and attn.cu joins it with the others.
+//
+// Inside a CTA each warp takes every fourth tile of a part by itself: its own
+// ring of tiles in shared memory filled by 16-byte asynchronous copies (page
+// by page, ATT_S - 1 tiles ahead and across parts), its own running maximum
+// and sums, no barrier but one merge at the end of a part. Rows are padded by
+// 16 bytes, so that ldmatrix meets no bank twice.
+//
+// The products run on mma.sync m16n8k16 (bf16 or fp16, f32 sums): 16 rows of A
+// by 8 entries or 8 output columns. Query heads of one kv head fill 8 rows at
+// most; the other 8 take the low-order parts of the same numbers, so that
+// neither an f32 query nor a probability is rounded to the cache's type:
+//   query: in the cache's type one part, exact. f32: bf16 hi + mid + low (24
+//     bits, two mma) or fp16 hi + low (22 bits, one mma) of q scaled by a power
+//     of two into fp16's range.
+//   probability: bf16 hi + low (16 bits) or, for f32 output, + lowest (24
+//     bits, a second mma); fp16 hi + low of 2^14 p (22 bits).
+// A row's parts end in the same thread (accumulators c0, c1 and c2, c3), which
+// adds them in f32. Each tile's product starts at zero and is added to the
+// running sum by an FFMA, since the tensor core's own accumulation cuts off
+// where an addition rounds.
+#pragma once
+#include <type_traits>
+
+#include "async.cuh"
+#include "kv_cache.cuh"
+
+namespace ofb {
+
+constexpr int ATT_W = 4;      // warps per CTA
+constexpr int ATT_TILE = 16;  // entries per tile
+constexpr int ATT_R = 8;      // query heads per pass
+constexpr int ATT_MAX_SEQS = 2048;
+
+struct AttnArgs {
+    const void *k, *v, *q;
+    void *out;
+    const int32_t *table, *lens;
+    int64_t page_stride, q_stride, out_stride;
+    int B, KVH, G, NB, H;  // NB: passes of at most ATT_R heads per kv head
+    int page_size, max_pages, n_pages, max_len;
+    float scale;      // times log2(e)
+    uint32_t *errors;
+    // scratch
+    int *prefix;      // [B + 1] tiles before each sequence, per pass
+    float2 *ml;       // [B][H] maximum (log2) and sum of whole parts
+    float *part_o;    // [2 * CTAs][ATT_R][d]
+    float2 *part_ml;  // [2 * CTAs][ATT_R]
+    float *z;         // [B][H][z_stride] scores in log2, or NULL
+    int64_t z_stride;
+    float *weight;
+};
+
+// How many entries of sequence b are attended to.
+__device__ __forceinline__ int attn_len(const AttnArgs &a, int b) { return min(max(a.lens[b], 0), a.max_len); }
+// Tiles per CTA when `total` tiles are dealt to `ctas` CTAs: at least one per
+// warp, so that few tiles do not leave many parts to join.
+__host__ __device__ __forceinline__ long long attn_run(long long total, int ctas) {
+    const long long n = (total + ctas - 1) / ctas;
+    return n < ATT_W ? ATT_W : n;
+}
+
+template <int D> struct AttnShape {
+    static constexpr int PITCH = D * 2 + 16;                 // bytes of a row in shared memory
+    static constexpr int TILE_BYTES = 2 * ATT_TILE * PITCH;  // K, then V
+    static constexpr int S = D <= 64 ? 5 : D <= 96 ? 4 : D <= 128 ? 3 : D <= 192 ? 4 : 3;  // ring slots
+    static constexpr int CTAS = D <= 128 ? 2 : 1;            // per SM
+    static constexpr int RING = ATT_W * S * TILE_BYTES;
+    static constexpr int SMEM = RING + ATT_W * ATT_R * 8 + (ATT_MAX_SEQS + 1) * 4;
+    static_assert(TILE_BYTES >= ATT_R * (D + 4) * 4, "a warp's sums must fit one ring slot");
+    static_assert(CTAS * (SMEM + 1536) <= 228 * 1024, "shared memory of an SM");
+};
+
+template <typename T> struct Mma;
+template <> struct Mma<__nv_bfloat16> {
+    static __device__ __forceinline__ void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+template <> struct Mma<__half> {
+    static __device__ __forceinline__ void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                     : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                     : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    }
+};
+
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix4_t(uint32_t (&r)[4], uint32_t addr) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+// 16 bytes, or 16 zero bytes when `bytes` is 0 (the source is then not read).
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+// Splits (x, y) into parts of T: p[i] holds part i of x (low half) and y.
+template <typename T, int N> __device__ __forceinline__ void split2(float x, float y, uint32_t (&p)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        const T a = from_f32<T>(x), b = from_f32<T>(y);
+        uint16_t ua, ub;
+        memcpy(&ua, &a, 2);
+        memcpy(&ub, &b, 2);
+        p[i] = ua | ((uint32_t)ub << 16);
+        if (i + 1 < N) x -= to_f32(a), y -= to_f32(b);
+    }
+}
+
+// A part: tiles [t, end) of (sequence b, pass vh) within this CTA's run.
+struct AttnPart {
+    int b, vh, t, end, nt;
+};
+// The part that begins at tile `f` of the row of all tiles, cut at f1.
+__device__ __forceinline__ AttnPart attn_part(const int *prefix, int B, int nvh, long long f, long long f1) {
+    int lo = 0, hi = B - 1;  // the last sequence that begins at or before f (and has tiles)
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if ((long long)prefix[mid] * nvh <= f) lo = mid;
+        else hi = mid - 1;
+    }
+    AttnPart p;
+    p.b = lo;
+    p.nt = prefix[lo + 1] - prefix[lo];
+    const long long r = f - (long long)prefix[lo] * nvh;
+    p.vh = (int)(r / p.nt);
+    p.t = (int)(r - (long long)p.vh * p.nt);
+    const long long left = f1 - f;
+    p.end = left < p.nt - p.t ? p.t + (int)left : p.nt;
+    return p;
+}
+
+template <int D, typename CT, typename IO>
+__global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_kernel(const __grid_constant__ AttnArgs a) {
+    using SH = AttnShape<D>;
+    constexpr bool F32 = sizeof(IO) == 4, BF = sizeof(CT) == 2 && std::is_same<CT, __nv_bfloat16>::value;
+    constexpr int NQ = F32 ? (BF ? 3 : 2) : 1;       // parts of a query
+    constexpr int NP = BF && F32 ? 3 : 2;            // parts of a probability
+    constexpr float PSCALE = BF ? 1.0f : 16384.0f;   // fp16 holds 2^14 p
+    constexpr int KS = D / 16;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c2 = (lane & 3) * 2;
+    uint8_t *ring = smem + warp * SH::S * SH::TILE_BYTES;
+    float2 *mml = reinterpret_cast<float2 *>(smem + SH::RING);  // [W][R]
+    int *prefix = reinterpret_cast<int *>(mml + ATT_W * ATT_R);
+    __shared__ uint32_t valid[ATT_W][8];  // per ring slot: which of the 16 entries are there
+    __shared__ int wsum[ATT_W];
+    __shared__ float *mo[ATT_W];  // each warp's sums at the end of a part, [R][D + 4]
+
+    pdl_wait();
+    pdl_trigger();
+
+    // tiles before each sequence; every CTA forms them for itself
+    for (int base = 0; base < a.B; base += ATT_W * 32) {
+        const int b = base + tid;
+        int n = 0;
+        if (b < a.B) {
+            if (a.lens[b] > a.max_len && blockIdx.x == 0) report(a.errors, OFB_CACHE_ELEN);
+            n = (attn_len(a, b) + ATT_TILE - 1) / ATT_TILE;
+        }
+        int s = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, s, o);
+            if (lane >= o) s += u;
+        }
+        if (lane == 31) wsum[warp] = s;
+        if (!base && !tid) prefix[0] = 0;
+        __syncthreads();
+        int before = prefix[base];
+        for (int w = 0; w < warp; w++) before += wsum[w];
+        if (b < a.B) prefix[b + 1] = before + s;
+        __syncthreads();
+    }
+    if (blockIdx.x == 0)
+        for (int b = tid; b <= a.B; b += ATT_W * 32) a.prefix[b] = prefix[b];
+    // sequences without entries: zeros
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+        if (prefix[b + 1] == prefix[b])
+            for (int i = tid; i < a.H * D; i += ATT_W * 32) static_cast<IO *>(a.out)[b * a.out_stride + i] = from_f32<IO>(0.0f);
+
+    const int nvh = a.KVH * a.NB;
+    const long long total = (long long)prefix[a.B] * nvh, run = attn_run(total, gridDim.x);
+    const long long f0 = blockIdx.x * run, f1 = min(total, f0 + run);
+    if (f0 >= f1) return;
+
+    const uint32_t ring_s = ax::smem_u32(ring);
+    // Copies tile t of part p into ring slot `slot`; lanes 0..15 find the rows.
+    auto load = [&](const AttnPart &p, int t, int slot) {
+        const int i = t * ATT_TILE + (lane & 15), len = attn_len(a, p.b);
+        int64_t off = -1;
+        if (i < len) {
+            const int col = i / a.page_size, page = a.table[(int64_t)p.b * a.max_pages + col];
+            if (page >= 0 && page < a.n_pages)
+                off = page * a.page_stride + ((int64_t)(p.vh / a.NB) * a.page_size + (i - col * a.page_size)) * D;
+            else report(a.errors, OFB_CACHE_EPAGE);
+        }
+        const uint32_t mask = __ballot_sync(0xffffffffu, off >= 0);
+        if (lane == 0) valid[warp][slot] = mask & 0xffffu;
+        const uint32_t dst = ring_s + slot * SH::TILE_BYTES;
+        constexpr int CH = D / 8;  // 16-byte chunks of a row
+#pragma unroll
+        for (int j = 0; j < ATT_TILE * CH / 32; j++) {
+            const int c = j * 32 + lane, r = c / CH, x = c - r * CH;
+            const int64_t o = __shfl_sync(0xffffffffu, off, r);
+            const int64_t e = o < 0 ? 0 : o + x * 8;
+            const int n = o < 0 ? 0 : 16;
+            cp16(dst + r * SH::PITCH + x * 16, static_cast<const CT *>(a.k) + e, n);
+            cp16(dst + (ATT_TILE + r) * SH::PITCH + x * 16, static_cast<const CT *>(a.v) + e, n);
+        }
+    };
+
+    // the part and tile that the ring is filled from, ahead of the one computed
+    AttnPart lp = attn_part(prefix, a.B, nvh, f0, f1);
+    long long lf = f0;
+    int lt = lp.t + warp;
+    bool more = true;
+    auto fill = [&](int slot) {
+        while (more && lt >= lp.end) {
+            lf += lp.end - lp.t;
+            if (lf >= f1) more = false;
+            else lp = attn_part(prefix, a.B, nvh, lf, f1), lt = lp.t + warp;
+        }
+        if (more) load(lp, lt, slot), lt += ATT_W;
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+#pragma unroll
+    for (int i = 0; i < SH::S - 1; i++) fill(i);
+    int slot = 0;  // of the next tile to compute
+
+    int npart = 0;
+    for (long long f = f0; f < f1; npart++) {
+        const AttnPart p = attn_part(prefix, a.B, nvh, f, f1);
+        const int kvh = p.vh / a.NB, h0 = (p.vh - kvh * a.NB) * ATT_R, rows = min(ATT_R, a.G - h0);
+        // queries: row g of A, parts as told at the top
+        uint32_t qa[KS][2][NQ];
+        float qscale = a.scale;
+        {
+            const IO *qr = static_cast<const IO *>(a.q) + p.b * a.q_stride + (int64_t)(kvh * a.G + h0 + g) * D;
+            float up = 1.0f;
+            if constexpr (F32 && !BF) {
+                // a power of two that brings the row's largest element to [2^13, 2^14)
+                float m = 0.0f;
+                if (g < rows)
+                    for (int i = c2; i < D; i += 8) m = fmaxf(m, fmaxf(fabsf(qr[i]), fabsf(qr[i + 1])));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                const int e = (int)(__float_as_uint(m) >> 23);  // 0: zero or subnormal, 255: not finite
+                if (e > 0 && e < 255) {
+                    const int sh = min(max(13 + 127 - e, -100), 100);
+                    up = __uint_as_float((uint32_t)(127 + sh) << 23);
+                    qscale = a.scale * __uint_as_float((uint32_t)(127 - sh) << 23);
+                }
+            }
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    float x = 0.0f, y = 0.0f;
+                    if (g < rows) {
+                        x = to_f32(qr[ks * 16 + u * 8 + c2]) * up;
+                        y = to_f32(qr[ks * 16 + u * 8 + c2 + 1]) * up;
+                    }
+                    split2<CT, NQ>(x, y, qa[ks][u]);
+                }
+        }
+        float o[D / 8][2], m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int i = 0; i < D / 8; i++) o[i][0] = o[i][1] = 0.0f;
+
+        for (int t = p.t + warp; t < p.end; t += ATT_W) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(SH::S - 2) : "memory");
+            __syncwarp();
+            fill(slot == 0 ? SH::S - 1 : slot - 1);
+            const uint32_t ks_s = ring_s + slot * SH::TILE_BYTES, vs_s = ks_s + ATT_TILE * SH::PITCH;
+            const uint32_t ok = valid[warp][slot];
+            slot = slot == SH::S - 1 ? 0 : slot + 1;
+
+            float s[2][4] = {}, s2[2][4] = {};
+            const uint32_t ka = ks_s + ((lane & 7) + ((lane >> 4) << 3)) * SH::PITCH + ((lane >> 3) & 1) * 16;
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+                uint32_t b[4];
+                ldmatrix4(b, ka + ks * 32);
+                const uint32_t a0[4] = {qa[ks][0][0], NQ > 1 ? qa[ks][0][NQ > 1 ? 1 : 0] : 0u, qa[ks][1][0],
+                                        NQ > 1 ? qa[ks][1][NQ > 1 ? 1 : 0] : 0u};
+                float(&c0)[4] = ks & 1 ? s2[0] : s[0];
+                float(&c1)[4] = ks & 1 ? s2[1] : s[1];
+                Mma<CT>::run(c0, a0, b[0], b[1]);
+                Mma<CT>::run(c1, a0, b[2], b[3]);
+                if constexpr (NQ > 2) {
+                    const uint32_t a1[4] = {qa[ks][0][2], 0u, qa[ks][1][2], 0u};
+                    Mma<CT>::run(c0, a1, b[0], b[1]);
+                    Mma<CT>::run(c1, a1, b[2], b[3]);
+                }
+            }
+            // scores of row g, entries 8j + c2 + {0, 1}, in log2
+            float z[2][2];
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    float x = s[j][u] + s2[j][u];
+                    if (NQ > 1) x += s[j][2 + u] + s2[j][2 + u];
+                    z[j][u] = (ok >> (8 * j + c2 + u)) & 1 ? x * qscale : -INFINITY;
+                }
+            if (a.z && g < rows) {
+                float *zr = a.z + ((int64_t)p.b * a.H + kvh * a.G + h0 + g) * a.z_stride + t * ATT_TILE + c2;
+                *reinterpret_cast<float2 *>(zr) = make_float2(z[0][0], z[0][1]);
+                *reinterpret_cast<float2 *>(zr + 8) = make_float2(z[1][0], z[1][1]);
+            }
+            float mt = fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[1][0], z[1][1]));
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
+            const float mn = fmaxf(m, mt), ref = mn == -INFINITY ? 0.0f : mn;
+            const float alpha = exp2f(m - ref);  // 0 at the first tile
+            m = mn;
+            uint32_t pa[2][NP];  // [entries 0-7 / 8-15][part]
+            float sum = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const float x = exp2f(z[j][0] - ref), y = exp2f(z[j][1] - ref);
+                sum += x + y;
+                split2<CT, NP>(x * PSCALE, y * PSCALE, pa[j]);
+            }
+            l = l * alpha + sum;
+            const uint32_t va = vs_s + ((lane & 7) + ((lane >> 3) & 1) * 8) * SH::PITCH + (lane >> 4) * 16;
+            const uint32_t a0[4] = {pa[0][0], pa[0][1], pa[1][0], pa[1][1]};
+#pragma unroll
+            for (int n = 0; n < D / 16; n++) {
+                uint32_t b[4];
+                ldmatrix4_t(b, va + n * 32);
+                float x[4] = {}, y[4] = {};
+                Mma<CT>::run(x, a0, b[0], b[1]);
+                Mma<CT>::run(y, a0, b[2], b[3]);
+                if constexpr (NP > 2) {
+                    const uint32_t a1[4] = {pa[0][2], 0u, pa[1][2], 0u};
+                    Mma<CT>::run(x, a1, b[0], b[1]);
+                    Mma<CT>::run(y, a1, b[2], b[3]);
+                }
+                o[2 * n][0] = o[2 * n][0] * alpha + (x[0] + x[2]);
+                o[2 * n][1] = o[2 * n][1] * alpha + (x[1] + x[3]);
+                o[2 * n + 1][0] = o[2 * n + 1][0] * alpha + (y[0] + y[2]);
+                o[2 * n + 1][1] = o[2 * n + 1][1] * alpha + (y[1] + y[3]);
+            }
+        }
+        // merge the warps: their sums, maxima and sums of exponentials. A warp
+        // leaves its sums in the ring slot it computed last, which the next
+        // fill is for (at the start: the one not filled yet).
+        l += __shfl_xor_sync(0xffffffffu, l, 1);
+        l += __shfl_xor_sync(0xffffffffu, l, 2);
+        __syncwarp();
+        float *const mslot = reinterpret_cast<float *>(ring + (slot == 0 ? SH::S - 1 : slot - 1) * SH::TILE_BYTES);
+        float *mw = mslot + g * (D + 4);
+        if (lane == 0) mo[warp] = mslot;
+#pragma unroll
+        for (int i = 0; i < D / 8; i++) *reinterpret_cast<float2 *>(mw + i * 8 + c2) = make_float2(o[i][0], o[i][1]);
+        if ((lane & 3) == 0) mml[warp * ATT_R + g] = make_float2(m, l);
+        __syncthreads();
+        const bool whole = p.t == 0 && p.end == p.nt;
+        const int64_t slot_id = 2 * (int64_t)blockIdx.x + (npart ? 1 : 0);
+        for (int i = tid; i < rows * (D / 4); i += ATT_W * 32) {
+            const int r = i / (D / 4), x = (i - r * (D / 4)) * 4;
+            float mm = -INFINITY;
+#pragma unroll
+            for (int w = 0; w < ATT_W; w++) mm = fmaxf(mm, mml[w * ATT_R + r].x);
+            const float ref = mm == -INFINITY ? 0.0f : mm;
+            float ll = 0.0f;
+            float4 acc = make_float4(0, 0, 0, 0);
+#pragma unroll
+            for (int w = 0; w < ATT_W; w++) {
+                const float2 e = mml[w * ATT_R + r];
+                const float s = exp2f(e.x - ref);
+                const float4 y = *reinterpret_cast<const float4 *>(mo[w] + r * (D + 4) + x);
+                ll += s * e.y;
+                acc.x += s * y.x, acc.y += s * y.y, acc.z += s * y.z, acc.w += s * y.w;
+            }
+            const int64_t head = kvh * a.G + h0 + r;
+            if (whole) {
+                // no entry attended to (all on bad pages): zeros
+                const float inv = ll > 0.0f || ll != ll ? 1.0f / (ll * PSCALE) : 0.0f;
+                IO *dst = static_cast<IO *>(a.out) + p.b * a.out_stride + head * D + x;
+                dst[0] = from_f32<IO>(acc.x * inv), dst[1] = from_f32<IO>(acc.y * inv);
+                dst[2] = from_f32<IO>(acc.z * inv), dst[3] = from_f32<IO>(acc.w * inv);
+                if (x == 0) a.ml[(int64_t)p.b * a.H + head] = make_float2(mm, ll);
+            } else {
+                const float u = 1.0f / PSCALE;
+                *reinterpret_cast<float4 *>(a.part_o + (slot_id * ATT_R + r) * D + x) = make_float4(acc.x * u, acc.y * u, acc.z * u, acc.w * u);
+                if (x == 0) a.part_ml[slot_id * ATT_R + r] = make_float2(mm, ll);
+            }
+        }
+        __syncthreads();  // the slots may be filled again
+        f += p.end - p.t;
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+using AttnKernel = void (*)(AttnArgs);
+struct AttnVariant {
+    AttnKernel kernel;
+    int smem, ctas;  // dynamic shared memory, CTAs per SM
+};
+// The instance for a head width: cache type bf16 or fp16, activations f32 or the cache's.
+AttnVariant attn_variant_64(bool bf16, bool f32);
+AttnVariant attn_variant_96(bool bf16, bool f32);
+AttnVariant attn_variant_128(bool bf16, bool f32);
+AttnVariant attn_variant_192(bool bf16, bool f32);
+AttnVariant attn_variant_256(bool bf16, bool f32);
+
+}  // namespace ofb
+
+#define OFB_ATTN_INSTANCES(D)                                                                                 \
+    namespace ofb {                                                                                           \
+    AttnVariant attn_variant_##D(bool bf16, bool f32) {                                                       \
+        const AttnKernel k = bf16 ? (f32 ? attn_split_kernel<D, __nv_bfloat16, float>                         \
+                                         : attn_split_kernel<D, __nv_bfloat16, __nv_bfloat16>)                \
+                                  : (f32 ? attn_split_kernel<D, __half, float> : attn_split_kernel<D, __half, __half>); \
+        return {k, AttnShape<D>::SMEM, AttnShape<D>::CTAS};                                                   \
+    }                                                                                                         \
+    }

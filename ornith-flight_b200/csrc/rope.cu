@@ -1,0 +1,351 @@
+// rope.cu — rotary positions with several axes, and the entry of new tokens
+// into the paged cache (ofb_rope, ofb_rope_append).
+//
+//   y[u] = x[u] cos a - x[v] sin a,  y[v] = x[v] cos a + x[u] sin a,
+//   a = pos[axis(i)] * f(i) for pair i = (u, v)
+//
+// HBM-bound: every element is read and written once, in one launch for q, k
+// and v. A CTA owns a few tokens. It first forms the cosine and sine of each
+// (token, pair) once in shared memory, for all heads: pos * f / pi in f64 (a
+// position of a million turns with f = 1 would lose its place in f32), less
+// the nearest even integer, so that the f32 that goes to sincospif is within
+// [-1, 1] and off by at most 2^-25 half turns. f(i)/pi comes with the launch:
+// the host forms it by one powl and repeated products, 1 KB of arguments.
+// Then each thread takes items of two 8-element chunks (a pair's two halves,
+// or 16 neighbours), read and written 16 bytes at a time. Sizes or addresses
+// that do not allow it (head_dim or rot_dim no multiple of 16, strides no
+// multiple of 8, pointers off 16 bytes) take the second kernel, a pair per
+// item.
+#include <math.h>
+
+#include "kv_cache.cuh"
+
+namespace ofb {
+
+constexpr int RP_THREADS = 256;
+constexpr int RP_PAIRS = 128;
+
+struct RopeArgs {
+    int T, H, KVH, d, rot, tpb;  // heads of q; kv heads (0: no cache); tokens per CTA
+    int n_pages, page_size, n_seqs, max_pages;
+    const void *q, *k, *v;
+    void *q_out, *ck, *cv;
+    int64_t qs, ks, vs, qos, page_stride, pos_stride;
+    const int32_t *pos, *seq, *index, *number, *table;
+    float *weight;
+    int32_t *order;
+    uint32_t *errors;
+    double half_turns[RP_PAIRS];  // f(i) / pi
+    uint8_t axis[RP_PAIRS];
+};
+
+// Shared memory: cs[tpb][rot/2], then entry[tpb]: the row's flat (page, slot),
+// or -1 where nothing is written.
+__device__ __forceinline__ void rope_setup(const RopeArgs &a, int t0, int nt, float2 *cs, int64_t *entry) {
+    const int pairs = a.rot / 2;
+    for (int i = threadIdx.x; i < nt * pairs; i += RP_THREADS) {
+        const int t = i / pairs, p = i - t * pairs;
+        const double h = (double)a.pos[a.axis[p] * a.pos_stride + t0 + t] * a.half_turns[p];
+        float s, c;
+        sincospif((float)(h - 2.0 * rint(0.5 * h)), &s, &c);
+        cs[i] = make_float2(c, s);
+    }
+    if (a.KVH && threadIdx.x < nt) {
+        const int t = t0 + threadIdx.x, b = a.seq[t], i = a.index[t];
+        int64_t e = -1;
+        if (b >= 0) {
+            const int col = i / a.page_size;
+            if (b >= a.n_seqs || i < 0 || col >= a.max_pages) {
+                report(a.errors, OFB_CACHE_EINDEX);
+            } else {
+                const int p = a.table[(int64_t)b * a.max_pages + col];
+                if (p < 0 || p >= a.n_pages) report(a.errors, OFB_CACHE_EPAGE);
+                else e = (int64_t)p * a.page_size + (i - col * a.page_size);
+            }
+        }
+        entry[threadIdx.x] = e;
+    }
+    __syncthreads();
+}
+
+// Weight 0 and the order number of the CTA's new entries.
+__device__ __forceinline__ void rope_meta(const RopeArgs &a, int t0, int nt, const int64_t *entry) {
+    if (!a.weight && !a.order) return;
+    for (int i = threadIdx.x; i < nt * a.KVH; i += RP_THREADS) {
+        const int t = i / a.KVH, h = i - t * a.KVH;
+        const int64_t e = entry[t];
+        if (e < 0) continue;
+        const int64_t p = e / a.page_size, m = (p * a.KVH + h) * a.page_size + (e - p * a.page_size);
+        if (a.weight) a.weight[m] = 0.0f;
+        if (a.order) a.order[m] = a.number ? a.number[t0 + t] : a.index[t0 + t];
+    }
+}
+
+__device__ __forceinline__ int64_t cache_row(const RopeArgs &a, int64_t e, int h) {
+    const int64_t p = e / a.page_size;
+    return p * a.page_stride + ((int64_t)h * a.page_size + (e - p * a.page_size)) * a.d;
+}
+
+template <typename IO, typename CT, bool ADJ>
+__global__ void __launch_bounds__(RP_THREADS) rope_vec_kernel(const __grid_constant__ RopeArgs a) {
+    extern __shared__ float2 cs[];
+    int64_t *entry = reinterpret_cast<int64_t *>(cs + (size_t)a.tpb * (a.rot / 2));
+    pdl_wait();
+    pdl_trigger();
+    const int t0 = blockIdx.x * a.tpb, nt = min(a.tpb, a.T - t0);
+    rope_setup(a, t0, nt, cs, entry);
+    const int per_row = a.d / 16, rows = a.H + 2 * a.KVH, per_tok = rows * per_row, half = a.rot / 2;
+    for (int it = threadIdx.x; it < nt * per_tok; it += RP_THREADS) {
+        const int t = it / per_tok, r = it - t * per_tok, row = r / per_row, j = r - row * per_row;
+        const IO *src;
+        int64_t to = 0;
+        const bool is_q = row < a.H, is_v = row >= a.H + a.KVH;
+        if (is_q) {
+            src = static_cast<const IO *>(a.q) + (int64_t)(t0 + t) * a.qs + (int64_t)row * a.d;
+        } else {
+            if (entry[t] < 0) continue;
+            const int h = row - a.H - (is_v ? a.KVH : 0);
+            src = is_v ? static_cast<const IO *>(a.v) + (int64_t)(t0 + t) * a.vs + (int64_t)h * a.d
+                       : static_cast<const IO *>(a.k) + (int64_t)(t0 + t) * a.ks + (int64_t)h * a.d;
+            to = cache_row(a, entry[t], h);
+        }
+        // chunk places of this item: the two halves of 8 pairs, or 16 neighbours
+        const bool turned = !is_v && j * 16 < a.rot;
+        const int ca = turned && !ADJ ? 8 * j : 16 * j, cb = turned && !ADJ ? half + 8 * j : 16 * j + 8;
+        float x[8], y[8];
+        load8(src + ca, x);
+        load8(src + cb, y);
+        if (turned) {
+            const float2 *c = cs + t * half + 8 * j;
+            if (ADJ) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float2 w = c[i], z = c[4 + i];
+                    const float u = x[2 * i], v = x[2 * i + 1], m = y[2 * i], n = y[2 * i + 1];
+                    x[2 * i] = u * w.x - v * w.y;
+                    x[2 * i + 1] = v * w.x + u * w.y;
+                    y[2 * i] = m * z.x - n * z.y;
+                    y[2 * i + 1] = n * z.x + m * z.y;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float2 w = c[i];
+                    const float u = x[i], v = y[i];
+                    x[i] = u * w.x - v * w.y;
+                    y[i] = v * w.x + u * w.y;
+                }
+            }
+        }
+        if (is_q) {
+            IO *dst = static_cast<IO *>(a.q_out) + (int64_t)(t0 + t) * a.qos + (int64_t)row * a.d;
+            store8(dst + ca, x);
+            store8(dst + cb, y);
+        } else {
+            CT *dst = static_cast<CT *>(is_v ? a.cv : a.ck) + to;
+            store8(dst + ca, x);
+            store8(dst + cb, y);
+        }
+    }
+    rope_meta(a, t0, nt, entry);
+}
+
+// Any sizes and strides: items are pairs (rot/2 per row), then single elements.
+template <typename IO, typename CT>
+__global__ void __launch_bounds__(RP_THREADS) rope_any_kernel(const __grid_constant__ RopeArgs a, int adjacent) {
+    extern __shared__ float2 cs[];
+    int64_t *entry = reinterpret_cast<int64_t *>(cs + (size_t)a.tpb * (a.rot / 2));
+    pdl_wait();
+    pdl_trigger();
+    const int t0 = blockIdx.x * a.tpb, nt = min(a.tpb, a.T - t0);
+    rope_setup(a, t0, nt, cs, entry);
+    const int half = a.rot / 2, per_row = a.d - half, rows = a.H + 2 * a.KVH, per_tok = rows * per_row;
+    for (int it = threadIdx.x; it < nt * per_tok; it += RP_THREADS) {
+        const int t = it / per_tok, r = it - t * per_tok, row = r / per_row, j = r - row * per_row;
+        const bool is_q = row < a.H, is_v = row >= a.H + a.KVH;
+        const IO *src;
+        int64_t to = 0;
+        if (is_q) {
+            src = static_cast<const IO *>(a.q) + (int64_t)(t0 + t) * a.qs + (int64_t)row * a.d;
+        } else {
+            if (entry[t] < 0) continue;
+            const int h = row - a.H - (is_v ? a.KVH : 0);
+            src = is_v ? static_cast<const IO *>(a.v) + (int64_t)(t0 + t) * a.vs + (int64_t)h * a.d
+                       : static_cast<const IO *>(a.k) + (int64_t)(t0 + t) * a.ks + (int64_t)h * a.d;
+            to = cache_row(a, entry[t], h);
+        }
+        // where this item's one or two elements are
+        const int ea = j >= half ? half + j : adjacent ? 2 * j : j, eb = j >= half ? ea : adjacent ? 2 * j + 1 : half + j;
+        float x = to_f32(src[ea]), y = to_f32(src[eb]);
+        if (!is_v && j < half) {
+            const float2 w = cs[t * half + j];
+            const float u = x, v = y;
+            x = u * w.x - v * w.y;
+            y = v * w.x + u * w.y;
+        }
+        if (is_q) {
+            IO *dst = static_cast<IO *>(a.q_out) + (int64_t)(t0 + t) * a.qos + (int64_t)row * a.d;
+            dst[ea] = from_f32<IO>(x);
+            dst[eb] = from_f32<IO>(y);
+        } else {
+            CT *dst = static_cast<CT *>(is_v ? a.cv : a.ck) + to;
+            dst[ea] = from_f32<CT>(x);
+            dst[eb] = from_f32<CT>(y);
+        }
+    }
+    rope_meta(a, t0, nt, entry);
+}
+
+// Checks a rotary form and lays out its pairs: axis and frequency / pi.
+static int rope_tables(const ofb_rope_config *r, int head_dim, const char *who, RopeArgs &a) {
+    if (r->rot_dim < 2 || r->rot_dim > 2 * RP_PAIRS || r->rot_dim % 2 || r->rot_dim > head_dim || r->n_axes < 1 ||
+        r->n_axes > 4 || (r->pairing != OFB_ROPE_HALVES && r->pairing != OFB_ROPE_ADJACENT) ||
+        (r->order != OFB_ROPE_BLOCKED && r->order != OFB_ROPE_DEALT) || (r->per_axis != 0 && r->per_axis != 1) ||
+        !(r->base > 0) || !isfinite(r->base)) {
+        set_error("%s: rotary form out of range (rot_dim %d, head_dim %d, axes %d, pairing %d, order %d, per_axis %d, base %g)", who,
+                  r->rot_dim, head_dim, r->n_axes, r->pairing, r->order, r->per_axis, r->base);
+        return OFB_EINVAL;
+    }
+    if (r->per_axis && r->order != OFB_ROPE_BLOCKED) {
+        set_error("%s: per_axis frequencies need blocked sections", who);
+        return OFB_EINVAL;
+    }
+    const int pairs = r->rot_dim / 2;
+    int64_t sum = 0;
+    for (int x = 0; x < r->n_axes; x++) {
+        if (r->section[x] < 0) { set_error("%s: section %d is negative", who, x); return OFB_EINVAL; }
+        sum += r->section[x];
+        if (r->order == OFB_ROPE_DEALT && x && (int64_t)r->section[x] * r->n_axes > pairs + r->n_axes - 1 - x) {
+            set_error("%s: section %d (%d pairs) cannot be dealt from %d pairs over %d axes", who, x, r->section[x], pairs, r->n_axes);
+            return OFB_EINVAL;
+        }
+    }
+    if (sum != pairs) { set_error("%s: the sections have %lld pairs, rot_dim/2 is %d", who, (long long)sum, pairs); return OFB_EINVAL; }
+    a.rot = r->rot_dim;
+    // powers by repeated products: with 64 bits of mantissa 127 of them stay
+    // within 2^-56, below what the f64 result can hold, for one powl per call
+    const long double inv_pi = 0.318309886183790671537767526745028724L;
+    int x = 0, left = r->section[0];
+    long double f = inv_pi, step = powl(r->base, -1.0L / (r->per_axis && left ? left : pairs));
+    for (int i = 0; i < pairs; i++) {
+        if (r->order == OFB_ROPE_BLOCKED) {
+            while (!left) {
+                left = r->section[++x];
+                if (r->per_axis && left) f = inv_pi, step = powl(r->base, -1.0L / left);
+            }
+            left--;
+            a.axis[i] = (uint8_t)x;
+        } else {
+            const int y = i % r->n_axes;
+            a.axis[i] = (uint8_t)(i / r->n_axes < r->section[y] ? y : 0);
+        }
+        a.half_turns[i] = (double)f;
+        f *= step;
+    }
+    return OFB_OK;
+}
+
+template <typename IO, typename CT> static cudaError_t rope_launch(RopeArgs &a, bool vec, bool adjacent, cudaStream_t s) {
+    const int per_tok = (a.H + 2 * a.KVH) * (vec ? a.d / 16 : a.d - a.rot / 2);
+    // two items per thread where a token alone does not give them, at most 8 tokens (2 KB of cosines each)
+    int tpb = per_tok >= 2 * RP_THREADS ? 1 : 2 * RP_THREADS / (per_tok > 0 ? per_tok : 1);
+    if (tpb > 8) tpb = 8;
+    while (tpb > 1 && (a.T + tpb - 1) / tpb < 2 * sm_count()) tpb--;
+    a.tpb = tpb;
+    const size_t smem = (size_t)tpb * (a.rot / 2) * sizeof(float2) + (size_t)tpb * sizeof(int64_t);
+    const dim3 grid((a.T + tpb - 1) / tpb), block(RP_THREADS);
+    if (!vec) return launch_pdl(rope_any_kernel<IO, CT>, grid, block, smem, s, a, (int)adjacent);
+    return adjacent ? launch_pdl(rope_vec_kernel<IO, CT, true>, grid, block, smem, s, a)
+                    : launch_pdl(rope_vec_kernel<IO, CT, false>, grid, block, smem, s, a);
+}
+
+static bool row_ok(const void *p, int64_t stride) { return !misaligned(p, 16) && stride % 8 == 0; }
+
+}  // namespace ofb
+
+using namespace ofb;
+
+extern "C" int ofb_rope(const ofb_rope_config *rope, const void *x, int type, int n_tokens, int n_heads, int head_dim,
+                        int64_t x_stride, const int32_t *pos, int64_t pos_stride, void *out, int64_t out_stride,
+                        void *stream) {
+    if (!rope || n_tokens < 0 || n_heads < 1 || n_heads > 65536 || head_dim < 1 || head_dim > 1024 ||
+        (n_tokens && (!x || !pos || !out))) {
+        set_error("ofb_rope: bad arguments");
+        return OFB_EINVAL;
+    }
+    if (type != OFB_TYPE_F32 && !cache_type(type)) {
+        set_error("ofb_rope: type %d is not F32/BF16/F16", type);
+        return OFB_EUNSUPPORTED;
+    }
+    const int64_t width = (int64_t)n_heads * head_dim;
+    if ((n_tokens > 1 && (x_stride < width || out_stride < width || (rope->n_axes > 1 && pos_stride < n_tokens))) ||
+        (x == out && n_tokens > 1 && x_stride != out_stride) || misaligned(x, type_size(type)) ||
+        misaligned(out, type_size(type)) || misaligned(pos, 4)) {
+        set_error("ofb_rope: strides or alignment (x %lld, out %lld, pos %lld)", (long long)x_stride, (long long)out_stride,
+                  (long long)pos_stride);
+        return OFB_EINVAL;
+    }
+    RopeArgs a = {};
+    int st = rope_tables(rope, head_dim, "ofb_rope", a);
+    if (st != OFB_OK) return st;
+    if (!n_tokens) return OFB_OK;
+    a.T = n_tokens, a.H = n_heads, a.d = head_dim;
+    a.q = x, a.q_out = out, a.qs = x_stride, a.qos = out_stride, a.pos = pos, a.pos_stride = pos_stride;
+    const bool vec = head_dim % 16 == 0 && a.rot % 16 == 0 && row_ok(x, x_stride) && row_ok(out, out_stride);
+    const bool adj = rope->pairing == OFB_ROPE_ADJACENT;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const cudaError_t e = type == OFB_TYPE_F32    ? rope_launch<float, __nv_bfloat16>(a, vec, adj, s)
+                          : type == OFB_TYPE_BF16 ? rope_launch<__nv_bfloat16, __nv_bfloat16>(a, vec, adj, s)
+                                                  : rope_launch<__half, __half>(a, vec, adj, s);
+    return e == cudaSuccess ? OFB_OK : cuda_status(e, "ofb_rope launch");
+}
+
+extern "C" int ofb_rope_append(const ofb_kv_cache *cache, const ofb_rope_config *rope, int type, int n_tokens, int n_heads,
+                               const void *q, int64_t q_stride, const void *k, int64_t k_stride, const void *v,
+                               int64_t v_stride, const int32_t *pos, int64_t pos_stride, const int32_t *seq,
+                               const int32_t *index, const int32_t *number, void *q_out, int64_t q_out_stride,
+                               void *stream) {
+    int st = check_cache(cache, "ofb_rope_append");
+    if (st != OFB_OK) return st;
+    if (type != OFB_TYPE_F32 && type != cache->type) {
+        set_error("ofb_rope_append: type %d is neither F32 nor the cache's", type);
+        return OFB_EUNSUPPORTED;
+    }
+    if (n_tokens < 0 || n_heads < 0 || n_heads > 65536 ||
+        (n_tokens && (!k || !v || !seq || !index || (rope && !pos) || (q && (!q_out || n_heads < 1))))) {
+        set_error("ofb_rope_append: bad arguments");
+        return OFB_EINVAL;
+    }
+    const int d = cache->head_dim;
+    const int64_t qw = (int64_t)n_heads * d, kw = (int64_t)cache->n_kv_heads * d;
+    const size_t ts = type_size(type);
+    if ((n_tokens > 1 && ((q && (q_stride < qw || q_out_stride < qw)) || k_stride < kw || v_stride < kw ||
+                          (rope && rope->n_axes > 1 && pos_stride < n_tokens))) ||
+        (q && q == q_out && n_tokens > 1 && q_stride != q_out_stride) || misaligned(q, ts) || misaligned(q_out, ts) ||
+        misaligned(k, ts) || misaligned(v, ts) || misaligned(pos, 4) || misaligned(seq, 4) || misaligned(index, 4) ||
+        misaligned(number, 4)) {
+        set_error("ofb_rope_append: strides or alignment (q %lld, k %lld, v %lld, q_out %lld, pos %lld)", (long long)q_stride,
+                  (long long)k_stride, (long long)v_stride, (long long)q_out_stride, (long long)pos_stride);
+        return OFB_EINVAL;
+    }
+    RopeArgs a = {};
+    if (rope && (st = rope_tables(rope, d, "ofb_rope_append", a)) != OFB_OK) return st;
+    if (!n_tokens) return OFB_OK;
+    a.T = n_tokens, a.H = q ? n_heads : 0, a.KVH = cache->n_kv_heads, a.d = d;
+    a.n_pages = cache->n_pages, a.page_size = cache->page_size, a.n_seqs = cache->n_seqs, a.max_pages = cache->max_pages;
+    a.q = q, a.k = k, a.v = v, a.q_out = q_out, a.ck = cache->k, a.cv = cache->v;
+    a.qs = q_stride, a.ks = k_stride, a.vs = v_stride, a.qos = q_out_stride;
+    a.page_stride = cache_page_stride(cache), a.pos = pos, a.pos_stride = pos_stride;
+    a.seq = seq, a.index = index, a.number = number, a.table = cache->page_table;
+    a.weight = cache->weight, a.order = cache->order, a.errors = cache->errors;
+    const bool vec = a.rot % 16 == 0 && row_ok(k, k_stride) && row_ok(v, v_stride) &&
+                     (!q || (row_ok(q, q_stride) && row_ok(q_out, q_out_stride)));
+    const bool adj = rope && rope->pairing == OFB_ROPE_ADJACENT;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    const bool bf = cache->type == OFB_TYPE_BF16;
+    const cudaError_t e = type == OFB_TYPE_F32 ? (bf ? rope_launch<float, __nv_bfloat16>(a, vec, adj, s)
+                                                     : rope_launch<float, __half>(a, vec, adj, s))
+                          : bf                 ? rope_launch<__nv_bfloat16, __nv_bfloat16>(a, vec, adj, s)
+                                               : rope_launch<__half, __half>(a, vec, adj, s);
+    return e == cudaSuccess ? OFB_OK : cuda_status(e, "ofb_rope_append launch");
+}

@@ -10,6 +10,7 @@ Reference interfaces mirrored (ornith-flight, file:line):
   dequantize_slice     gguf_dequantize_expert_slice_from_buf  engine/src/gguf.c:652-711
   route                model_get_routing / inline router  engine/src/model.c:264-321, :1017-1049
   MoeLayer.forward     MoE block of model_forward         engine/src/model.c:992-1143
+  rope, rope_append, attn_decode   GQA attention of model_forward  engine/src/model.c:563-679
 """
 from __future__ import annotations
 
@@ -23,10 +24,14 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libornith_cuda.so")
 
 OK, EINVAL, ECUDA, ENOMEM, EUNSUPPORTED, ETOOLARGE = range(6)
-TYPE_F32, TYPE_F16, TYPE_Q4_K, TYPE_Q6_K = 0, 1, 12, 14
+TYPE_F32, TYPE_F16, TYPE_Q4_K, TYPE_Q6_K, TYPE_BF16 = 0, 1, 12, 14, 30
 OUT_F32, OUT_BF16 = 0, 1
 LAYOUT_CONTIGUOUS, LAYOUT_INTERLEAVED = 0, 1
 ROUTE_FORWARD, ROUTE_GET_ROUTING = 0, 1
+ROPE_HALVES, ROPE_ADJACENT = 0, 1
+ROPE_BLOCKED, ROPE_DEALT = 0, 1
+CACHE_EPAGE, CACHE_ELEN, CACHE_EINDEX = 1, 2, 4
+EVICT_MAX_LEN = 393216
 QK = 256
 BLOCK_BYTES = {TYPE_Q4_K: 144, TYPE_Q6_K: 210}
 
@@ -53,12 +58,34 @@ class GgufMoeLayer(ctypes.Structure):
     _fields_ = [("cfg", MoeConfig), ("weights", MoeWeights)]
 
 
+class RopeConfig(ctypes.Structure):
+    """ofb_rope_config: rotary positions with up to four axes. `section` gives
+    the pairs of each axis (their sum is rot_dim/2)."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("rot_dim", "pairing", "order", "n_axes", "per_axis")] + [
+        ("section", ctypes.c_int32 * 4), ("base", ctypes.c_double)]
+
+    def __init__(self, rot_dim: int, section=None, base: float = 10000.0, pairing: int = ROPE_HALVES,
+                 order: int = ROPE_BLOCKED, per_axis: bool = False):
+        section = [rot_dim // 2] if section is None else list(section)
+        if not 1 <= len(section) <= 4:
+            raise OfbError(EINVAL, f"RopeConfig: {len(section)} axes, 1 to 4 are possible")
+        super().__init__(rot_dim, pairing, order, len(section), int(per_axis), (ctypes.c_int32 * 4)(*section), base)
+
+
+class KvCacheStruct(ctypes.Structure):
+    """ofb_kv_cache."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("k", "v", "weight", "order", "page_table", "errors")] + [
+        ("page_stride", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in (
+            "type", "n_kv_heads", "head_dim", "page_size", "n_pages", "n_seqs", "max_pages")]
+
+
 def _load() -> ctypes.CDLL:
     if not os.path.exists(LIB_PATH):
         raise ImportError(f"{LIB_PATH} is not built; run `make -C {_HERE}` (or __graft_entry__.build())")
     lib = ctypes.CDLL(LIB_PATH)
     vp, u64, i32, sz = ctypes.c_void_p, ctypes.c_uint64, ctypes.c_int, ctypes.c_size_t
     cfgp, wp = ctypes.POINTER(MoeConfig), ctypes.POINTER(MoeWeights)
+    rp, kvp, i64 = ctypes.POINTER(RopeConfig), ctypes.POINTER(KvCacheStruct), ctypes.c_int64
     sig = {
         "ofb_status_string": (ctypes.c_char_p, [i32]),
         "ofb_last_error": (ctypes.c_char_p, []),
@@ -96,6 +123,12 @@ def _load() -> ctypes.CDLL:
         "ofb_gguf_upload": (i32, [vp, ctypes.c_char_p, vp, u64, vp]),
         "ofb_gguf_upload_moe_layer": (i32, [vp, i32, i32, vp, vp]),
         "ofb_gguf_free_moe_layer": (i32, [vp]),
+        "ofb_rope": (i32, [rp, vp, i32, i32, i32, i32, i64, vp, i64, vp, i64, vp]),
+        "ofb_rope_append": (i32, [kvp, rp, i32, i32, i32, vp, i64, vp, i64, vp, i64, vp, i64, vp, vp, vp, vp, i64, vp]),
+        "ofb_attn_scratch_size": (sz, [kvp, i32, i32, i32, i32]),
+        "ofb_attn_decode": (i32, [kvp, vp, i32, i64, i32, ctypes.c_float, vp, i32, i32, i32, vp, i64, vp, sz, vp]),
+        "ofb_kv_evict_scratch_size": (sz, [kvp, i32, i32]),
+        "ofb_kv_evict": (i32, [kvp, vp, i32, i32, i32, i32, vp, vp, vp, sz, vp]),
         "ofb_ep_group_create": (i32, [cfgp, i32, i32, i32, ctypes.POINTER(vp), vp]),
         "ofb_ep_group_connect": (i32, [vp, vp]),
         "ofb_ep_group_create_nccl": (i32, [cfgp, vp, i32, ctypes.POINTER(vp), vp]),
@@ -193,6 +226,205 @@ def sample(logits: torch.Tensor, temperature: float, r: float, stream=None) -> i
     tok = torch.empty(1, dtype=torch.int32, device=logits.device)
     _check(lib.ofb_sample(_ptr(logits), logits.numel(), temperature, r, _ptr(scratch), _ptr(tok), _stream(stream)))
     return int(tok.item())
+
+
+# ---- attention cache ----------------------------------------------------------
+# Each call runs on the device of its tensors, on `stream` or that device's
+# current stream. Tensors of other types, shapes, strides or devices than the
+# call takes raise OfbError (EINVAL) before anything is launched.
+
+_TYPE_OF = {torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16, torch.float16: TYPE_F16}
+
+
+def _need(ok: bool, what: str) -> None:
+    if not ok:
+        raise OfbError(EINVAL, what)
+
+
+def _ints(t: torch.Tensor, shape, device, name: str) -> int:
+    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous() or t.device != device:
+        raise OfbError(EINVAL, f"{name} must be contiguous int32 {tuple(shape)} on {device}")
+    return t.data_ptr()
+
+
+def _rows(t: torch.Tensor, shape, dtype, device, name: str) -> int:
+    """Elements from one row of t [rows, heads, head_dim] to the next; heads dense."""
+    if t.shape != shape or t.dtype != dtype or t.device != device:
+        raise OfbError(EINVAL, f"{name} must be {dtype} {tuple(shape)} on {device}")
+    st = t.stride()
+    if (st[2] != 1 and shape[2] > 1) or (st[1] != shape[2] and shape[1] > 1):
+        raise OfbError(EINVAL, f"{name}: the heads of a row must be consecutive")
+    return st[0]
+
+
+def _on(device: torch.device, stream, body):
+    """body() with `device` and `stream` current."""
+    if device.type != "cuda":
+        raise OfbError(EINVAL, "tensors must be on a CUDA device")
+    if stream is None and device.index == torch.cuda.current_device():
+        return body(torch.cuda.current_stream().cuda_stream)
+    with torch.cuda.device(device), torch.cuda.stream(stream):
+        return body(torch.cuda.current_stream().cuda_stream)
+
+
+class KvCache:
+    """One layer's paged cache (ofb_kv_cache). k, v: bf16 or fp16
+    [n_pages, kv heads, page, head_dim], a page dense (pages may lie further
+    apart, alike in both); weight f32 and order int32 [n_pages, kv heads, page];
+    page_table int32 [sequences, pages of a sequence]. The tensors stay the
+    caller's and are written in place by rope_append, attn_decode (weight) and
+    kv_evict."""
+
+    def __init__(self, k: torch.Tensor, v: torch.Tensor, page_table: torch.Tensor,
+                 weight: torch.Tensor | None = None, order: torch.Tensor | None = None):
+        _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.device == v.device,
+              "KvCache: k and v must have one 4-d shape, type and device")
+        _need(k.dtype in (torch.bfloat16, torch.float16), "KvCache: k and v must be bfloat16 or float16")
+        n, h, p, d = k.shape
+        _need(k.numel() > 0, "KvCache: empty k")
+        for t in (k, v):
+            _need(t[0].is_contiguous(), "KvCache: a page must be dense")
+        _need(n == 1 or k.stride(0) == v.stride(0), "KvCache: the pages of k and v must lie alike")
+        _need(page_table.dim() == 2 and page_table.numel() > 0, "KvCache: page_table must be [sequences, pages]")
+        self.device = k.device
+        table = _ints(page_table, page_table.shape, k.device, "KvCache: page_table")
+        for t, dt, name in ((weight, torch.float32, "weight"), (order, torch.int32, "order")):
+            _need(t is None or (t.shape == k.shape[:3] and t.dtype == dt and t.is_contiguous() and t.device == k.device),
+                  f"KvCache: {name} must be contiguous {dt} [n_pages, kv heads, page] beside k")
+        self.k, self.v, self.page_table, self.weight, self.order = k, v, page_table, weight, order
+        self.errors = torch.zeros(1, dtype=torch.int32, device=k.device)
+        self.dtype, self.n_kv_heads, self.head_dim, self.n_seqs = k.dtype, h, d, page_table.shape[0]
+        self.struct = KvCacheStruct(k.data_ptr(), v.data_ptr(), _ptr(weight), _ptr(order), table, self.errors.data_ptr(),
+                                    k.stride(0) if n > 1 else 0, _TYPE_OF[k.dtype], h, d, p, n, *page_table.shape)
+        self._ref = ctypes.byref(self.struct)
+
+    def device_errors(self) -> int:
+        """CACHE_E* bits that calls on this cache have met since the last call
+        (0: none). Waits for the device."""
+        bits = int(self.errors.item())
+        self.errors.zero_()
+        return bits
+
+
+def rope(x: torch.Tensor, pos: torch.Tensor, cfg: RopeConfig, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """x [tokens, heads, head_dim] (f32, bf16 or fp16) turned by its tokens'
+    positions pos int32 [axes, tokens] (ofb_rope); out may be x."""
+    _need(x.dim() == 3 and x.dtype in _TYPE_OF, "rope: x must be f32, bf16 or fp16 [tokens, heads, head_dim]")
+    T, H, d = shape = x.shape
+    xs = _rows(x, shape, x.dtype, x.device, "rope: x")
+    p = _ints(pos, (cfg.n_axes, T), x.device, "rope: pos")
+
+    def body(s):
+        y = torch.empty(shape, dtype=x.dtype, device=x.device) if out is None else out
+        ys = _rows(y, shape, x.dtype, x.device, "rope: out")
+        _check(lib.ofb_rope(ctypes.byref(cfg), x.data_ptr(), _TYPE_OF[x.dtype], T, H, d, xs, p, T, y.data_ptr(), ys, s))
+        return y
+
+    return _on(x.device, stream, body)
+
+
+def rope_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, seq: torch.Tensor, index: torch.Tensor,
+                number: torch.Tensor | None = None, q: torch.Tensor | None = None, pos: torch.Tensor | None = None,
+                rope: RopeConfig | None = None, q_out: torch.Tensor | None = None, stream=None) -> torch.Tensor | None:
+    """New tokens enter the cache (ofb_rope_append): k, v [tokens, kv heads,
+    head_dim] become entry index[t] of sequence seq[t] (-1: padding), k turned
+    by `rope` at pos int32 [axes, tokens] when given, with weight 0 and order
+    number[t] (index[t] when None). Returns the turned q [tokens, heads,
+    head_dim] (in q_out, which may be q), None without q."""
+    _need(k.dim() == 3, "rope_append: k must be [tokens, kv heads, head_dim]")
+    T, d, dev, dt = k.shape[0], cache.head_dim, cache.device, k.dtype
+    _need(dt in (torch.float32, cache.dtype), "rope_append: k, v and q must be f32 or of the cache's type")
+    shape = (T, cache.n_kv_heads, d)
+    ks, vs = _rows(k, shape, dt, dev, "rope_append: k"), _rows(v, shape, dt, dev, "rope_append: v")
+    _need((rope is None) == (pos is None), "rope_append: rope and pos go together")
+    pp = None if rope is None else _ints(pos, (rope.n_axes, T), dev, "rope_append: pos")
+    sp, ip = _ints(seq, (T,), dev, "rope_append: seq"), _ints(index, (T,), dev, "rope_append: index")
+    np_ = None if number is None else _ints(number, (T,), dev, "rope_append: number")
+    H = qs = 0
+    if q is not None:
+        _need(q.dim() == 3, "rope_append: q must be [tokens, heads, head_dim]")
+        H = q.shape[1]
+        qs = _rows(q, (T, H, d), dt, dev, "rope_append: q")
+
+    def body(s):
+        y, ys = None, 0
+        if q is not None:
+            y = torch.empty((T, H, d), dtype=dt, device=dev) if q_out is None else q_out
+            ys = _rows(y, (T, H, d), dt, dev, "rope_append: q_out")
+        _check(lib.ofb_rope_append(cache._ref, None if rope is None else ctypes.byref(rope), _TYPE_OF[dt], T, H, _ptr(q), qs,
+                                   k.data_ptr(), ks, v.data_ptr(), vs, pp, T, sp, ip, np_, _ptr(y), ys, s))
+        return y
+
+    return _on(dev, stream, body)
+
+
+def _scratch(size: int, device) -> torch.Tensor:
+    if not size:
+        raise OfbError(EINVAL, lib.ofb_last_error().decode())
+    return torch.empty(size, dtype=torch.uint8, device=device)
+
+
+def attn_scratch(cache: KvCache, n_heads: int, n_seqs: int, max_len: int = 0, accumulate: bool = False) -> torch.Tensor:
+    """Scratch for attn_decode calls of up to these sizes that do not overlap."""
+    with torch.cuda.device(cache.device):
+        return _scratch(lib.ofb_attn_scratch_size(cache._ref, n_heads, n_seqs, max_len, int(accumulate)), cache.device)
+
+
+def attn_decode(cache: KvCache, q: torch.Tensor, lens: torch.Tensor, scale: float | None = None, max_len: int = 0,
+                accumulate: bool = False, out: torch.Tensor | None = None, scratch: torch.Tensor | None = None,
+                stream=None) -> torch.Tensor:
+    """Attention of one new token per sequence, q [sequences, heads, head_dim]
+    (f32 or the cache's type), over the first lens[b] entries of sequence b
+    (ofb_attn_decode). scale: 1/sqrt(head_dim) by default; max_len: a bound on
+    lens (0: the page table's reach); accumulate: add the weights to cache.weight."""
+    _need(q.dim() == 3, "attn_decode: q must be [sequences, heads, head_dim]")
+    dev, d = cache.device, cache.head_dim
+    B, H = q.shape[0], q.shape[1]
+    shape = (B, H, d)
+    _need(q.dtype in (torch.float32, cache.dtype), "attn_decode: q must be f32 or of the cache's type")
+    qs, lp = _rows(q, shape, q.dtype, dev, "attn_decode: q"), _ints(lens, (B,), dev, "attn_decode: lens")
+
+    def body(s):
+        w = attn_scratch(cache, H, B, max_len, accumulate) if scratch is None else scratch
+        _need(w.device == dev and w.is_contiguous(), "attn_decode: scratch must be contiguous beside the cache")
+        y = torch.empty(shape, dtype=q.dtype, device=dev) if out is None else out
+        ys = _rows(y, shape, q.dtype, dev, "attn_decode: out")
+        _check(lib.ofb_attn_decode(cache._ref, q.data_ptr(), _TYPE_OF[q.dtype], qs, H, d ** -0.5 if scale is None else scale,
+                                   lp, B, max_len, int(accumulate), y.data_ptr(), ys, w.data_ptr(),
+                                   w.numel() * w.element_size(), s))
+        return y
+
+    return _on(dev, stream, body)
+
+
+def evict_scratch(cache: KvCache, n_seqs: int, keep: int) -> torch.Tensor:
+    """Scratch for kv_evict calls of up to these sizes that do not overlap."""
+    return _scratch(lib.ofb_kv_evict_scratch_size(cache._ref, n_seqs, keep), cache.device)
+
+
+def kv_evict(cache: KvCache, lens: torch.Tensor, keep: int, recent: int = 0, max_len: int = 0,
+             kept: torch.Tensor | None = None, lens_out: torch.Tensor | None = None, scratch: torch.Tensor | None = None,
+             stream=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Brings each sequence down to `keep` entries per kv head: the `recent`
+    youngest and then the heaviest (ofb_kv_evict). Returns (kept, lens_out):
+    int32 [sequences, kv heads, keep], the place each entry comes from (-1
+    behind the end), and the new lengths."""
+    dev = cache.device
+    _need(lens.dim() == 1, "kv_evict: lens must be [sequences]")
+    B = lens.shape[0]
+    lp = _ints(lens, (B,), dev, "kv_evict: lens")
+
+    def body(s):
+        w = evict_scratch(cache, B, keep) if scratch is None else scratch
+        _need(w.device == dev and w.is_contiguous(), "kv_evict: scratch must be contiguous beside the cache")
+        shape = (B, cache.n_kv_heads, keep)
+        src = torch.empty(shape, dtype=torch.int32, device=dev) if kept is None else kept
+        new = torch.empty(B, dtype=torch.int32, device=dev) if lens_out is None else lens_out
+        _check(lib.ofb_kv_evict(cache._ref, lp, B, max_len, keep, recent, _ints(new, (B,), dev, "kv_evict: lens_out"),
+                                _ints(src, shape, dev, "kv_evict: kept"), w.data_ptr(), w.numel() * w.element_size(), s))
+        return src, new
+
+    return _on(dev, stream, body)
 
 
 # ---- synthetic inputs ---------------------------------------------------------
