@@ -16,7 +16,8 @@
 namespace ofb {
 
 constexpr int AJ_THREADS = 256;
-constexpr int AJ_CHUNK = 512;  // entries of one weight CTA
+constexpr int AJ_CHUNK = 512;   // entries of one weight CTA
+constexpr int AJ_MAX_CTAS = 1024;  // of the split kernel
 
 struct AttnJoinArgs {
     AttnArgs a;
@@ -49,14 +50,15 @@ __device__ __forceinline__ float2 warp_ml(const AttnJoinArgs &j, const PartRange
     float l = 0.0f;
     for (int i = lane; i < n; i += 32) {
         const float2 e = j.a.part_ml[pr.slot(i) * ATT_R + r];
-        l += exp2f(e.x - ref) * e.y;
+        l += exp2_fast(e.x - ref) * e.y;
     }
     return make_float2(ref, warp_sum(l));
 }
 
 template <typename IO> __global__ void __launch_bounds__(AJ_THREADS) attn_join_kernel(const __grid_constant__ AttnJoinArgs j) {
     __shared__ float acc[AJ_THREADS / 32][256 + 4];
-    __shared__ float2 ml[128];
+    __shared__ float2 ml[AJ_MAX_CTAS];  // join: (weight, -) of each part; weights: (maximum, 1 / sum) of a head
+    __shared__ float red[2][AJ_THREADS / 32];
     const AttnArgs &a = j.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_wait();
@@ -68,22 +70,44 @@ template <typename IO> __global__ void __launch_bounds__(AJ_THREADS) attn_join_k
         const PartRange pr = part_range(j, b, kvh * a.NB + g / ATT_R, nt);
         if (pr.c0 == pr.c1) return;
         const int r = g % ATT_R, n = (int)(pr.c1 - pr.c0) + 1;
-        const float2 e = warp_ml(j, pr, r, lane);
+        // the parts' weights 2^(m_i - M) and the sum of exponentials, by all threads
+        float m = -INFINITY, l = 0.0f;
+        for (int i = tid; i < n; i += AJ_THREADS) {
+            ml[i] = a.part_ml[pr.slot(i) * ATT_R + r];
+            m = fmaxf(m, ml[i].x);
+        }
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (lane == 0) red[0][warp] = m;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < AJ_THREADS / 32; w++) m = fmaxf(m, red[0][w]);
+        const float ref = m == -INFINITY ? 0.0f : m;
+        for (int i = tid; i < n; i += AJ_THREADS) {
+            const float f = exp2_fast(ml[i].x - ref);
+            l += f * ml[i].y;
+            ml[i].x = f;
+        }
+        l = warp_sum(l);
+        if (lane == 0) red[1][warp] = l;
+        __syncthreads();
+        l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < AJ_THREADS / 32; w++) l += red[1][w];
         for (int x0 = 0; x0 < j.d; x0 += 128) {
             const int x = x0 + lane * 4;
             if (x >= j.d) continue;
             float4 s = make_float4(0, 0, 0, 0);
-#pragma unroll 4
+#pragma unroll 8
             for (int i = warp; i < n; i += AJ_THREADS / 32) {
-                const int64_t p = pr.slot(i) * ATT_R + r;
-                const float f = exp2f(a.part_ml[p].x - e.x);
-                const float4 y = *reinterpret_cast<const float4 *>(a.part_o + p * j.d + x);
+                const float f = ml[i].x;
+                const float4 y = *reinterpret_cast<const float4 *>(a.part_o + (pr.slot(i) * ATT_R + r) * j.d + x);
                 s.x += f * y.x, s.y += f * y.y, s.z += f * y.z, s.w += f * y.w;
             }
             *reinterpret_cast<float4 *>(&acc[warp][x]) = s;
         }
         __syncthreads();
-        const float inv = e.y > 0.0f || e.y != e.y ? 1.0f / e.y : 0.0f;
+        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
         for (int x = tid; x < j.d; x += AJ_THREADS) {
             float s = 0.0f;
 #pragma unroll
@@ -112,7 +136,7 @@ template <typename IO> __global__ void __launch_bounds__(AJ_THREADS) attn_join_k
             const float2 e = ml[g];
 #pragma unroll
             for (int k = 0; k < AJ_CHUNK / AJ_THREADS; k++)
-                if (i0 + k * AJ_THREADS + tid < len) add[k] += exp2f(z[k * AJ_THREADS] - e.x) * e.y;
+                if (i0 + k * AJ_THREADS + tid < len) add[k] += exp2_fast(z[k * AJ_THREADS] - e.x) * e.y;
         }
         __syncthreads();
     }
@@ -120,15 +144,18 @@ template <typename IO> __global__ void __launch_bounds__(AJ_THREADS) attn_join_k
     for (int k = 0; k < AJ_CHUNK / AJ_THREADS; k++) {
         const int i = i0 + k * AJ_THREADS + tid;
         if (i >= len) continue;
-        const int col = i / a.page_size, page = a.table[(int64_t)b * a.max_pages + col];
+        const int col = a.page.div(i), page = a.table[(int64_t)b * a.max_pages + col];
         if (page < 0 || page >= a.n_pages) continue;
         a.weight[((int64_t)page * a.KVH + kvh) * a.page_size + (i - col * a.page_size)] += add[k];
     }
 }
 
+constexpr int ATT_SHORT = 4;
+
 struct AttnPlan {
     AttnVariant v;
     int max_len, ctas, NB;
+    int cluster;  // CTAs per (sequence, pass) that join by themselves, or 0: runs and a second launch
     int64_t z_stride;
     size_t prefix, ml, part_o, part_ml, z, total;
 };
@@ -162,7 +189,16 @@ static int attn_plan(const ofb_kv_cache *c, int n_heads, int n_seqs, int max_len
     }
     p.NB = (n_heads / c->n_kv_heads + ATT_R - 1) / ATT_R;
     const int64_t runs = (tiles * n_seqs * c->n_kv_heads * p.NB + ATT_W - 1) / ATT_W;
-    const int most = sm_count() * p.v.ctas;
+    const int most = sm_count() * p.v.ctas < AJ_MAX_CTAS ? sm_count() * p.v.ctas : AJ_MAX_CTAS;
+    // Short sequences: as many CTAs as give each warp ATT_SHORT tiles at most,
+    // where all of them have room at once. Weights need all of a kv head's
+    // query heads in one pass.
+    p.cluster = 0;
+    if (!accumulate || p.NB == 1) {
+        int n = 1;
+        while (n < 8 && tiles > n * ATT_W) n *= 2;
+        if (tiles <= (int64_t)n * ATT_W * ATT_SHORT && (int64_t)n_seqs * c->n_kv_heads * p.NB * n <= most) p.cluster = n;
+    }
     p.ctas = runs < 1 ? 1 : runs < most ? (int)runs : most;
     p.z_stride = tiles * ATT_TILE;
     size_t at = 0;
@@ -215,6 +251,7 @@ extern "C" int ofb_attn_decode(const ofb_kv_cache *cache, const void *q, int typ
     a.page_stride = cache_page_stride(cache), a.q_stride = q_stride, a.out_stride = out_stride;
     a.B = n_seqs, a.KVH = cache->n_kv_heads, a.G = n_heads / a.KVH, a.NB = p.NB, a.H = n_heads;
     a.page_size = cache->page_size, a.max_pages = cache->max_pages, a.n_pages = cache->n_pages, a.max_len = p.max_len;
+    a.page = fast_div(a.page_size), a.tiled = a.page_size % ATT_TILE == 0;
     a.scale = scale * 1.4426950408889634f;
     a.errors = cache->errors;
     a.prefix = reinterpret_cast<int *>(w + p.prefix), a.ml = reinterpret_cast<float2 *>(w + p.ml);
@@ -228,12 +265,20 @@ extern "C" int ofb_attn_decode(const ofb_kv_cache *cache, const void *q, int typ
     if (blocks > INT32_MAX) { set_error("ofb_attn_decode: too many weight blocks"); return OFB_ETOOLARGE; }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     // a raised shared-memory limit per kernel and device
-    static size_t attr[20][64];
-    const int vi = (cache->head_dim == 64 ? 0 : cache->head_dim == 96 ? 1 : cache->head_dim == 128 ? 2 : cache->head_dim == 192 ? 3 : 4) * 4 +
-                   (cache->type == OFB_TYPE_BF16 ? 2 : 0) + (type == OFB_TYPE_F32 ? 1 : 0);
-    cudaError_t e = ensure_dyn_smem(p.v.kernel, p.v.smem, attr[vi]);
+    static size_t attr[40][64];
+    const int vi = (cache->head_dim == 64 ? 0 : cache->head_dim == 96 ? 1 : cache->head_dim == 128 ? 2 : cache->head_dim == 192 ? 3 : 4) * 8 +
+                   (cache->type == OFB_TYPE_BF16 ? 4 : 0) + (type == OFB_TYPE_F32 ? 2 : 0);
+    if (p.cluster) {
+        cudaError_t e = ensure_dyn_smem(p.v.cluster, p.v.head, attr[vi + 1]);
+        if (e != cudaSuccess) return cuda_status(e, "ofb_attn_decode smem attribute");
+        e = launch_pdl_cluster(p.v.cluster, dim3((unsigned)(n_seqs * a.KVH * a.NB * p.cluster)), dim3(ATT_W * 32), p.cluster,
+                               p.v.head, s, a);
+        return e == cudaSuccess ? OFB_OK : cuda_status(e, "ofb_attn_decode launch");
+    }
+    const size_t smem = p.v.head + (size_t)n_seqs * 4 + (n_seqs + 3) / 4 * 4;
+    cudaError_t e = ensure_dyn_smem(p.v.run, smem, attr[vi]);
     if (e != cudaSuccess) return cuda_status(e, "ofb_attn_decode smem attribute");
-    e = launch_pdl(p.v.kernel, dim3(p.ctas), dim3(ATT_W * 32), p.v.smem, s, a);
+    e = launch_pdl(p.v.run, dim3(p.ctas), dim3(ATT_W * 32), smem, s, a);
     if (e != cudaSuccess) return cuda_status(e, "ofb_attn_decode launch");
     if (p.ctas == 1 && !accumulate) return OFB_OK;  // every part is whole
     const dim3 grid((unsigned)blocks), block(AJ_THREADS);

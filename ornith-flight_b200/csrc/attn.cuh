@@ -14,9 +14,14 @@
 //
 // Inside a CTA each warp takes every fourth tile of a part by itself: its own
 // ring of tiles in shared memory filled by 16-byte asynchronous copies (page
-// by page, ATT_S - 1 tiles ahead and across parts), its own running maximum
-// and sums, no barrier but one merge at the end of a part. Rows are padded by
-// 16 bytes, so that ldmatrix meets no bank twice.
+// by page, ATT_S - 1 tiles ahead and across parts, the page numbers one tile
+// before that), its own running maximum and sums, no barrier but one merge at
+// the end of a part. Rows are padded by 16 bytes, so that ldmatrix meets no
+// bank twice.
+//
+// Short sequences take a cluster of CTAs each instead of runs (CLUSTER): its
+// CTAs share the tiles of one (sequence, kv head) and join their sums through
+// distributed shared memory, which saves the second launch.
 //
 // The products run on mma.sync m16n8k16 (bf16 or fp16, f32 sums): 16 rows of A
 // by 8 entries or 8 output columns. Query heads of one kv head fill 8 rows at
@@ -28,14 +33,19 @@
 //   probability: bf16 hi + low (16 bits) or, for f32 output, + lowest (24
 //     bits, a second mma); fp16 hi + low of 2^14 p (22 bits).
 // A row's parts end in the same thread (accumulators c0, c1 and c2, c3), which
-// adds them in f32. Each tile's product starts at zero and is added to the
-// running sum by an FFMA, since the tensor core's own accumulation cuts off
-// where an addition rounds.
+// adds them in f32. With f32 output each tile's product starts at zero and is
+// added to the running sum by an FFMA, since the tensor core's own accumulation
+// cuts off where an addition rounds; with 16-bit output, whose own rounding is
+// coarser than that by far, the tensor core accumulates up to head_dim 128.
 #pragma once
+#include <cooperative_groups.h>
+
 #include <type_traits>
 
 #include "async.cuh"
 #include "kv_cache.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace ofb {
 
@@ -50,7 +60,9 @@ struct AttnArgs {
     const int32_t *table, *lens;
     int64_t page_stride, q_stride, out_stride;
     int B, KVH, G, NB, H;  // NB: passes of at most ATT_R heads per kv head
+    FastDiv page;  // by page_size
     int page_size, max_pages, n_pages, max_len;
+    int tiled;        // page_size is a multiple of ATT_TILE: a tile lies in one page
     float scale;      // times log2(e)
     uint32_t *errors;
     // scratch
@@ -63,6 +75,11 @@ struct AttnArgs {
     float *weight;
 };
 
+__device__ __forceinline__ float exp2_fast(float x) {  // 2 steps at most; below 2^-126 it gives 0
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 // How many entries of sequence b are attended to.
 __device__ __forceinline__ int attn_len(const AttnArgs &a, int b) { return min(max(a.lens[b], 0), a.max_len); }
 // Tiles per CTA when `total` tiles are dealt to `ctas` CTAs: at least one per
@@ -78,9 +95,13 @@ template <int D> struct AttnShape {
     static constexpr int S = D <= 64 ? 5 : D <= 96 ? 4 : D <= 128 ? 3 : D <= 192 ? 4 : 3;  // ring slots
     static constexpr int CTAS = D <= 128 ? 2 : 1;            // per SM
     static constexpr int RING = ATT_W * S * TILE_BYTES;
-    static constexpr int SMEM = RING + ATT_W * ATT_R * 8 + (ATT_MAX_SEQS + 1) * 4;
+    // behind the ring: the warps' and the CTA's (maximum, sum), then per sequence
+    // the tiles before it and the entries of its last tile
+    static constexpr int HEAD = RING + (ATT_W + 2) * ATT_R * 8;
+    static constexpr int smem(int B) { return HEAD + (B + 1) * 4 + (B + 3) / 4 * 4; }
     static_assert(TILE_BYTES >= ATT_R * (D + 4) * 4, "a warp's sums must fit one ring slot");
-    static_assert(CTAS * (SMEM + 1536) <= 228 * 1024, "shared memory of an SM");
+    static_assert(CTAS * (smem(512) + 1536) <= 228 * 1024, "shared memory of an SM");
+    static_assert(smem(ATT_MAX_SEQS) + 1536 <= 227 * 1024, "shared memory of a CTA");
 };
 
 template <typename T> struct Mma;
@@ -116,25 +137,45 @@ __device__ __forceinline__ void cp16(uint32_t dst, const void *src, int bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
+template <typename T> __device__ __forceinline__ uint32_t pack2(float x, float y);  // x in the low half
+template <> __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float x, float y) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+    return r;
+}
+template <> __device__ __forceinline__ uint32_t pack2<__half>(float x, float y) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(y), "f"(x));
+    return r;
+}
+template <typename T> __device__ __forceinline__ float2 unpack2(uint32_t p);
+template <> __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t p) {
+    return make_float2(__uint_as_float(p << 16), __uint_as_float(p & 0xffff0000u));
+}
+template <> __device__ __forceinline__ float2 unpack2<__half>(uint32_t p) {
+    __half2 h;
+    memcpy(&h, &p, 4);
+    return __half22float2(h);
+}
 // Splits (x, y) into parts of T: p[i] holds part i of x (low half) and y.
 template <typename T, int N> __device__ __forceinline__ void split2(float x, float y, uint32_t (&p)[N]) {
 #pragma unroll
     for (int i = 0; i < N; i++) {
-        const T a = from_f32<T>(x), b = from_f32<T>(y);
-        uint16_t ua, ub;
-        memcpy(&ua, &a, 2);
-        memcpy(&ub, &b, 2);
-        p[i] = ua | ((uint32_t)ub << 16);
-        if (i + 1 < N) x -= to_f32(a), y -= to_f32(b);
+        p[i] = pack2<T>(x, y);
+        if (i + 1 < N) {
+            const float2 f = unpack2<T>(p[i]);
+            x -= f.x, y -= f.y;
+        }
     }
 }
 
-// A part: tiles [t, end) of (sequence b, pass vh) within this CTA's run.
+// A part: tiles [t, end) of (sequence b, pass vh), of nt tiles that hold len
+// entries.
 struct AttnPart {
-    int b, vh, t, end, nt;
+    int b, vh, t, end, nt, len;
 };
 // The part that begins at tile `f` of the row of all tiles, cut at f1.
-__device__ __forceinline__ AttnPart attn_part(const int *prefix, int B, int nvh, long long f, long long f1) {
+__device__ __forceinline__ AttnPart attn_part(const int *prefix, const uint8_t *last, int B, int nvh, long long f, long long f1) {
     int lo = 0, hi = B - 1;  // the last sequence that begins at or before f (and has tiles)
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -144,6 +185,7 @@ __device__ __forceinline__ AttnPart attn_part(const int *prefix, int B, int nvh,
     AttnPart p;
     p.b = lo;
     p.nt = prefix[lo + 1] - prefix[lo];
+    p.len = (p.nt - 1) * ATT_TILE + last[lo];
     const long long r = f - (long long)prefix[lo] * nvh;
     p.vh = (int)(r / p.nt);
     p.t = (int)(r - (long long)p.vh * p.nt);
@@ -152,107 +194,145 @@ __device__ __forceinline__ AttnPart attn_part(const int *prefix, int B, int nvh,
     return p;
 }
 
-template <int D, typename CT, typename IO>
+template <int D, typename CT, typename IO, bool CLUSTER>
 __global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_kernel(const __grid_constant__ AttnArgs a) {
     using SH = AttnShape<D>;
-    constexpr bool F32 = sizeof(IO) == 4, BF = sizeof(CT) == 2 && std::is_same<CT, __nv_bfloat16>::value;
+    constexpr bool F32 = sizeof(IO) == 4, BF = std::is_same<CT, __nv_bfloat16>::value;
     constexpr int NQ = F32 ? (BF ? 3 : 2) : 1;       // parts of a query
     constexpr int NP = BF && F32 ? 3 : 2;            // parts of a probability
     constexpr float PSCALE = BF ? 1.0f : 16384.0f;   // fp16 holds 2^14 p
-    constexpr int KS = D / 16;
+    constexpr bool DIRECT = !F32 && D <= 128;        // the tensor core accumulates (registers allow no more)
+    constexpr int NO = DIRECT ? 4 : 2;               // accumulators of 8 columns
+    constexpr int KS = D / 16, CH = D / 8;           // k steps; 16-byte chunks of a row
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c2 = (lane & 3) * 2;
     uint8_t *ring = smem + warp * SH::S * SH::TILE_BYTES;
     float2 *mml = reinterpret_cast<float2 *>(smem + SH::RING);  // [W][R]
-    int *prefix = reinterpret_cast<int *>(mml + ATT_W * ATT_R);
+    float2 *cml = mml + ATT_W * ATT_R;                          // [2][R]: this CTA's, the cluster's
+    int *prefix = reinterpret_cast<int *>(smem + SH::HEAD);     // [B + 1]
+    uint8_t *last = reinterpret_cast<uint8_t *>(prefix + a.B + 1);
     __shared__ uint32_t valid[ATT_W][8];  // per ring slot: which of the 16 entries are there
     __shared__ int wsum[ATT_W];
     __shared__ float *mo[ATT_W];  // each warp's sums at the end of a part, [R][D + 4]
+    __shared__ int mo_at;         // CLUSTER: mo[0] as an offset, for the other CTAs
+    cg::cluster_group cl = cg::this_cluster();
 
     pdl_wait();
     pdl_trigger();
 
-    // tiles before each sequence; every CTA forms them for itself
-    for (int base = 0; base < a.B; base += ATT_W * 32) {
-        const int b = base + tid;
-        int n = 0;
-        if (b < a.B) {
-            if (a.lens[b] > a.max_len && blockIdx.x == 0) report(a.errors, OFB_CACHE_ELEN);
-            n = (attn_len(a, b) + ATT_TILE - 1) / ATT_TILE;
-        }
-        int s = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, s, o);
-            if (lane >= o) s += u;
-        }
-        if (lane == 31) wsum[warp] = s;
-        if (!base && !tid) prefix[0] = 0;
-        __syncthreads();
-        int before = prefix[base];
-        for (int w = 0; w < warp; w++) before += wsum[w];
-        if (b < a.B) prefix[b + 1] = before + s;
-        __syncthreads();
-    }
-    if (blockIdx.x == 0)
-        for (int b = tid; b <= a.B; b += ATT_W * 32) a.prefix[b] = prefix[b];
-    // sequences without entries: zeros
-    for (int b = blockIdx.x; b < a.B; b += gridDim.x)
-        if (prefix[b + 1] == prefix[b])
-            for (int i = tid; i < a.H * D; i += ATT_W * 32) static_cast<IO *>(a.out)[b * a.out_stride + i] = from_f32<IO>(0.0f);
-
     const int nvh = a.KVH * a.NB;
-    const long long total = (long long)prefix[a.B] * nvh, run = attn_run(total, gridDim.x);
-    const long long f0 = blockIdx.x * run, f1 = min(total, f0 + run);
-    if (f0 >= f1) return;
+    long long f0 = 0, f1 = 1;
+    AttnPart first;
+    if constexpr (CLUSTER) {
+        const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank(), u = blockIdx.x / C;
+        first.b = u / nvh;
+        first.vh = u - first.b * nvh;
+        if (a.lens[first.b] > a.max_len && first.vh == 0 && rank == 0 && tid == 0) report(a.errors, OFB_CACHE_ELEN);
+        first.len = attn_len(a, first.b);
+        first.nt = (first.len + ATT_TILE - 1) / ATT_TILE;
+        first.t = (int)((long long)rank * first.nt / C);
+        first.end = (int)((long long)(rank + 1) * first.nt / C);
+    } else {
+        // tiles before each sequence; every CTA forms them for itself
+        for (int base = 0; base < a.B; base += ATT_W * 32) {
+            const int b = base + tid;
+            int n = 0;
+            if (b < a.B) {
+                const int len = attn_len(a, b);
+                if (a.lens[b] > a.max_len && blockIdx.x == 0) report(a.errors, OFB_CACHE_ELEN);
+                n = (len + ATT_TILE - 1) / ATT_TILE;
+                last[b] = (uint8_t)(len - (n - 1) * ATT_TILE);
+            }
+            int s = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, s, o);
+                if (lane >= o) s += u;
+            }
+            if (lane == 31) wsum[warp] = s;
+            if (!base && !tid) prefix[0] = 0;
+            __syncthreads();
+            int before = prefix[base];
+            for (int w = 0; w < warp; w++) before += wsum[w];
+            if (b < a.B) prefix[b + 1] = before + s;
+            __syncthreads();
+        }
+        if (blockIdx.x == 0)
+            for (int b = tid; b <= a.B; b += ATT_W * 32) a.prefix[b] = prefix[b];
+        // sequences without entries: zeros
+        for (int b = blockIdx.x; b < a.B; b += gridDim.x)
+            if (prefix[b + 1] == prefix[b])
+                for (int i = tid; i < a.H * D; i += ATT_W * 32) static_cast<IO *>(a.out)[b * a.out_stride + i] = from_f32<IO>(0.0f);
+        const long long total = (long long)prefix[a.B] * nvh, run = attn_run(total, gridDim.x);
+        f0 = blockIdx.x * run, f1 = min(total, f0 + run);
+        if (f0 >= f1) return;
+        first = attn_part(prefix, last, a.B, nvh, f0, f1);
+    }
 
     const uint32_t ring_s = ax::smem_u32(ring);
-    // Copies tile t of part p into ring slot `slot`; lanes 0..15 find the rows.
-    auto load = [&](const AttnPart &p, int t, int slot) {
-        const int i = t * ATT_TILE + (lane & 15), len = attn_len(a, p.b);
-        int64_t off = -1;
-        if (i < len) {
-            const int col = i / a.page_size, page = a.table[(int64_t)p.b * a.max_pages + col];
-            if (page >= 0 && page < a.n_pages)
-                off = page * a.page_stride + ((int64_t)(p.vh / a.NB) * a.page_size + (i - col * a.page_size)) * D;
-            else report(a.errors, OFB_CACHE_EPAGE);
-        }
-        const uint32_t mask = __ballot_sync(0xffffffffu, off >= 0);
-        if (lane == 0) valid[warp][slot] = mask & 0xffffu;
-        const uint32_t dst = ring_s + slot * SH::TILE_BYTES;
-        constexpr int CH = D / 8;  // 16-byte chunks of a row
-#pragma unroll
-        for (int j = 0; j < ATT_TILE * CH / 32; j++) {
-            const int c = j * 32 + lane, r = c / CH, x = c - r * CH;
-            const int64_t o = __shfl_sync(0xffffffffu, off, r);
-            const int64_t e = o < 0 ? 0 : o + x * 8;
-            const int n = o < 0 ? 0 : 16;
-            cp16(dst + r * SH::PITCH + x * 16, static_cast<const CT *>(a.k) + e, n);
-            cp16(dst + (ATT_TILE + r) * SH::PITCH + x * 16, static_cast<const CT *>(a.v) + e, n);
-        }
-    };
-
-    // the part and tile that the ring is filled from, ahead of the one computed
-    AttnPart lp = attn_part(prefix, a.B, nvh, f0, f1);
+    // The tile that the ring is filled with next: its part, number, and its
+    // rows' entries (lanes 0..15) with the page numbers already asked for.
+    AttnPart lp = first;
     long long lf = f0;
-    int lt = lp.t + warp;
+    int lt = lp.t + warp, l_entry = 0, l_page = -1;
     bool more = true;
-    auto fill = [&](int slot) {
+    auto look_up = [&]() {
         while (more && lt >= lp.end) {
             lf += lp.end - lp.t;
-            if (lf >= f1) more = false;
-            else lp = attn_part(prefix, a.B, nvh, lf, f1), lt = lp.t + warp;
+            if (CLUSTER || lf >= f1) more = false;
+            else lp = attn_part(prefix, last, a.B, nvh, lf, f1), lt = lp.t + warp;
         }
-        if (more) load(lp, lt, slot), lt += ATT_W;
+        if (more) {
+            l_entry = lt * ATT_TILE + (a.tiled ? 0 : lane & 15);
+            if (l_entry < lp.len) l_page = a.table[(int64_t)lp.b * a.max_pages + a.page.div(l_entry)];
+        }
+    };
+    auto fill = [&](int slot) {
+        if (more) {
+            const uint32_t dst = ring_s + slot * SH::TILE_BYTES;
+            const CT *const k = static_cast<const CT *>(a.k), *const v = static_cast<const CT *>(a.v);
+            const int kvh = a.NB == 1 ? lp.vh : lp.vh / a.NB, in = l_entry - a.page.div(l_entry) * a.page_size;
+            const bool there = l_entry < lp.len, ok = there && l_page >= 0 && l_page < a.n_pages;
+            if (there && !ok) report(a.errors, OFB_CACHE_EPAGE);
+            const int64_t off = ok ? l_page * a.page_stride + ((int64_t)kvh * a.page_size + in) * D : -1;
+            if (a.tiled) {  // 16 rows on end
+                const int rows = off < 0 ? 0 : min(ATT_TILE, lp.len - l_entry);
+                const CT *ks = k + (off < 0 ? 0 : off) + lane * 8, *vs = v + (off < 0 ? 0 : off) + lane * 8;
+                if (lane == 0) valid[warp][slot] = (1u << rows) - 1u;
+#pragma unroll
+                for (int j = 0; j < ATT_TILE * CH / 32; j++) {
+                    const int c = j * 32 + lane, r = c / CH, x = c - r * CH;
+                    const bool in_row = r < rows;
+                    // a row that is not there is not read: its address need not exist
+                    cp16(dst + r * SH::PITCH + x * 16, in_row ? ks + j * 256 : k, in_row ? 16 : 0);
+                    cp16(dst + (ATT_TILE + r) * SH::PITCH + x * 16, in_row ? vs + j * 256 : v, in_row ? 16 : 0);
+                }
+            } else {
+                const uint32_t mask = __ballot_sync(0xffffffffu, off >= 0);
+                if (lane == 0) valid[warp][slot] = mask & 0xffffu;
+#pragma unroll
+                for (int j = 0; j < ATT_TILE * CH / 32; j++) {
+                    const int c = j * 32 + lane, r = c / CH, x = c - r * CH;
+                    const int64_t o = __shfl_sync(0xffffffffu, off, r);
+                    const int64_t e = o < 0 ? 0 : o + x * 8;
+                    const int n = o < 0 ? 0 : 16;
+                    cp16(dst + r * SH::PITCH + x * 16, k + e, n);
+                    cp16(dst + (ATT_TILE + r) * SH::PITCH + x * 16, v + e, n);
+                }
+            }
+            lt += ATT_W;
+            look_up();
+        }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    look_up();
 #pragma unroll
     for (int i = 0; i < SH::S - 1; i++) fill(i);
     int slot = 0;  // of the next tile to compute
 
     int npart = 0;
     for (long long f = f0; f < f1; npart++) {
-        const AttnPart p = attn_part(prefix, a.B, nvh, f, f1);
+        const AttnPart p = npart ? attn_part(prefix, last, a.B, nvh, f, f1) : first;
         const int kvh = p.vh / a.NB, h0 = (p.vh - kvh * a.NB) * ATT_R, rows = min(ATT_R, a.G - h0);
         // queries: row g of A, parts as told at the top
         uint32_t qa[KS][2][NQ];
@@ -286,16 +366,18 @@ __global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_ker
                     split2<CT, NQ>(x, y, qa[ks][u]);
                 }
         }
-        float o[D / 8][2], m = -INFINITY, l = 0.0f;
+        float o[D / 8][NO], m = -INFINITY, l = 0.0f;
 #pragma unroll
-        for (int i = 0; i < D / 8; i++) o[i][0] = o[i][1] = 0.0f;
+        for (int i = 0; i < D / 8; i++)
+#pragma unroll
+            for (int u = 0; u < NO; u++) o[i][u] = 0.0f;
 
         for (int t = p.t + warp; t < p.end; t += ATT_W) {
             asm volatile("cp.async.wait_group %0;" ::"n"(SH::S - 2) : "memory");
             __syncwarp();
             fill(slot == 0 ? SH::S - 1 : slot - 1);
             const uint32_t ks_s = ring_s + slot * SH::TILE_BYTES, vs_s = ks_s + ATT_TILE * SH::PITCH;
-            const uint32_t ok = valid[warp][slot];
+            const uint32_t ok = valid[warp][slot] >> c2;
             slot = slot == SH::S - 1 ? 0 : slot + 1;
 
             float s[2][4] = {}, s2[2][4] = {};
@@ -324,7 +406,7 @@ __global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_ker
                 for (int u = 0; u < 2; u++) {
                     float x = s[j][u] + s2[j][u];
                     if (NQ > 1) x += s[j][2 + u] + s2[j][2 + u];
-                    z[j][u] = (ok >> (8 * j + c2 + u)) & 1 ? x * qscale : -INFINITY;
+                    z[j][u] = (ok >> (8 * j + u)) & 1 ? x * qscale : -INFINITY;
                 }
             if (a.z && g < rows) {
                 float *zr = a.z + ((int64_t)p.b * a.H + kvh * a.G + h0 + g) * a.z_stride + t * ATT_TILE + c2;
@@ -335,35 +417,47 @@ __global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_ker
             mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
             mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
             const float mn = fmaxf(m, mt), ref = mn == -INFINITY ? 0.0f : mn;
-            const float alpha = exp2f(m - ref);  // 0 at the first tile
+            const float alpha = exp2_fast(m - ref);  // 0 at the first tile
+            const bool grown = __any_sync(0xffffffffu, mn != m);
             m = mn;
             uint32_t pa[2][NP];  // [entries 0-7 / 8-15][part]
             float sum = 0.0f;
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                const float x = exp2f(z[j][0] - ref), y = exp2f(z[j][1] - ref);
+                const float x = exp2_fast(z[j][0] - ref), y = exp2_fast(z[j][1] - ref);
                 sum += x + y;
                 split2<CT, NP>(x * PSCALE, y * PSCALE, pa[j]);
             }
             l = l * alpha + sum;
+            if (DIRECT && grown) {
+#pragma unroll
+                for (int i = 0; i < D / 8; i++)
+#pragma unroll
+                    for (int u = 0; u < NO; u++) o[i][u] *= alpha;
+            }
             const uint32_t va = vs_s + ((lane & 7) + ((lane >> 3) & 1) * 8) * SH::PITCH + (lane >> 4) * 16;
             const uint32_t a0[4] = {pa[0][0], pa[0][1], pa[1][0], pa[1][1]};
 #pragma unroll
             for (int n = 0; n < D / 16; n++) {
                 uint32_t b[4];
                 ldmatrix4_t(b, va + n * 32);
-                float x[4] = {}, y[4] = {};
-                Mma<CT>::run(x, a0, b[0], b[1]);
-                Mma<CT>::run(y, a0, b[2], b[3]);
-                if constexpr (NP > 2) {
-                    const uint32_t a1[4] = {pa[0][2], 0u, pa[1][2], 0u};
-                    Mma<CT>::run(x, a1, b[0], b[1]);
-                    Mma<CT>::run(y, a1, b[2], b[3]);
+                if constexpr (DIRECT) {
+                    Mma<CT>::run(o[2 * n], a0, b[0], b[1]);
+                    Mma<CT>::run(o[2 * n + 1], a0, b[2], b[3]);
+                } else {
+                    float x[4] = {}, y[4] = {};
+                    Mma<CT>::run(x, a0, b[0], b[1]);
+                    Mma<CT>::run(y, a0, b[2], b[3]);
+                    if constexpr (NP > 2) {
+                        const uint32_t a1[4] = {pa[0][2], 0u, pa[1][2], 0u};
+                        Mma<CT>::run(x, a1, b[0], b[1]);
+                        Mma<CT>::run(y, a1, b[2], b[3]);
+                    }
+                    o[2 * n][0] = o[2 * n][0] * alpha + (x[0] + x[2]);
+                    o[2 * n][1] = o[2 * n][1] * alpha + (x[1] + x[3]);
+                    o[2 * n + 1][0] = o[2 * n + 1][0] * alpha + (y[0] + y[2]);
+                    o[2 * n + 1][1] = o[2 * n + 1][1] * alpha + (y[1] + y[3]);
                 }
-                o[2 * n][0] = o[2 * n][0] * alpha + (x[0] + x[2]);
-                o[2 * n][1] = o[2 * n][1] * alpha + (x[1] + x[3]);
-                o[2 * n + 1][0] = o[2 * n + 1][0] * alpha + (y[0] + y[2]);
-                o[2 * n + 1][1] = o[2 * n + 1][1] * alpha + (y[1] + y[3]);
             }
         }
         // merge the warps: their sums, maxima and sums of exponentials. A warp
@@ -375,11 +469,14 @@ __global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_ker
         float *const mslot = reinterpret_cast<float *>(ring + (slot == 0 ? SH::S - 1 : slot - 1) * SH::TILE_BYTES);
         float *mw = mslot + g * (D + 4);
         if (lane == 0) mo[warp] = mslot;
+        if (CLUSTER && tid == 0) mo_at = (int)(reinterpret_cast<uint8_t *>(mslot) - smem);
 #pragma unroll
-        for (int i = 0; i < D / 8; i++) *reinterpret_cast<float2 *>(mw + i * 8 + c2) = make_float2(o[i][0], o[i][1]);
+        for (int i = 0; i < D / 8; i++)
+            *reinterpret_cast<float2 *>(mw + i * 8 + c2) =
+                DIRECT ? make_float2(o[i][0] + o[i][NO - 2], o[i][1] + o[i][NO - 1]) : make_float2(o[i][0], o[i][1]);
         if ((lane & 3) == 0) mml[warp * ATT_R + g] = make_float2(m, l);
         __syncthreads();
-        const bool whole = p.t == 0 && p.end == p.nt;
+        const bool whole = !CLUSTER && p.t == 0 && p.end == p.nt;
         const int64_t slot_id = 2 * (int64_t)blockIdx.x + (npart ? 1 : 0);
         for (int i = tid; i < rows * (D / 4); i += ATT_W * 32) {
             const int r = i / (D / 4), x = (i - r * (D / 4)) * 4;
@@ -392,13 +489,16 @@ __global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_ker
 #pragma unroll
             for (int w = 0; w < ATT_W; w++) {
                 const float2 e = mml[w * ATT_R + r];
-                const float s = exp2f(e.x - ref);
+                const float s = exp2_fast(e.x - ref);
                 const float4 y = *reinterpret_cast<const float4 *>(mo[w] + r * (D + 4) + x);
                 ll += s * e.y;
                 acc.x += s * y.x, acc.y += s * y.y, acc.z += s * y.z, acc.w += s * y.w;
             }
             const int64_t head = kvh * a.G + h0 + r;
-            if (whole) {
+            if (CLUSTER) {  // in place of warp 0's sums, whose elements only this thread reads
+                *reinterpret_cast<float4 *>(mo[0] + r * (D + 4) + x) = acc;
+                if (x == 0) cml[r] = make_float2(mm, ll);
+            } else if (whole) {
                 // no entry attended to (all on bad pages): zeros
                 const float inv = ll > 0.0f || ll != ll ? 1.0f / (ll * PSCALE) : 0.0f;
                 IO *dst = static_cast<IO *>(a.out) + p.b * a.out_stride + head * D + x;
@@ -411,6 +511,50 @@ __global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_ker
                 if (x == 0) a.part_ml[slot_id * ATT_R + r] = make_float2(mm, ll);
             }
         }
+        if constexpr (CLUSTER) {
+            // join the cluster's CTAs; each writes some of the columns
+            const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
+            cl.sync();
+            if (tid < rows) {
+                float mm = -INFINITY, ll = 0.0f;
+                for (int r = 0; r < C; r++) mm = fmaxf(mm, cl.map_shared_rank(cml, r)[tid].x);
+                const float ref = mm == -INFINITY ? 0.0f : mm;
+                for (int r = 0; r < C; r++) {
+                    const float2 e = cl.map_shared_rank(cml, r)[tid];
+                    ll += exp2_fast(e.x - ref) * e.y;
+                }
+                cml[ATT_R + tid] = make_float2(ref, ll > 0.0f || ll != ll ? 1.0f / ll : 0.0f);
+            }
+            __syncthreads();
+            // (a CTA's sums are in the slot that its warp 0 came to: it says which)
+            for (int i = rank * ATT_W * 32 + tid; i < rows * (D / 4); i += C * ATT_W * 32) {
+                const int r = i / (D / 4), x = (i - r * (D / 4)) * 4;
+                const float2 fin = cml[ATT_R + r];
+                float4 acc = make_float4(0, 0, 0, 0);
+                for (int c = 0; c < C; c++) {
+                    const float s = exp2_fast(cl.map_shared_rank(cml, c)[r].x - fin.x);
+                    const int at = *cl.map_shared_rank(&mo_at, c);
+                    const float4 y = *reinterpret_cast<const float4 *>(cl.map_shared_rank(smem, c) + at + (r * (D + 4) + x) * 4);
+                    acc.x += s * y.x, acc.y += s * y.y, acc.z += s * y.z, acc.w += s * y.w;
+                }
+                const float inv = fin.y / PSCALE;
+                IO *dst = static_cast<IO *>(a.out) + p.b * a.out_stride + (int64_t)(kvh * a.G + h0 + r) * D + x;
+                dst[0] = from_f32<IO>(acc.x * inv), dst[1] = from_f32<IO>(acc.y * inv);
+                dst[2] = from_f32<IO>(acc.z * inv), dst[3] = from_f32<IO>(acc.w * inv);
+            }
+            if (a.z) {  // one pass per kv head here: this CTA's entries are its own
+                const int i1 = min(p.end * ATT_TILE, p.len);
+                for (int i = p.t * ATT_TILE + tid; i < i1; i += ATT_W * 32) {
+                    const float *z = a.z + ((int64_t)p.b * a.H + kvh * a.G) * a.z_stride + i;
+                    float add = 0.0f;
+                    for (int r = 0; r < rows; r++) add += exp2_fast(z[r * a.z_stride] - cml[ATT_R + r].x) * cml[ATT_R + r].y;
+                    const int col = a.page.div(i), page = a.table[(int64_t)p.b * a.max_pages + col];
+                    if (page >= 0 && page < a.n_pages) a.weight[((int64_t)page * a.KVH + kvh) * a.page_size + (i - col * a.page_size)] += add;
+                }
+            }
+            cl.sync();  // no CTA leaves while its sums are read
+            break;
+        }
         __syncthreads();  // the slots may be filled again
         f += p.end - p.t;
     }
@@ -419,24 +563,26 @@ __global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_ker
 
 using AttnKernel = void (*)(AttnArgs);
 struct AttnVariant {
-    AttnKernel kernel;
-    int smem, ctas;  // dynamic shared memory, CTAs per SM
+    AttnKernel run, cluster;
+    int head, ctas;  // shared memory without the per-sequence part, CTAs per SM
 };
-// The instance for a head width: cache type bf16 or fp16, activations f32 or the cache's.
+// The instances for a head width: cache type bf16 or fp16, activations f32 or the cache's.
 AttnVariant attn_variant_64(bool bf16, bool f32);
 AttnVariant attn_variant_96(bool bf16, bool f32);
 AttnVariant attn_variant_128(bool bf16, bool f32);
 AttnVariant attn_variant_192(bool bf16, bool f32);
 AttnVariant attn_variant_256(bool bf16, bool f32);
 
+template <int D, typename CT, typename IO> AttnVariant attn_instances() {
+    return {attn_split_kernel<D, CT, IO, false>, attn_split_kernel<D, CT, IO, true>, AttnShape<D>::smem(0), AttnShape<D>::CTAS};
+}
+
 }  // namespace ofb
 
-#define OFB_ATTN_INSTANCES(D)                                                                                 \
-    namespace ofb {                                                                                           \
-    AttnVariant attn_variant_##D(bool bf16, bool f32) {                                                       \
-        const AttnKernel k = bf16 ? (f32 ? attn_split_kernel<D, __nv_bfloat16, float>                         \
-                                         : attn_split_kernel<D, __nv_bfloat16, __nv_bfloat16>)                \
-                                  : (f32 ? attn_split_kernel<D, __half, float> : attn_split_kernel<D, __half, __half>); \
-        return {k, AttnShape<D>::SMEM, AttnShape<D>::CTAS};                                                   \
-    }                                                                                                         \
+#define OFB_ATTN_INSTANCES(D)                                                                                   \
+    namespace ofb {                                                                                             \
+    AttnVariant attn_variant_##D(bool bf16, bool f32) {                                                         \
+        if (bf16) return f32 ? attn_instances<D, __nv_bfloat16, float>() : attn_instances<D, __nv_bfloat16, __nv_bfloat16>(); \
+        return f32 ? attn_instances<D, __half, float>() : attn_instances<D, __half, __half>();                  \
+    }                                                                                                           \
     }

@@ -42,6 +42,7 @@ struct EvictArgs {
     int32_t *lens_out, *kept, *lists;
     uint32_t *errors;
     int64_t page_stride;
+    FastDiv page;
     int KVH, d, page_size, n_pages, max_pages, max_len, keep, recent, chunk;
 };
 
@@ -78,15 +79,11 @@ __global__ void __launch_bounds__(EV_THREADS) evict_kernel(const __grid_constant
         return;
     }
     const int32_t *table = a.table + (int64_t)b * a.max_pages;
-    // flat (page, slot) of entry i, or -1
+    // row of entry i among a kv head's rows [n_pages][KVH][page_size], or -1
     auto entry = [&](int i) -> int64_t {
-        const int col = i / a.page_size, p = table[col];
+        const int col = a.page.div(i), p = table[col];
         if (p < 0 || p >= a.n_pages) return -1;
-        return (int64_t)p * a.page_size + (i - col * a.page_size);
-    };
-    auto meta = [&](int64_t e) {
-        const int64_t p = e / a.page_size;
-        return (p * a.KVH + h) * a.page_size + (e - p * a.page_size);
+        return ((int64_t)p * a.KVH + h) * a.page_size + (i - col * a.page_size);
     };
     const int i0 = min(rank * a.chunk, n), i1 = min(i0 + a.chunk, n), m = i1 - i0;
 
@@ -100,9 +97,8 @@ __global__ void __launch_bounds__(EV_THREADS) evict_kernel(const __grid_constant
         if (e < 0) {
             report(a.errors, OFB_CACHE_EPAGE);
         } else {
-            const int64_t at = meta(e);
-            key = weight_key(a.weight[at]);
-            if (a.recent) top = max(top, a.order[at]);
+            key = weight_key(a.weight[e]);
+            if (a.recent) top = max(top, a.order[e]);
         }
         keys[i] = key;
     }
@@ -115,7 +111,7 @@ __global__ void __launch_bounds__(EV_THREADS) evict_kernel(const __grid_constant
         const int64_t above = (int64_t)top - a.recent;
         for (int i = tid; i < m; i += EV_THREADS) {
             const int64_t e = entry(i0 + i);
-            if (e >= 0 && a.order[meta(e)] > above) keys[i] = 0xffffffffu;
+            if (e >= 0 && a.order[e] > above) keys[i] = 0xffffffffu;
         }
     }
     __syncthreads();
@@ -219,16 +215,15 @@ __global__ void __launch_bounds__(EV_THREADS) evict_kernel(const __grid_constant
         int64_t from = -1, to = -1;
         if (lane < cnt) {
             const int hole = hole_list[m0 + lane], spare = spare_list[m0 + lane];
-            const int64_t es = entry(spare), eh = entry(hole);
+            const int cs = a.page.div(spare), ch = a.page.div(hole), ps = table[cs], ph = table[ch];
+            const int ss = spare - cs * a.page_size, sh = hole - ch * a.page_size;
             if (kept) kept[hole] = spare;
-            if (es >= 0 && eh >= 0) {
-                const int64_t ps = es / a.page_size, ph = eh / a.page_size;
-                const int64_t ms = (ps * a.KVH + h) * a.page_size + (es - ps * a.page_size);
-                const int64_t mh = (ph * a.KVH + h) * a.page_size + (eh - ph * a.page_size);
+            if (ps >= 0 && ps < a.n_pages && ph >= 0 && ph < a.n_pages) {
+                const int64_t ms = ((int64_t)ps * a.KVH + h) * a.page_size + ss, mh = ((int64_t)ph * a.KVH + h) * a.page_size + sh;
                 a.weight[mh] = a.weight[ms];
                 a.order[mh] = a.order[ms];
-                from = ps * a.page_stride + ((int64_t)h * a.page_size + (es - ps * a.page_size)) * a.d;
-                to = ph * a.page_stride + ((int64_t)h * a.page_size + (eh - ph * a.page_size)) * a.d;
+                from = ps * a.page_stride + ((int64_t)h * a.page_size + ss) * a.d;
+                to = ph * a.page_stride + ((int64_t)h * a.page_size + sh) * a.d;
             }
         }
         // 16-byte chunks of K and V rows, element type of 2 bytes
@@ -313,7 +308,7 @@ extern "C" int ofb_kv_evict(const ofb_kv_cache *cache, const int32_t *lens, int 
     a.lens = lens, a.lens_out = lens_out, a.kept = kept, a.lists = static_cast<int32_t *>(scratch), a.errors = cache->errors;
     a.page_stride = cache_page_stride(cache);
     a.KVH = cache->n_kv_heads, a.d = cache->head_dim, a.page_size = cache->page_size, a.n_pages = cache->n_pages;
-    a.max_pages = cache->max_pages, a.max_len = bound, a.keep = keep, a.recent = recent;
+    a.page = fast_div(a.page_size), a.max_pages = cache->max_pages, a.max_len = bound, a.keep = keep, a.recent = recent;
     const int C = evict_cluster((int)rows, bound);
     a.chunk = (bound + C - 1) / C;
     const size_t smem = (size_t)(3 * EV_BINS + a.chunk) * 4;
@@ -321,18 +316,6 @@ extern "C" int ofb_kv_evict(const ofb_kv_cache *cache, const int32_t *lens, int 
     // with room for the kernel's static arrays, which count against the default limit too
     cudaError_t e = ensure_dyn_smem(evict_kernel, smem + 1024, attr);
     if (e != cudaSuccess) return cuda_status(e, "ofb_kv_evict smem attribute");
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(rows * C));
-    cfg.blockDim = dim3(EV_THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = static_cast<cudaStream_t>(stream);
-    cudaLaunchAttribute at[2];
-    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at[0].val.programmaticStreamSerializationAllowed = 1;
-    at[1].id = cudaLaunchAttributeClusterDimension;
-    at[1].val.clusterDim.x = C, at[1].val.clusterDim.y = 1, at[1].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, evict_kernel, a);
+    e = launch_pdl_cluster(evict_kernel, dim3((unsigned)(rows * C)), dim3(EV_THREADS), C, smem, static_cast<cudaStream_t>(stream), a);
     return e == cudaSuccess ? OFB_OK : cuda_status(e, "ofb_kv_evict launch");
 }

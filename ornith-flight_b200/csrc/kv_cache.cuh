@@ -39,6 +39,24 @@ template <typename T> __device__ __forceinline__ void store8(T *p, const float (
     *reinterpret_cast<uint4 *>(p) = u;
 }
 
+// Division of entry numbers (below 2^31) by a launch constant: one high product
+// and a shift instead of the ~30 instructions of a division.
+struct FastDiv {
+    uint32_t d, mul, shift;
+    __device__ __forceinline__ int div(int n) const {
+        return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift);
+    }
+};
+inline FastDiv fast_div(int d) {
+    FastDiv f;
+    f.d = (uint32_t)d;
+    f.shift = 0;
+    while ((1u << f.shift) < f.d) f.shift++;
+    // round-up method: floor(2^32 (2^shift - d) / d) + 1, exact for n < 2^31
+    f.mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << f.shift) - f.d)) / f.d + 1);
+    return f;
+}
+
 __device__ __forceinline__ void report(uint32_t *errors, uint32_t bits) {
     if (errors) atomicOr(errors, bits);
 }

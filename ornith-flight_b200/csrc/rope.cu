@@ -11,8 +11,8 @@
 // the nearest even integer, so that the f32 that goes to sincospif is within
 // [-1, 1] and off by at most 2^-25 half turns. f(i)/pi comes with the launch:
 // the host forms it by one powl and repeated products, 1 KB of arguments.
-// Then each thread takes items of two 8-element chunks (a pair's two halves,
-// or 16 neighbours), read and written 16 bytes at a time. Sizes or addresses
+// Then each thread takes items of two 8-element chunks (the two halves of 8
+// pairs, or 16 neighbours), read and written 16 bytes at a time. Sizes or addresses
 // that do not allow it (head_dim or rot_dim no multiple of 16, strides no
 // multiple of 8, pointers off 16 bytes) take the second kernel, a pair per
 // item.
@@ -28,6 +28,7 @@ constexpr int RP_PAIRS = 128;
 struct RopeArgs {
     int T, H, KVH, d, rot, tpb;  // heads of q; kv heads (0: no cache); tokens per CTA
     int n_pages, page_size, n_seqs, max_pages;
+    FastDiv page, rows;  // by page_size, by H + 2 KVH
     const void *q, *k, *v;
     void *q_out, *ck, *cv;
     int64_t qs, ks, vs, qos, page_stride, pos_stride;
@@ -39,161 +40,190 @@ struct RopeArgs {
     uint8_t axis[RP_PAIRS];
 };
 
-// Shared memory: cs[tpb][rot/2], then entry[tpb]: the row's flat (page, slot),
-// or -1 where nothing is written.
-__device__ __forceinline__ void rope_setup(const RopeArgs &a, int t0, int nt, float2 *cs, int64_t *entry) {
+// Where a CTA's tokens go: page -1 where nothing is written.
+struct RopeEntry {
+    int page, slot;
+};
+// Shared memory: cosines [tpb][rot/2], sines [tpb][rot/2], entries [tpb].
+struct RopeShared {
+    float *c, *s;
+    RopeEntry *entry;
+    __device__ __forceinline__ RopeShared(const RopeArgs &a, float *base)
+        : c(base), s(base + a.tpb * (a.rot / 2)), entry(reinterpret_cast<RopeEntry *>(base + a.tpb * a.rot)) {}
+};
+
+__device__ __forceinline__ void rope_setup(const RopeArgs &a, int t0, int nt, const RopeShared &sh) {
     const int pairs = a.rot / 2;
+    // read through a plain address: lanes want different pairs, which the
+    // constant bank would serve one at a time
+    const double *freq = a.half_turns;
+    const uint8_t *axis = a.axis;
+    asm("" : "+l"(freq), "+l"(axis));
     for (int i = threadIdx.x; i < nt * pairs; i += RP_THREADS) {
         const int t = i / pairs, p = i - t * pairs;
-        const double h = (double)a.pos[a.axis[p] * a.pos_stride + t0 + t] * a.half_turns[p];
+        const double h = (double)a.pos[axis[p] * a.pos_stride + t0 + t] * freq[p];
         float s, c;
         sincospif((float)(h - 2.0 * rint(0.5 * h)), &s, &c);
-        cs[i] = make_float2(c, s);
+        sh.c[i] = c;
+        sh.s[i] = s;
     }
     if (a.KVH && threadIdx.x < nt) {
         const int t = t0 + threadIdx.x, b = a.seq[t], i = a.index[t];
-        int64_t e = -1;
+        RopeEntry e = {-1, 0};
         if (b >= 0) {
-            const int col = i / a.page_size;
+            const int col = i < 0 ? 0 : a.page.div(i);
             if (b >= a.n_seqs || i < 0 || col >= a.max_pages) {
                 report(a.errors, OFB_CACHE_EINDEX);
             } else {
                 const int p = a.table[(int64_t)b * a.max_pages + col];
                 if (p < 0 || p >= a.n_pages) report(a.errors, OFB_CACHE_EPAGE);
-                else e = (int64_t)p * a.page_size + (i - col * a.page_size);
+                else e = {p, i - col * a.page_size};
             }
         }
-        entry[threadIdx.x] = e;
+        sh.entry[threadIdx.x] = e;
     }
     __syncthreads();
 }
 
 // Weight 0 and the order number of the CTA's new entries.
-__device__ __forceinline__ void rope_meta(const RopeArgs &a, int t0, int nt, const int64_t *entry) {
+__device__ __forceinline__ void rope_meta(const RopeArgs &a, int t0, int nt, const RopeEntry *entry) {
     if (!a.weight && !a.order) return;
     for (int i = threadIdx.x; i < nt * a.KVH; i += RP_THREADS) {
         const int t = i / a.KVH, h = i - t * a.KVH;
-        const int64_t e = entry[t];
-        if (e < 0) continue;
-        const int64_t p = e / a.page_size, m = (p * a.KVH + h) * a.page_size + (e - p * a.page_size);
+        const RopeEntry e = entry[t];
+        if (e.page < 0) continue;
+        const int64_t m = ((int64_t)e.page * a.KVH + h) * a.page_size + e.slot;
         if (a.weight) a.weight[m] = 0.0f;
         if (a.order) a.order[m] = a.number ? a.number[t0 + t] : a.index[t0 + t];
     }
 }
 
-__device__ __forceinline__ int64_t cache_row(const RopeArgs &a, int64_t e, int h) {
-    const int64_t p = e / a.page_size;
-    return p * a.page_stride + ((int64_t)h * a.page_size + (e - p * a.page_size)) * a.d;
+// A row of the launch: query, key or value row of one token.
+struct RopeRow {
+    int t, h;
+    bool is_q, is_v;
+};
+__device__ __forceinline__ RopeRow rope_row(const RopeArgs &a, int vr) {
+    RopeRow r;
+    r.t = a.rows.div(vr);
+    const int row = vr - r.t * (int)a.rows.d;
+    r.is_q = row < a.H;
+    r.is_v = row >= a.H + a.KVH;
+    r.h = row - (r.is_q ? 0 : r.is_v ? a.H + a.KVH : a.H);
+    return r;
+}
+template <typename IO> __device__ __forceinline__ const IO *rope_src(const RopeArgs &a, const RopeRow &r, int t0) {
+    const void *p = r.is_q ? a.q : r.is_v ? a.v : a.k;
+    const int64_t stride = r.is_q ? a.qs : r.is_v ? a.vs : a.ks;
+    return static_cast<const IO *>(p) + (t0 + r.t) * stride + (int64_t)r.h * a.d;
+}
+__device__ __forceinline__ int64_t rope_cache_at(const RopeArgs &a, const RopeEntry &e, int h) {
+    return e.page * a.page_stride + ((int64_t)h * a.page_size + e.slot) * a.d;
 }
 
+// Thread (slot, j) takes chunk pair j of rows slot, slot + slots, ...; the next
+// row's chunks are on their way while one is turned, the first while the
+// cosines are formed.
 template <typename IO, typename CT, bool ADJ>
 __global__ void __launch_bounds__(RP_THREADS) rope_vec_kernel(const __grid_constant__ RopeArgs a) {
-    extern __shared__ float2 cs[];
-    int64_t *entry = reinterpret_cast<int64_t *>(cs + (size_t)a.tpb * (a.rot / 2));
+    extern __shared__ __align__(16) float rope_smem[];
+    const RopeShared sh(a, rope_smem);
     pdl_wait();
     pdl_trigger();
-    const int t0 = blockIdx.x * a.tpb, nt = min(a.tpb, a.T - t0);
-    rope_setup(a, t0, nt, cs, entry);
-    const int per_row = a.d / 16, rows = a.H + 2 * a.KVH, per_tok = rows * per_row, half = a.rot / 2;
-    for (int it = threadIdx.x; it < nt * per_tok; it += RP_THREADS) {
-        const int t = it / per_tok, r = it - t * per_tok, row = r / per_row, j = r - row * per_row;
-        const IO *src;
-        int64_t to = 0;
-        const bool is_q = row < a.H, is_v = row >= a.H + a.KVH;
-        if (is_q) {
-            src = static_cast<const IO *>(a.q) + (int64_t)(t0 + t) * a.qs + (int64_t)row * a.d;
-        } else {
-            if (entry[t] < 0) continue;
-            const int h = row - a.H - (is_v ? a.KVH : 0);
-            src = is_v ? static_cast<const IO *>(a.v) + (int64_t)(t0 + t) * a.vs + (int64_t)h * a.d
-                       : static_cast<const IO *>(a.k) + (int64_t)(t0 + t) * a.ks + (int64_t)h * a.d;
-            to = cache_row(a, entry[t], h);
+    const int t0 = blockIdx.x * a.tpb, nt = min(a.tpb, a.T - t0), half = a.rot / 2;
+    const int per_row = a.d / 16, slots = RP_THREADS / per_row, slot = threadIdx.x / per_row, j = threadIdx.x - slot * per_row;
+    const int total = slot < slots ? nt * (int)a.rows.d : 0;
+    // chunk places: of a turned row the two halves of 8 pairs, or 16 neighbours
+    const bool in_rot = j * 16 < a.rot;
+    const int ta = in_rot && !ADJ ? 8 * j : 16 * j, tb = in_rot && !ADJ ? half + 8 * j : 16 * j + 8;
+    float x[8], y[8], nx[8], ny[8];
+    RopeRow r = {}, nr = {};
+    if (slot < total) {
+        r = rope_row(a, slot);
+        const IO *src = rope_src<IO>(a, r, t0);
+        load8(src + ta, x);
+        load8(src + tb, y);
+    }
+    rope_setup(a, t0, nt, sh);
+    for (int vr = slot; vr < total; vr += slots) {
+        if (vr + slots < total) {
+            nr = rope_row(a, vr + slots);
+            const IO *src = rope_src<IO>(a, nr, t0);
+            load8(src + ta, nx);
+            load8(src + tb, ny);
         }
-        // chunk places of this item: the two halves of 8 pairs, or 16 neighbours
-        const bool turned = !is_v && j * 16 < a.rot;
-        const int ca = turned && !ADJ ? 8 * j : 16 * j, cb = turned && !ADJ ? half + 8 * j : 16 * j + 8;
-        float x[8], y[8];
-        load8(src + ca, x);
-        load8(src + cb, y);
-        if (turned) {
-            const float2 *c = cs + t * half + 8 * j;
+        if (in_rot && !r.is_v) {
+            float c[8], s[8];
+            load8(sh.c + r.t * half + 8 * j, c);
+            load8(sh.s + r.t * half + 8 * j, s);
             if (ADJ) {
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float2 w = c[i], z = c[4 + i];
                     const float u = x[2 * i], v = x[2 * i + 1], m = y[2 * i], n = y[2 * i + 1];
-                    x[2 * i] = u * w.x - v * w.y;
-                    x[2 * i + 1] = v * w.x + u * w.y;
-                    y[2 * i] = m * z.x - n * z.y;
-                    y[2 * i + 1] = n * z.x + m * z.y;
+                    x[2 * i] = u * c[i] - v * s[i];
+                    x[2 * i + 1] = v * c[i] + u * s[i];
+                    y[2 * i] = m * c[4 + i] - n * s[4 + i];
+                    y[2 * i + 1] = n * c[4 + i] + m * s[4 + i];
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float2 w = c[i];
                     const float u = x[i], v = y[i];
-                    x[i] = u * w.x - v * w.y;
-                    y[i] = v * w.x + u * w.y;
+                    x[i] = u * c[i] - v * s[i];
+                    y[i] = v * c[i] + u * s[i];
                 }
             }
         }
-        if (is_q) {
-            IO *dst = static_cast<IO *>(a.q_out) + (int64_t)(t0 + t) * a.qos + (int64_t)row * a.d;
-            store8(dst + ca, x);
-            store8(dst + cb, y);
-        } else {
-            CT *dst = static_cast<CT *>(is_v ? a.cv : a.ck) + to;
-            store8(dst + ca, x);
-            store8(dst + cb, y);
+        if (r.is_q) {
+            IO *dst = static_cast<IO *>(a.q_out) + (t0 + r.t) * a.qos + (int64_t)r.h * a.d;
+            store8(dst + ta, x);
+            store8(dst + tb, y);
+        } else if (sh.entry[r.t].page >= 0) {
+            CT *dst = static_cast<CT *>(r.is_v ? a.cv : a.ck) + rope_cache_at(a, sh.entry[r.t], r.h);
+            store8(dst + ta, x);
+            store8(dst + tb, y);
         }
+        r = nr;
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = nx[i], y[i] = ny[i];
     }
-    rope_meta(a, t0, nt, entry);
+    rope_meta(a, t0, nt, sh.entry);
 }
 
 // Any sizes and strides: items are pairs (rot/2 per row), then single elements.
 template <typename IO, typename CT>
 __global__ void __launch_bounds__(RP_THREADS) rope_any_kernel(const __grid_constant__ RopeArgs a, int adjacent) {
-    extern __shared__ float2 cs[];
-    int64_t *entry = reinterpret_cast<int64_t *>(cs + (size_t)a.tpb * (a.rot / 2));
+    extern __shared__ __align__(16) float rope_smem[];
+    const RopeShared sh(a, rope_smem);
     pdl_wait();
     pdl_trigger();
-    const int t0 = blockIdx.x * a.tpb, nt = min(a.tpb, a.T - t0);
-    rope_setup(a, t0, nt, cs, entry);
-    const int half = a.rot / 2, per_row = a.d - half, rows = a.H + 2 * a.KVH, per_tok = rows * per_row;
-    for (int it = threadIdx.x; it < nt * per_tok; it += RP_THREADS) {
-        const int t = it / per_tok, r = it - t * per_tok, row = r / per_row, j = r - row * per_row;
-        const bool is_q = row < a.H, is_v = row >= a.H + a.KVH;
-        const IO *src;
-        int64_t to = 0;
-        if (is_q) {
-            src = static_cast<const IO *>(a.q) + (int64_t)(t0 + t) * a.qs + (int64_t)row * a.d;
-        } else {
-            if (entry[t] < 0) continue;
-            const int h = row - a.H - (is_v ? a.KVH : 0);
-            src = is_v ? static_cast<const IO *>(a.v) + (int64_t)(t0 + t) * a.vs + (int64_t)h * a.d
-                       : static_cast<const IO *>(a.k) + (int64_t)(t0 + t) * a.ks + (int64_t)h * a.d;
-            to = cache_row(a, entry[t], h);
-        }
+    const int t0 = blockIdx.x * a.tpb, nt = min(a.tpb, a.T - t0), half = a.rot / 2;
+    rope_setup(a, t0, nt, sh);
+    const int per_row = a.d - half, total = nt * (int)a.rows.d * per_row;
+    for (int it = threadIdx.x; it < total; it += RP_THREADS) {
+        const int vr = it / per_row, j = it - vr * per_row;
+        const RopeRow r = rope_row(a, vr);
+        if (!r.is_q && sh.entry[r.t].page < 0) continue;
+        const IO *src = rope_src<IO>(a, r, t0);
         // where this item's one or two elements are
         const int ea = j >= half ? half + j : adjacent ? 2 * j : j, eb = j >= half ? ea : adjacent ? 2 * j + 1 : half + j;
         float x = to_f32(src[ea]), y = to_f32(src[eb]);
-        if (!is_v && j < half) {
-            const float2 w = cs[t * half + j];
-            const float u = x, v = y;
-            x = u * w.x - v * w.y;
-            y = v * w.x + u * w.y;
+        if (!r.is_v && j < half) {
+            const float c = sh.c[r.t * half + j], s = sh.s[r.t * half + j], u = x, v = y;
+            x = u * c - v * s;
+            y = v * c + u * s;
         }
-        if (is_q) {
-            IO *dst = static_cast<IO *>(a.q_out) + (int64_t)(t0 + t) * a.qos + (int64_t)row * a.d;
+        if (r.is_q) {
+            IO *dst = static_cast<IO *>(a.q_out) + (t0 + r.t) * a.qos + (int64_t)r.h * a.d;
             dst[ea] = from_f32<IO>(x);
             dst[eb] = from_f32<IO>(y);
         } else {
-            CT *dst = static_cast<CT *>(is_v ? a.cv : a.ck) + to;
+            CT *dst = static_cast<CT *>(r.is_v ? a.cv : a.ck) + rope_cache_at(a, sh.entry[r.t], r.h);
             dst[ea] = from_f32<CT>(x);
             dst[eb] = from_f32<CT>(y);
         }
     }
-    rope_meta(a, t0, nt, entry);
+    rope_meta(a, t0, nt, sh.entry);
 }
 
 // Checks a rotary form and lays out its pairs: axis and frequency / pi.
@@ -246,13 +276,17 @@ static int rope_tables(const ofb_rope_config *r, int head_dim, const char *who, 
 }
 
 template <typename IO, typename CT> static cudaError_t rope_launch(RopeArgs &a, bool vec, bool adjacent, cudaStream_t s) {
-    const int per_tok = (a.H + 2 * a.KVH) * (vec ? a.d / 16 : a.d - a.rot / 2);
-    // two items per thread where a token alone does not give them, at most 8 tokens (2 KB of cosines each)
-    int tpb = per_tok >= 2 * RP_THREADS ? 1 : 2 * RP_THREADS / (per_tok > 0 ? per_tok : 1);
-    if (tpb > 8) tpb = 8;
+    const int rows = a.H + 2 * a.KVH;
+    const int64_t per_tok = (int64_t)rows * (vec ? a.d / 16 : a.d - a.rot / 2);
+    // three items per thread where a token alone does not give them, at most 8
+    // tokens (2 KB of cosines and sines each), and two CTAs per SM first
+    int tpb = (int)(3 * RP_THREADS / per_tok);
+    tpb = tpb < 1 ? 1 : tpb > 8 ? 8 : tpb;
     while (tpb > 1 && (a.T + tpb - 1) / tpb < 2 * sm_count()) tpb--;
     a.tpb = tpb;
-    const size_t smem = (size_t)tpb * (a.rot / 2) * sizeof(float2) + (size_t)tpb * sizeof(int64_t);
+    a.rows = fast_div(rows);
+    a.page = fast_div(a.page_size ? a.page_size : 1);
+    const size_t smem = (size_t)tpb * (a.rot * sizeof(float) + sizeof(RopeEntry));
     const dim3 grid((a.T + tpb - 1) / tpb), block(RP_THREADS);
     if (!vec) return launch_pdl(rope_any_kernel<IO, CT>, grid, block, smem, s, a, (int)adjacent);
     return adjacent ? launch_pdl(rope_vec_kernel<IO, CT, true>, grid, block, smem, s, a)
