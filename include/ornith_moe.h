@@ -305,7 +305,7 @@ typedef struct {
  * or F16 (arithmetic in f32, rounded once). x and out: row t starts at element
  * t*x_stride (t*out_stride), its heads are consecutive; out may be x with the
  * same stride, otherwise they must not overlap. pos: int32 [n_axes][n_tokens],
- * axis a at a*pos_stride. head_dim 1..1024. */
+ * axis a at a*pos_stride. head_dim 1..1024, n_tokens up to 2^30. */
 int ofb_rope(const ofb_rope_config *rope, const void *x, int type, int n_tokens, int n_heads, int head_dim,
              int64_t x_stride, const int32_t *pos, int64_t pos_stride, void *out, int64_t out_stride, void *stream);
 

@@ -16,7 +16,7 @@
 namespace ofb {
 
 constexpr int AJ_THREADS = 256;
-constexpr int AJ_CHUNK = 512;   // entries of one weight CTA
+constexpr int AJ_CHUNK = 4 * AJ_THREADS;  // entries of one weight CTA
 constexpr int AJ_MAX_CTAS = 1024;  // of the split kernel
 
 struct AttnJoinArgs {
@@ -26,14 +26,14 @@ struct AttnJoinArgs {
 
 // Where the parts of (sequence b, pass vh) are: CTAs c0..c1 of the split kernel.
 struct PartRange {
-    long long c0, c1, f0, run;
-    __device__ __forceinline__ int64_t slot(int i) const { return 2 * (c0 + i) + ((c0 + i) * run < f0 ? 1 : 0); }
+    int c0, c1, f0, run;
+    __device__ __forceinline__ int slot(int i) const { return 2 * (c0 + i) + (i == 0 && c0 * run < f0 ? 1 : 0); }
 };
 __device__ __forceinline__ PartRange part_range(const AttnJoinArgs &j, int b, int vh, int nt) {
     const int nvh = j.a.KVH * j.a.NB;
     PartRange r;
-    r.run = attn_run((long long)j.a.prefix[j.a.B] * nvh, j.ctas);
-    r.f0 = (long long)j.a.prefix[b] * nvh + (long long)vh * nt;
+    r.run = attn_run(j.a.prefix[j.a.B] * nvh, j.ctas);
+    r.f0 = j.a.prefix[b] * nvh + vh * nt;
     r.c0 = r.f0 / r.run;
     r.c1 = (r.f0 + nt - 1) / r.run;
     return r;
@@ -101,7 +101,7 @@ template <typename IO> __global__ void __launch_bounds__(AJ_THREADS) attn_join_k
 #pragma unroll 8
             for (int i = warp; i < n; i += AJ_THREADS / 32) {
                 const float f = ml[i].x;
-                const float4 y = *reinterpret_cast<const float4 *>(a.part_o + (pr.slot(i) * ATT_R + r) * j.d + x);
+                const float4 y = *reinterpret_cast<const float4 *>(a.part_o + (int64_t)(pr.slot(i) * ATT_R + r) * j.d + x);
                 s.x += f * y.x, s.y += f * y.y, s.z += f * y.z, s.w += f * y.w;
             }
             *reinterpret_cast<float4 *>(&acc[warp][x]) = s;
@@ -116,13 +116,13 @@ template <typename IO> __global__ void __launch_bounds__(AJ_THREADS) attn_join_k
         }
         return;
     }
-    // weights of entries [i0, i0 + AJ_CHUNK) of one (sequence, kv head)
-    const unsigned w = blockIdx.x - j.n_out;
-    const int u = (int)(w / j.chunks), b = u / a.KVH, kvh = u - b * a.KVH, i0 = (int)(w - (unsigned)u * j.chunks) * AJ_CHUNK;
-    const int len = attn_len(a, b);
+    // weights of entries [i0, i0 + AJ_CHUNK) of one (sequence, kv head), four
+    // consecutive ones per thread
+    const int w = blockIdx.x - j.n_out, u = w / j.chunks, b = u / a.KVH, kvh = u - b * a.KVH, i0 = (w - u * j.chunks) * AJ_CHUNK;
+    const int len = attn_len(a, b), i = i0 + 4 * tid;
     if (i0 >= len) return;
     const int nt = a.prefix[b + 1] - a.prefix[b];
-    float add[AJ_CHUNK / AJ_THREADS] = {};
+    float4 add = make_float4(0, 0, 0, 0);
     for (int g0 = 0; g0 < a.G; g0 += 128) {  // ml holds 128 heads at a time
         const int ng = min(a.G - g0, 128);
         for (int g = warp; g < ng; g += AJ_THREADS / 32) {
@@ -131,22 +131,26 @@ template <typename IO> __global__ void __launch_bounds__(AJ_THREADS) attn_join_k
             if (lane == 0) ml[g] = make_float2(e.x == -INFINITY ? 0.0f : e.x, e.y > 0.0f || e.y != e.y ? 1.0f / e.y : 0.0f);
         }
         __syncthreads();
-        const float *z = a.z + ((int64_t)b * a.H + kvh * a.G + g0) * a.z_stride + i0 + tid;
-        for (int g = 0; g < ng; g++, z += a.z_stride) {
-            const float2 e = ml[g];
-#pragma unroll
-            for (int k = 0; k < AJ_CHUNK / AJ_THREADS; k++)
-                if (i0 + k * AJ_THREADS + tid < len) add[k] += exp2_fast(z[k * AJ_THREADS] - e.x) * e.y;
+        // scores are there up to the end of the last tile of 16
+        if (i < len) {
+            const float *z = a.z + ((int64_t)b * a.H + kvh * a.G + g0) * a.z_stride + i;
+#pragma unroll 4
+            for (int g = 0; g < ng; g++) {
+                const float2 e = ml[g];
+                const float4 x = *reinterpret_cast<const float4 *>(z + g * a.z_stride);
+                add.x += exp2_fast(x.x - e.x) * e.y, add.y += exp2_fast(x.y - e.x) * e.y;
+                add.z += exp2_fast(x.z - e.x) * e.y, add.w += exp2_fast(x.w - e.x) * e.y;
+            }
         }
         __syncthreads();
     }
+    const float v[4] = {add.x, add.y, add.z, add.w};
 #pragma unroll
-    for (int k = 0; k < AJ_CHUNK / AJ_THREADS; k++) {
-        const int i = i0 + k * AJ_THREADS + tid;
-        if (i >= len) continue;
-        const int col = a.page.div(i), page = a.table[(int64_t)b * a.max_pages + col];
+    for (int k = 0; k < 4; k++) {
+        if (i + k >= len) break;
+        const int col = a.page.div(i + k), page = a.table[(int64_t)b * a.max_pages + col];
         if (page < 0 || page >= a.n_pages) continue;
-        a.weight[((int64_t)page * a.KVH + kvh) * a.page_size + (i - col * a.page_size)] += add[k];
+        a.weight[((int64_t)page * a.KVH + kvh) * a.page_size + (i + k - col * a.page_size)] += v[k];
     }
 }
 
@@ -175,7 +179,8 @@ static int attn_plan(const ofb_kv_cache *c, int n_heads, int n_seqs, int max_len
     const int reach = cache_reach(c);
     p.max_len = max_len && max_len < reach ? max_len : reach;
     const int64_t tiles = ((int64_t)p.max_len + ATT_TILE - 1) / ATT_TILE;
-    if (tiles * n_seqs > INT32_MAX) {
+    p.NB = (n_heads / c->n_kv_heads + ATT_R - 1) / ATT_R;
+    if (tiles * n_seqs > INT32_MAX / ((int64_t)c->n_kv_heads * p.NB)) {
         set_error("ofb_attn_decode: %d sequences of %d entries are too many tiles", n_seqs, p.max_len);
         return OFB_ETOOLARGE;
     }
@@ -187,7 +192,6 @@ static int attn_plan(const ofb_kv_cache *c, int n_heads, int n_seqs, int max_len
     case 192: p.v = attn_variant_192(bf, f32); break;
     default: p.v = attn_variant_256(bf, f32); break;
     }
-    p.NB = (n_heads / c->n_kv_heads + ATT_R - 1) / ATT_R;
     const int64_t runs = (tiles * n_seqs * c->n_kv_heads * p.NB + ATT_W - 1) / ATT_W;
     const int most = sm_count() * p.v.ctas < AJ_MAX_CTAS ? sm_count() * p.v.ctas : AJ_MAX_CTAS;
     // Short sequences: as many CTAs as give each warp ATT_SHORT tiles at most,

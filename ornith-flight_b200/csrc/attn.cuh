@@ -49,6 +49,10 @@ namespace cg = cooperative_groups;
 
 namespace ofb {
 
+#ifndef V_S
+#define V_S 3
+#define V_C 2
+#endif
 constexpr int ATT_W = 4;      // warps per CTA
 constexpr int ATT_TILE = 16;  // entries per tile
 constexpr int ATT_R = 8;      // query heads per pass
@@ -84,16 +88,16 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2 steps at most; below
 __device__ __forceinline__ int attn_len(const AttnArgs &a, int b) { return min(max(a.lens[b], 0), a.max_len); }
 // Tiles per CTA when `total` tiles are dealt to `ctas` CTAs: at least one per
 // warp, so that few tiles do not leave many parts to join.
-__host__ __device__ __forceinline__ long long attn_run(long long total, int ctas) {
-    const long long n = (total + ctas - 1) / ctas;
+__host__ __device__ __forceinline__ int attn_run(int total, int ctas) {
+    const int n = total / ctas + (total % ctas != 0);
     return n < ATT_W ? ATT_W : n;
 }
 
 template <int D> struct AttnShape {
     static constexpr int PITCH = D * 2 + 16;                 // bytes of a row in shared memory
     static constexpr int TILE_BYTES = 2 * ATT_TILE * PITCH;  // K, then V
-    static constexpr int S = D <= 64 ? 5 : D <= 96 ? 4 : D <= 128 ? 3 : D <= 192 ? 4 : 3;  // ring slots
-    static constexpr int CTAS = D <= 128 ? 2 : 1;            // per SM
+    static constexpr int S = D <= 64 ? 5 : D <= 96 ? 4 : D <= 128 ? V_S : D <= 192 ? 4 : 3;  // ring slots
+    static constexpr int CTAS = D <= 96 ? 2 : D <= 128 ? V_C : 1;            // per SM
     static constexpr int RING = ATT_W * S * TILE_BYTES;
     // behind the ring: the warps' and the CTA's (maximum, sum), then per sequence
     // the tiles before it and the entries of its last tile
@@ -107,14 +111,14 @@ template <int D> struct AttnShape {
 template <typename T> struct Mma;
 template <> struct Mma<__nv_bfloat16> {
     static __device__ __forceinline__ void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
 };
 template <> struct Mma<__half> {
     static __device__ __forceinline__ void run(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-        asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
     }
@@ -175,22 +179,22 @@ struct AttnPart {
     int b, vh, t, end, nt, len;
 };
 // The part that begins at tile `f` of the row of all tiles, cut at f1.
-__device__ __forceinline__ AttnPart attn_part(const int *prefix, const uint8_t *last, int B, int nvh, long long f, long long f1) {
+__device__ __forceinline__ AttnPart attn_part(const int *prefix, const uint8_t *last, int B, int nvh, int f, int f1) {
     int lo = 0, hi = B - 1;  // the last sequence that begins at or before f (and has tiles)
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if ((long long)prefix[mid] * nvh <= f) lo = mid;
+        if (prefix[mid] * nvh <= f) lo = mid;
         else hi = mid - 1;
     }
     AttnPart p;
     p.b = lo;
     p.nt = prefix[lo + 1] - prefix[lo];
     p.len = (p.nt - 1) * ATT_TILE + last[lo];
-    const long long r = f - (long long)prefix[lo] * nvh;
-    p.vh = (int)(r / p.nt);
-    p.t = (int)(r - (long long)p.vh * p.nt);
-    const long long left = f1 - f;
-    p.end = left < p.nt - p.t ? p.t + (int)left : p.nt;
+    const int r = f - prefix[lo] * nvh;
+    p.vh = r / p.nt;
+    p.t = r - p.vh * p.nt;
+    const int left = f1 - f;
+    p.end = left < p.nt - p.t ? p.t + left : p.nt;
     return p;
 }
 
@@ -221,7 +225,7 @@ __global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_ker
     pdl_trigger();
 
     const int nvh = a.KVH * a.NB;
-    long long f0 = 0, f1 = 1;
+    int f0 = 0, f1 = 1;
     AttnPart first;
     if constexpr (CLUSTER) {
         const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank(), u = blockIdx.x / C;
@@ -230,8 +234,8 @@ __global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_ker
         if (a.lens[first.b] > a.max_len && first.vh == 0 && rank == 0 && tid == 0) report(a.errors, OFB_CACHE_ELEN);
         first.len = attn_len(a, first.b);
         first.nt = (first.len + ATT_TILE - 1) / ATT_TILE;
-        first.t = (int)((long long)rank * first.nt / C);
-        first.end = (int)((long long)(rank + 1) * first.nt / C);
+        first.t = (int)((int64_t)rank * first.nt / C);
+        first.end = (int)((int64_t)(rank + 1) * first.nt / C);
     } else {
         // tiles before each sequence; every CTA forms them for itself
         for (int base = 0; base < a.B; base += ATT_W * 32) {
@@ -263,8 +267,9 @@ __global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_ker
         for (int b = blockIdx.x; b < a.B; b += gridDim.x)
             if (prefix[b + 1] == prefix[b])
                 for (int i = tid; i < a.H * D; i += ATT_W * 32) static_cast<IO *>(a.out)[b * a.out_stride + i] = from_f32<IO>(0.0f);
-        const long long total = (long long)prefix[a.B] * nvh, run = attn_run(total, gridDim.x);
-        f0 = blockIdx.x * run, f1 = min(total, f0 + run);
+        const int total = prefix[a.B] * nvh, run = attn_run(total, gridDim.x);
+        // (the last run's end may lie past 31 bits)
+        f0 = (int)min((int64_t)blockIdx.x * run, (int64_t)total), f1 = f0 + min(run, total - f0);
         if (f0 >= f1) return;
         first = attn_part(prefix, last, a.B, nvh, f0, f1);
     }
@@ -273,7 +278,7 @@ __global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_ker
     // The tile that the ring is filled with next: its part, number, and its
     // rows' entries (lanes 0..15) with the page numbers already asked for.
     AttnPart lp = first;
-    long long lf = f0;
+    int lf = f0;
     int lt = lp.t + warp, l_entry = 0, l_page = -1;
     bool more = true;
     auto look_up = [&]() {
@@ -299,13 +304,22 @@ __global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_ker
                 const int rows = off < 0 ? 0 : min(ATT_TILE, lp.len - l_entry);
                 const CT *ks = k + (off < 0 ? 0 : off) + lane * 8, *vs = v + (off < 0 ? 0 : off) + lane * 8;
                 if (lane == 0) valid[warp][slot] = (1u << rows) - 1u;
+if (rows == ATT_TILE) {
 #pragma unroll
-                for (int j = 0; j < ATT_TILE * CH / 32; j++) {
-                    const int c = j * 32 + lane, r = c / CH, x = c - r * CH;
-                    const bool in_row = r < rows;
-                    // a row that is not there is not read: its address need not exist
-                    cp16(dst + r * SH::PITCH + x * 16, in_row ? ks + j * 256 : k, in_row ? 16 : 0);
-                    cp16(dst + (ATT_TILE + r) * SH::PITCH + x * 16, in_row ? vs + j * 256 : v, in_row ? 16 : 0);
+                    for (int j = 0; j < ATT_TILE * CH / 32; j++) {
+                        const int c = j * 32 + lane, r = c / CH, x = c - r * CH;
+                        cp16(dst + r * SH::PITCH + x * 16, ks + j * 256, 16);
+                        cp16(dst + (ATT_TILE + r) * SH::PITCH + x * 16, vs + j * 256, 16);
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < ATT_TILE * CH / 32; j++) {
+                        const int c = j * 32 + lane, r = c / CH, x = c - r * CH;
+                        const bool in_row = r < rows;
+                        // a row that is not there is not read: its address need not exist
+                        cp16(dst + r * SH::PITCH + x * 16, in_row ? ks + j * 256 : k, in_row ? 16 : 0);
+                        cp16(dst + (ATT_TILE + r) * SH::PITCH + x * 16, in_row ? vs + j * 256 : v, in_row ? 16 : 0);
+                    }
                 }
             } else {
                 const uint32_t mask = __ballot_sync(0xffffffffu, off >= 0);
@@ -331,7 +345,7 @@ __global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_ker
     int slot = 0;  // of the next tile to compute
 
     int npart = 0;
-    for (long long f = f0; f < f1; npart++) {
+    for (int f = f0; f < f1; npart++) {
         const AttnPart p = npart ? attn_part(prefix, last, a.B, nvh, f, f1) : first;
         const int kvh = p.vh / a.NB, h0 = (p.vh - kvh * a.NB) * ATT_R, rows = min(ATT_R, a.G - h0);
         // queries: row g of A, parts as told at the top

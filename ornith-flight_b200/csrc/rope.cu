@@ -24,9 +24,15 @@ namespace ofb {
 
 constexpr int RP_THREADS = 256;
 constexpr int RP_PAIRS = 128;
+constexpr int RP_TOKENS = 1 << 30;
+#ifndef V_RP
+#define V_RP 2
+#endif
+constexpr int RP_CTAS = V_RP;  // per SM
 
 struct RopeArgs {
-    int T, H, KVH, d, rot, tpb;  // heads of q; kv heads (0: no cache); tokens per CTA
+    int T, H, KVH, d, rot, tpb;  // heads of q; kv heads (0: no cache); tokens of a group
+    int shared;                  // floats of RopeShared
     int n_pages, page_size, n_seqs, max_pages;
     FastDiv page, rows;  // by page_size, by H + 2 KVH
     const void *q, *k, *v;
@@ -40,16 +46,16 @@ struct RopeArgs {
     uint8_t axis[RP_PAIRS];
 };
 
-// Where a CTA's tokens go: page -1 where nothing is written.
+// Where a CTA's tokens go (a page below 0: nowhere) and their order numbers.
 struct RopeEntry {
-    int page, slot;
+    int page, slot, number, asked;
 };
 // Shared memory: cosines [tpb][rot/2], sines [tpb][rot/2], entries [tpb].
 struct RopeShared {
     float *c, *s;
     RopeEntry *entry;
     __device__ __forceinline__ RopeShared(const RopeArgs &a, float *base)
-        : c(base), s(base + a.tpb * (a.rot / 2)), entry(reinterpret_cast<RopeEntry *>(base + a.tpb * a.rot)) {}
+        : c(base), s(base + a.tpb * (a.rot / 2)), entry(reinterpret_cast<RopeEntry *>(base + (a.tpb * a.rot + 3) / 4 * 4)) {}
 };
 
 __device__ __forceinline__ void rope_setup(const RopeArgs &a, int t0, int nt, const RopeShared &sh) {
@@ -69,7 +75,7 @@ __device__ __forceinline__ void rope_setup(const RopeArgs &a, int t0, int nt, co
     }
     if (a.KVH && threadIdx.x < nt) {
         const int t = t0 + threadIdx.x, b = a.seq[t], i = a.index[t];
-        RopeEntry e = {-1, 0};
+        RopeEntry e = {-1, 0, 0, 0};
         if (b >= 0) {
             const int col = i < 0 ? 0 : a.page.div(i);
             if (b >= a.n_seqs || i < 0 || col >= a.max_pages) {
@@ -77,7 +83,7 @@ __device__ __forceinline__ void rope_setup(const RopeArgs &a, int t0, int nt, co
             } else {
                 const int p = a.table[(int64_t)b * a.max_pages + col];
                 if (p < 0 || p >= a.n_pages) report(a.errors, OFB_CACHE_EPAGE);
-                else e = {p, i - col * a.page_size};
+                else e = {p, i - col * a.page_size, a.number ? a.number[t] : i, 0};
             }
         }
         sh.entry[threadIdx.x] = e;
@@ -86,108 +92,228 @@ __device__ __forceinline__ void rope_setup(const RopeArgs &a, int t0, int nt, co
 }
 
 // Weight 0 and the order number of the CTA's new entries.
-__device__ __forceinline__ void rope_meta(const RopeArgs &a, int t0, int nt, const RopeEntry *entry) {
+__device__ __forceinline__ void rope_meta(const RopeArgs &a, int nt, const RopeEntry *entry) {
     if (!a.weight && !a.order) return;
-    for (int i = threadIdx.x; i < nt * a.KVH; i += RP_THREADS) {
+    // from the last thread down: the first ones look pages up
+    for (int i = RP_THREADS - 1 - threadIdx.x; i < nt * a.KVH; i += RP_THREADS) {
         const int t = i / a.KVH, h = i - t * a.KVH;
         const RopeEntry e = entry[t];
         if (e.page < 0) continue;
         const int64_t m = ((int64_t)e.page * a.KVH + h) * a.page_size + e.slot;
         if (a.weight) a.weight[m] = 0.0f;
-        if (a.order) a.order[m] = a.number ? a.number[t0 + t] : a.index[t0 + t];
+        if (a.order) a.order[m] = e.number;
     }
 }
 
-// A row of the launch: query, key or value row of one token.
+// A row of the launch: row `row` of token t of the group, the queries first,
+// then the keys and the values.
 struct RopeRow {
-    int t, h;
-    bool is_q, is_v;
+    int t, row;
 };
 __device__ __forceinline__ RopeRow rope_row(const RopeArgs &a, int vr) {
-    RopeRow r;
-    r.t = a.rows.div(vr);
-    const int row = vr - r.t * (int)a.rows.d;
-    r.is_q = row < a.H;
-    r.is_v = row >= a.H + a.KVH;
-    r.h = row - (r.is_q ? 0 : r.is_v ? a.H + a.KVH : a.H);
-    return r;
+    const int t = a.rows.div(vr);
+    return {t, vr - t * (int)a.rows.d};
 }
 template <typename IO> __device__ __forceinline__ const IO *rope_src(const RopeArgs &a, const RopeRow &r, int t0) {
-    const void *p = r.is_q ? a.q : r.is_v ? a.v : a.k;
-    const int64_t stride = r.is_q ? a.qs : r.is_v ? a.vs : a.ks;
-    return static_cast<const IO *>(p) + (t0 + r.t) * stride + (int64_t)r.h * a.d;
+    const bool is_q = r.row < a.H, is_v = r.row >= a.H + a.KVH;
+    const void *p = is_q ? a.q : is_v ? a.v : a.k;
+    const int64_t stride = is_q ? a.qs : is_v ? a.vs : a.ks;
+    const int h = r.row - (is_q ? 0 : is_v ? a.H + a.KVH : a.H);
+    return static_cast<const IO *>(p) + (t0 + r.t) * stride + (int64_t)h * a.d;
 }
 __device__ __forceinline__ int64_t rope_cache_at(const RopeArgs &a, const RopeEntry &e, int h) {
     return e.page * a.page_stride + ((int64_t)h * a.page_size + e.slot) * a.d;
 }
 
-// Thread (slot, j) takes chunk pair j of rows slot, slot + slots, ...; the next
-// row's chunks are on their way while one is turned, the first while the
-// cosines are formed.
+// Sixteen elements of a row as loaded.
+template <typename IO> struct RopeRaw {
+    uint4 x[sizeof(IO) / 2], y[sizeof(IO) / 2];
+    __device__ __forceinline__ void load(const IO *p, int at, int bt) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(IO) / 2; i++) {
+            x[i] = reinterpret_cast<const uint4 *>(p + at)[i];
+            y[i] = reinterpret_cast<const uint4 *>(p + bt)[i];
+        }
+    }
+};
+
+// CTAs go round over the groups of tpb tokens. Thread (slot, j) takes chunk
+// pair j of rows slot, slot + slots, ... of a group in batches; as soon as an
+// item is unpacked the same item of the next batch (or of the next group's
+// first) is asked for, so that loads never run dry. A group's cosines are formed
+// from positions that were asked for a group earlier (and page numbers, from
+// places asked for two groups earlier), into the half of the shared memory that
+// the group before does not read: one barrier per group.
 template <typename IO, typename CT, bool ADJ>
-__global__ void __launch_bounds__(RP_THREADS) rope_vec_kernel(const __grid_constant__ RopeArgs a) {
+__global__ void __launch_bounds__(RP_THREADS, RP_CTAS) rope_vec_kernel(const __grid_constant__ RopeArgs a) {
+    constexpr int BATCH = sizeof(IO) == 2 ? 4 : 2;
     extern __shared__ __align__(16) float rope_smem[];
-    const RopeShared sh(a, rope_smem);
+    const int half = a.rot / 2, tid = threadIdx.x;
     pdl_wait();
     pdl_trigger();
-    const int t0 = blockIdx.x * a.tpb, nt = min(a.tpb, a.T - t0), half = a.rot / 2;
-    const int per_row = a.d / 16, slots = RP_THREADS / per_row, slot = threadIdx.x / per_row, j = threadIdx.x - slot * per_row;
-    const int total = slot < slots ? nt * (int)a.rows.d : 0;
-    // chunk places: of a turned row the two halves of 8 pairs, or 16 neighbours
-    const bool in_rot = j * 16 < a.rot;
-    const int ta = in_rot && !ADJ ? 8 * j : 16 * j, tb = in_rot && !ADJ ? half + 8 * j : 16 * j + 8;
-    float x[8], y[8], nx[8], ny[8];
-    RopeRow r = {}, nr = {};
-    if (slot < total) {
-        r = rope_row(a, slot);
-        const IO *src = rope_src<IO>(a, r, t0);
-        load8(src + ta, x);
-        load8(src + tb, y);
+    const int per_row = a.d / 16, slots = RP_THREADS / per_row, slot = tid / per_row, j = tid - slot * per_row;
+    // The thread's two chunks of 8 elements and where their cosines are. HALVES:
+    // the two halves of 8 pairs, or two chunks behind rot; ADJACENT: 4 pairs
+    // each, half a row apart. Neighbouring threads have neighbouring chunks.
+    int ta, tb;
+    bool turn_a, turn_b;
+    if (ADJ) {
+        ta = 8 * j, tb = a.d / 2 + 8 * j;
+        turn_a = ta < a.rot, turn_b = tb < a.rot;
+    } else {
+        const int pr = a.rot / 16, rest = (a.d - a.rot) / 2;
+        turn_a = turn_b = j < pr;
+        ta = turn_a ? 8 * j : a.rot + 8 * (j - pr), tb = ta + (turn_a ? half : rest);
     }
-    rope_setup(a, t0, nt, sh);
-    for (int vr = slot; vr < total; vr += slots) {
-        if (vr + slots < total) {
-            nr = rope_row(a, vr + slots);
-            const IO *src = rope_src<IO>(a, nr, t0);
-            load8(src + ta, nx);
-            load8(src + tb, ny);
+    const int dt = slots / (int)a.rows.d, drow = slots - dt * (int)a.rows.d;  // from one item's row to the next's
+    // the (token, pair)s whose cosines this thread forms: tpb * rot/2 <= 2 RP_THREADS
+    const int n_cs = a.tpb * half;
+    int ct[2] = {0, 0};
+    int64_t cpos[2] = {0, 0};
+    double cf[2] = {0.0, 0.0};
+    {
+        const double *freq = a.half_turns;  // see rope_setup
+        const uint8_t *axis = a.axis;
+        asm("" : "+l"(freq), "+l"(axis));
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int i = tid + k * RP_THREADS;
+            if (i < n_cs) {
+                ct[k] = i / half;
+                const int p = i - ct[k] * half;
+                cpos[k] = axis[p] * a.pos_stride + ct[k];
+                cf[k] = freq[p];
+            }
         }
-        if (in_rot && !r.is_v) {
-            float c[8], s[8];
-            load8(sh.c + r.t * half + 8 * j, c);
-            load8(sh.s + r.t * half + 8 * j, s);
-            if (ADJ) {
+    }
+    int pos[2] = {0, 0}, seq = -1, index = 0, number = 0;
+    auto ask_pos = [&](int t0) {
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const float u = x[2 * i], v = x[2 * i + 1], m = y[2 * i], n = y[2 * i + 1];
-                    x[2 * i] = u * c[i] - v * s[i];
-                    x[2 * i + 1] = v * c[i] + u * s[i];
-                    y[2 * i] = m * c[4 + i] - n * s[4 + i];
-                    y[2 * i + 1] = n * c[4 + i] + m * s[4 + i];
+        for (int k = 0; k < 2; k++)
+            if (tid + k * RP_THREADS < n_cs && t0 + ct[k] < a.T) pos[k] = a.pos[cpos[k] + t0];
+    };
+    auto ask_place = [&](int t0) {
+        seq = -1;
+        if (a.KVH && tid < a.tpb && t0 + tid < a.T) {
+            seq = a.seq[t0 + tid], index = a.index[t0 + tid];
+            if (a.number) number = a.number[t0 + tid];
+        }
+    };
+    RopeEntry at = {-1, 0, 0, 0};
+    auto ask_page = [&]() {  // uses seq, index and number
+        at.page = -1;
+        if (seq < 0) return;
+        const int col = index < 0 ? 0 : a.page.div(index);
+        if (seq >= a.n_seqs || index < 0 || col >= a.max_pages) {
+            report(a.errors, OFB_CACHE_EINDEX);
+        } else {
+            at = {a.table[(int64_t)seq * a.max_pages + col], index - col * a.page_size, a.number ? number : index, 1};
+        }
+    };
+    const int step = gridDim.x * a.tpb;
+    int t0 = blockIdx.x * a.tpb, half_at = 0;
+    ask_pos(t0);
+    ask_place(t0);
+    ask_page();
+    ask_place(t0 + step);
+    RopeRaw<IO> raw[BATCH];
+    auto rows_of = [&](int t) { return slot < slots && t < a.T ? min(a.tpb, a.T - t) * (int)a.rows.d : 0; };
+    auto advance = [&](RopeRow &r) {
+        r.t += dt, r.row += drow;
+        if (r.row >= (int)a.rows.d) r.row -= (int)a.rows.d, r.t++;
+    };
+    RopeRow ask, now;  // the row asked for next, the row worked on
+    int total = rows_of(t0);
+    now = ask = rope_row(a, slot);
+#pragma unroll
+    for (int k = 0; k < BATCH; k++) {
+        if (slot + k * slots < total) raw[k].load(rope_src<IO>(a, ask, t0), ta, tb);
+        advance(ask);
+    }
+    for (; t0 < a.T; t0 += step, half_at ^= 1) {
+        const int nt = min(a.tpb, a.T - t0), total_next = rows_of(t0 + step);
+        const RopeShared sh(a, rope_smem + half_at * a.shared);
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+            const int i = tid + k * RP_THREADS;
+            if (i >= n_cs) break;
+            const double h = (double)pos[k] * cf[k];
+            float s, c;
+            sincospif((float)(h - 2.0 * rint(0.5 * h)), &s, &c);
+            sh.c[i] = c;
+            sh.s[i] = s;
+        }
+        if (tid < nt) {
+            if (at.asked && (at.page < 0 || at.page >= a.n_pages)) {
+                report(a.errors, OFB_CACHE_EPAGE);
+                at.page = -1;
+            }
+            sh.entry[tid] = at;
+            at.asked = 0;
+        }
+        __syncthreads();
+        ask_pos(t0 + step);
+        ask_page();
+        ask_place(t0 + 2 * step);
+        for (int vr = slot; vr < total; vr += BATCH * slots) {
+            // the batch after this one: of this group, or the next group's first
+            const bool here = vr + BATCH * slots < total;
+            const int t_next = here ? t0 : t0 + step, n_next = here ? total : total_next;
+            int v_next = here ? vr + BATCH * slots : slot;
+            if (!here) ask = rope_row(a, slot);
+#pragma unroll
+            for (int k = 0; k < BATCH; k++, v_next += slots) {
+                float x[8], y[8];
+                load8(reinterpret_cast<const IO *>(raw[k].x), x);
+                load8(reinterpret_cast<const IO *>(raw[k].y), y);
+                if (v_next < n_next) raw[k].load(rope_src<IO>(a, ask, t_next), ta, tb);
+                advance(ask);
+                const RopeRow r = now;
+                advance(now);
+                if (vr + k * slots >= total) continue;
+                const bool is_q = r.row < a.H, is_v = r.row >= a.H + a.KVH;
+                const float *cs = sh.c + r.t * half, *sn = sh.s + r.t * half;
+                if (ADJ) {
+                    auto turn4 = [&](float(&z)[8], int at) {
+                        const float4 c = *reinterpret_cast<const float4 *>(cs + at), s = *reinterpret_cast<const float4 *>(sn + at);
+                        const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            const float u = z[2 * i], v = z[2 * i + 1];
+                            z[2 * i] = u * cc[i] - v * ss[i];
+                            z[2 * i + 1] = v * cc[i] + u * ss[i];
+                        }
+                    };
+                    if (turn_a && !is_v) turn4(x, ta / 2);
+                    if (turn_b && !is_v) turn4(y, tb / 2);
+                } else if (turn_a && !is_v) {
+                    float c[8], s[8];
+                    load8(cs + 8 * j, c);
+                    load8(sn + 8 * j, s);
+#pragma unroll
+                    for (int i = 0; i < 8; i++) {
+                        const float u = x[i], v = y[i];
+                        x[i] = u * c[i] - v * s[i];
+                        y[i] = v * c[i] + u * s[i];
+                    }
                 }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float u = x[i], v = y[i];
-                    x[i] = u * c[i] - v * s[i];
-                    y[i] = v * c[i] + u * s[i];
+                if (is_q) {
+                    IO *dst = static_cast<IO *>(a.q_out) + (t0 + r.t) * a.qos + (int64_t)r.row * a.d;
+                    store8(dst + ta, x);
+                    store8(dst + tb, y);
+                } else {
+                    const RopeEntry e = sh.entry[r.t];
+                    if (e.page < 0) continue;
+                    CT *dst = static_cast<CT *>(is_v ? a.cv : a.ck) + rope_cache_at(a, e, r.row - a.H - (is_v ? a.KVH : 0));
+                    store8(dst + ta, x);
+                    store8(dst + tb, y);
                 }
             }
         }
-        if (r.is_q) {
-            IO *dst = static_cast<IO *>(a.q_out) + (t0 + r.t) * a.qos + (int64_t)r.h * a.d;
-            store8(dst + ta, x);
-            store8(dst + tb, y);
-        } else if (sh.entry[r.t].page >= 0) {
-            CT *dst = static_cast<CT *>(r.is_v ? a.cv : a.ck) + rope_cache_at(a, sh.entry[r.t], r.h);
-            store8(dst + ta, x);
-            store8(dst + tb, y);
-        }
-        r = nr;
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i] = nx[i], y[i] = ny[i];
+        now = rope_row(a, slot);
+        rope_meta(a, nt, sh.entry);
+        total = total_next;
     }
-    rope_meta(a, t0, nt, sh.entry);
 }
 
 // Any sizes and strides: items are pairs (rot/2 per row), then single elements.
@@ -203,27 +329,28 @@ __global__ void __launch_bounds__(RP_THREADS) rope_any_kernel(const __grid_const
     for (int it = threadIdx.x; it < total; it += RP_THREADS) {
         const int vr = it / per_row, j = it - vr * per_row;
         const RopeRow r = rope_row(a, vr);
-        if (!r.is_q && sh.entry[r.t].page < 0) continue;
+        const bool is_q = r.row < a.H, is_v = r.row >= a.H + a.KVH;
+        if (!is_q && sh.entry[r.t].page < 0) continue;
         const IO *src = rope_src<IO>(a, r, t0);
         // where this item's one or two elements are
         const int ea = j >= half ? half + j : adjacent ? 2 * j : j, eb = j >= half ? ea : adjacent ? 2 * j + 1 : half + j;
         float x = to_f32(src[ea]), y = to_f32(src[eb]);
-        if (!r.is_v && j < half) {
+        if (!is_v && j < half) {
             const float c = sh.c[r.t * half + j], s = sh.s[r.t * half + j], u = x, v = y;
             x = u * c - v * s;
             y = v * c + u * s;
         }
-        if (r.is_q) {
-            IO *dst = static_cast<IO *>(a.q_out) + (t0 + r.t) * a.qos + (int64_t)r.h * a.d;
+        if (is_q) {
+            IO *dst = static_cast<IO *>(a.q_out) + (t0 + r.t) * a.qos + (int64_t)r.row * a.d;
             dst[ea] = from_f32<IO>(x);
             dst[eb] = from_f32<IO>(y);
         } else {
-            CT *dst = static_cast<CT *>(r.is_v ? a.cv : a.ck) + rope_cache_at(a, sh.entry[r.t], r.h);
+            CT *dst = static_cast<CT *>(is_v ? a.cv : a.ck) + rope_cache_at(a, sh.entry[r.t], r.row - a.H - (is_v ? a.KVH : 0));
             dst[ea] = from_f32<CT>(x);
             dst[eb] = from_f32<CT>(y);
         }
     }
-    rope_meta(a, t0, nt, sh.entry);
+    rope_meta(a, nt, sh.entry);
 }
 
 // Checks a rotary form and lays out its pairs: axis and frequency / pi.
@@ -278,16 +405,19 @@ static int rope_tables(const ofb_rope_config *r, int head_dim, const char *who, 
 template <typename IO, typename CT> static cudaError_t rope_launch(RopeArgs &a, bool vec, bool adjacent, cudaStream_t s) {
     const int rows = a.H + 2 * a.KVH;
     const int64_t per_tok = (int64_t)rows * (vec ? a.d / 16 : a.d - a.rot / 2);
-    // three items per thread where a token alone does not give them, at most 8
-    // tokens (2 KB of cosines and sines each), and two CTAs per SM first
-    int tpb = (int)(3 * RP_THREADS / per_tok);
+    // one batch of items per thread where a token alone does not give them, at
+    // most 8 tokens (2 KB of cosines and sines each), and two CTAs per SM first
+    int tpb = (int)((sizeof(IO) == 2 ? 4 : 2) * RP_THREADS / per_tok);
     tpb = tpb < 1 ? 1 : tpb > 8 ? 8 : tpb;
+    while (tpb > 1 && tpb * (a.rot / 2) > 2 * RP_THREADS) tpb--;
     while (tpb > 1 && (a.T + tpb - 1) / tpb < 2 * sm_count()) tpb--;
     a.tpb = tpb;
     a.rows = fast_div(rows);
     a.page = fast_div(a.page_size ? a.page_size : 1);
-    const size_t smem = (size_t)tpb * (a.rot * sizeof(float) + sizeof(RopeEntry));
-    const dim3 grid((a.T + tpb - 1) / tpb), block(RP_THREADS);
+    a.shared = (tpb * a.rot + 3) / 4 * 4 + tpb * (int)(sizeof(RopeEntry) / sizeof(float));
+    const size_t smem = (size_t)(vec ? 2 : 1) * a.shared * sizeof(float);
+    const int groups = (a.T + tpb - 1) / tpb, most = RP_CTAS * sm_count();
+    const dim3 grid(vec && groups > most ? most : groups), block(RP_THREADS);
     if (!vec) return launch_pdl(rope_any_kernel<IO, CT>, grid, block, smem, s, a, (int)adjacent);
     return adjacent ? launch_pdl(rope_vec_kernel<IO, CT, true>, grid, block, smem, s, a)
                     : launch_pdl(rope_vec_kernel<IO, CT, false>, grid, block, smem, s, a);
@@ -319,6 +449,7 @@ extern "C" int ofb_rope(const ofb_rope_config *rope, const void *x, int type, in
                   (long long)pos_stride);
         return OFB_EINVAL;
     }
+    if (n_tokens > RP_TOKENS) { set_error("ofb_rope: %d tokens, %d at most", n_tokens, RP_TOKENS); return OFB_ETOOLARGE; }
     RopeArgs a = {};
     int st = rope_tables(rope, head_dim, "ofb_rope", a);
     if (st != OFB_OK) return st;
@@ -362,6 +493,7 @@ extern "C" int ofb_rope_append(const ofb_kv_cache *cache, const ofb_rope_config 
                   (long long)k_stride, (long long)v_stride, (long long)q_out_stride, (long long)pos_stride);
         return OFB_EINVAL;
     }
+    if (n_tokens > RP_TOKENS) { set_error("ofb_rope_append: %d tokens, %d at most", n_tokens, RP_TOKENS); return OFB_ETOOLARGE; }
     RopeArgs a = {};
     if (rope && (st = rope_tables(rope, d, "ofb_rope_append", a)) != OFB_OK) return st;
     if (!n_tokens) return OFB_OK;
