@@ -1,156 +1,214 @@
 // attn.cu — ofb_attn_decode: the join of the split kernel's parts (attn.cuh)
 // and the entry point.
 //
-// Second launch (programmatic, its CTAs come up as the split kernel's leave):
-// one CTA per query head joins the parts of a head that more than one CTA
-// worked on,
+// Second launch (programmatic, its CTAs come up as the split kernel's leave): the
+// parts of a head that more than one run holds are joined in the order of the runs,
 //   M = max m_i, out = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i,
-// in the order of the parts, so the result does not depend on timing. With
-// `accumulate`, further CTAs add each entry's probability, summed over the
-// query heads of its kv head in their order, to the cache's weight: they read
-// the scores the split kernel left (4 bytes per entry and query head, an
-// eighth of the entry's K and V at 8 heads of 128; forming them again would
-// read all of K a second time).
+// so the result does not depend on which CTA took which run, nor on when. A CTA
+// takes one head, its warps every eighth part, where a head has many parts, and
+// eight heads of a kv head, a warp each, where it has few. With `accumulate`,
+// further CTAs add each entry's probability, summed over the query heads of its
+// kv head in their order, to the cache's weight: they read the scores the split
+// kernel left (4 bytes per entry and query head, an eighth of the entry's K and V
+// at 8 heads of 128; forming them again would read all of K a second time).
 #include "attn.cuh"
 
 namespace ofb {
 
 constexpr int AJ_THREADS = 256;
-constexpr int AJ_CHUNK = 4 * AJ_THREADS;  // entries of one weight CTA
-constexpr int AJ_MAX_CTAS = 1024;  // of the split kernel
+constexpr int AJ_TURNS = 2;
+constexpr int AJ_CHUNK = AJ_TURNS * 4 * AJ_THREADS;  // entries of one weight CTA
 
 struct AttnJoinArgs {
     AttnArgs a;
-    int ctas, d, n_out, chunks;  // CTAs of the split kernel; join CTAs, weight CTAs per (sequence, kv head)
+    int ctas, warps, d;       // of the split kernel: CTAs, warps of each; head_dim
+    int wide, n_out, chunks;  // one head per CTA; join CTAs; weight CTAs per (sequence, kv head)
 };
 
-// Where the parts of (sequence b, pass vh) are: CTAs c0..c1 of the split kernel.
+// The runs that hold parts of (sequence b, pass vh): n of them from CTA c0's on.
 struct PartRange {
-    int c0, c1, f0, run;
-    __device__ __forceinline__ int slot(int i) const { return 2 * (c0 + i) + (i == 0 && c0 * run < f0 ? 1 : 0); }
+    AttnSplit sp;
+    int f0, n, c0;
+    __device__ __forceinline__ int slot(int i) const { return 2 * (c0 + i) + (i == 0 && sp.first(c0) < f0 ? 1 : 0); }
 };
 __device__ __forceinline__ PartRange part_range(const AttnJoinArgs &j, int b, int vh, int nt) {
     const int nvh = j.a.KVH * j.a.NB;
     PartRange r;
-    r.run = attn_run(j.a.prefix[j.a.B] * nvh, j.ctas);
+    r.sp = AttnSplit::make(j.a.prefix[j.a.B] * nvh, j.ctas, j.warps);
     r.f0 = j.a.prefix[b] * nvh + vh * nt;
-    r.c0 = r.f0 / r.run;
-    r.c1 = (r.f0 + nt - 1) / r.run;
+    r.c0 = r.f0 / r.sp.run;
+    r.n = (r.f0 + nt - 1) / r.sp.run - r.c0 + 1;
     return r;
 }
 
 // Maximum and sum of exponentials over the parts of row r, by one warp.
 __device__ __forceinline__ float2 warp_ml(const AttnJoinArgs &j, const PartRange &pr, int r, int lane) {
-    const int n = (int)(pr.c1 - pr.c0) + 1;
     float m = -INFINITY;
-    for (int i = lane; i < n; i += 32) m = fmaxf(m, j.a.part_ml[pr.slot(i) * ATT_R + r].x);
+    for (int i = lane; i < pr.n; i += 32) m = fmaxf(m, j.a.part_ml[pr.slot(i) * ATT_R + r].x);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float ref = m == -INFINITY ? 0.0f : m;
     float l = 0.0f;
-    for (int i = lane; i < n; i += 32) {
+    for (int i = lane; i < pr.n; i += 32) {
         const float2 e = j.a.part_ml[pr.slot(i) * ATT_R + r];
         l += exp2_fast(e.x - ref) * e.y;
     }
     return make_float2(ref, warp_sum(l));
 }
 
+// Sums over parts w, w + step, ... of row r, by one warp: lane x4 has columns
+// 4 lane .. and, with more than 128 columns, 128 + 4 lane ..
+struct JoinSum {
+    float m, l;
+    float4 o[2];
+    __device__ __forceinline__ void add(const AttnJoinArgs &j, const PartRange &pr, int r, int w, int step, int lane) {
+        m = -INFINITY, l = 0.0f;
+        o[0] = o[1] = make_float4(0, 0, 0, 0);
+        constexpr int UN = 4;
+        for (int i0 = w; i0 < pr.n; i0 += UN * step) {
+            float2 e[UN];
+            float4 y[UN][2];
+#pragma unroll
+            for (int k = 0; k < UN; k++) {
+                const int i = i0 + k * step;
+                e[k] = make_float2(-INFINITY, 0.0f);
+                y[k][0] = y[k][1] = make_float4(0, 0, 0, 0);
+                if (i < pr.n) {
+                    const int p = pr.slot(i) * ATT_R + r;
+                    const float *src = j.a.part_o + (int64_t)p * j.d;
+                    e[k] = j.a.part_ml[p];
+                    if (4 * lane < j.d) y[k][0] = *reinterpret_cast<const float4 *>(src + 4 * lane);
+                    if (128 + 4 * lane < j.d) y[k][1] = *reinterpret_cast<const float4 *>(src + 128 + 4 * lane);
+                }
+            }
+            float mn = m;
+#pragma unroll
+            for (int k = 0; k < UN; k++) mn = fmaxf(mn, e[k].x);
+            const float ref = mn == -INFINITY ? 0.0f : mn, old = exp2_fast(m - ref);
+            m = mn;
+            l *= old;
+#pragma unroll
+            for (int h = 0; h < 2; h++) o[h].x *= old, o[h].y *= old, o[h].z *= old, o[h].w *= old;
+#pragma unroll
+            for (int k = 0; k < UN; k++) {
+                const float f = exp2_fast(e[k].x - ref);
+                l += f * e[k].y;
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    o[h].x += f * y[k][h].x, o[h].y += f * y[k][h].y, o[h].z += f * y[k][h].z, o[h].w += f * y[k][h].w;
+            }
+        }
+    }
+};
+
 template <typename IO> __global__ void __launch_bounds__(AJ_THREADS) attn_join_kernel(const __grid_constant__ AttnJoinArgs j) {
-    __shared__ float acc[AJ_THREADS / 32][256 + 4];
-    __shared__ float2 ml[AJ_MAX_CTAS];  // join: (weight, -) of each part; weights: (maximum, 1 / sum) of a head
-    __shared__ float red[2][AJ_THREADS / 32];
+    constexpr int W = AJ_THREADS / 32;
+    __shared__ __align__(16) float acc[W][256 + 4];
+    __shared__ float2 ml[128];  // join: (maximum, sum) per warp; weights: (maximum, 1 / sum) of a head
     const AttnArgs &a = j.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_wait();
     pdl_trigger();
     if (blockIdx.x < j.n_out) {
-        const int b = blockIdx.x / a.H, h = blockIdx.x - b * a.H, kvh = h / a.G, g = h - kvh * a.G;
-        const int nt = a.prefix[b + 1] - a.prefix[b];
+        int b, vh, r;
+        if (j.wide) {
+            b = blockIdx.x / a.H;
+            const int h = blockIdx.x - b * a.H, kvh = h / a.G, g = h - kvh * a.G;
+            vh = kvh * a.NB + g / ATT_R, r = g % ATT_R;
+        } else {
+            b = blockIdx.x / (a.KVH * a.NB), vh = blockIdx.x - b * a.KVH * a.NB, r = warp;
+        }
+        const int kvh = vh / a.NB, g = (vh - kvh * a.NB) * ATT_R + r, nt = a.prefix[b + 1] - a.prefix[b];
         if (!nt) return;
-        const PartRange pr = part_range(j, b, kvh * a.NB + g / ATT_R, nt);
-        if (pr.c0 == pr.c1) return;
-        const int r = g % ATT_R, n = (int)(pr.c1 - pr.c0) + 1;
-        // the parts' weights 2^(m_i - M) and the sum of exponentials, by all threads
-        float m = -INFINITY, l = 0.0f;
-        for (int i = tid; i < n; i += AJ_THREADS) {
-            ml[i] = a.part_ml[pr.slot(i) * ATT_R + r];
-            m = fmaxf(m, ml[i].x);
-        }
+        const PartRange pr = part_range(j, b, vh, nt);
+        if (pr.n == 1 || g >= a.G) return;  // (`wide`: the CTA's only head, so all leave)
+        IO *const out = static_cast<IO *>(a.out) + b * a.out_stride + (int64_t)(kvh * a.G + g) * j.d;
+        JoinSum s;
+        s.add(j, pr, r, j.wide ? warp : 0, j.wide ? W : 1, lane);
+        if (!j.wide) {
+            const float inv = s.l > 0.0f || s.l != s.l ? 1.0f / s.l : 0.0f;
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (lane == 0) red[0][warp] = m;
-        __syncthreads();
-#pragma unroll
-        for (int w = 0; w < AJ_THREADS / 32; w++) m = fmaxf(m, red[0][w]);
-        const float ref = m == -INFINITY ? 0.0f : m;
-        for (int i = tid; i < n; i += AJ_THREADS) {
-            const float f = exp2_fast(ml[i].x - ref);
-            l += f * ml[i].y;
-            ml[i].x = f;
-        }
-        l = warp_sum(l);
-        if (lane == 0) red[1][warp] = l;
-        __syncthreads();
-        l = 0.0f;
-#pragma unroll
-        for (int w = 0; w < AJ_THREADS / 32; w++) l += red[1][w];
-        for (int x0 = 0; x0 < j.d; x0 += 128) {
-            const int x = x0 + lane * 4;
-            if (x >= j.d) continue;
-            float4 s = make_float4(0, 0, 0, 0);
-#pragma unroll 8
-            for (int i = warp; i < n; i += AJ_THREADS / 32) {
-                const float f = ml[i].x;
-                const float4 y = *reinterpret_cast<const float4 *>(a.part_o + (int64_t)(pr.slot(i) * ATT_R + r) * j.d + x);
-                s.x += f * y.x, s.y += f * y.y, s.z += f * y.z, s.w += f * y.w;
+            for (int h = 0; h < 2; h++) {
+                const int x = 128 * h + 4 * lane;
+                if (x >= j.d) break;
+                out[x] = from_f32<IO>(s.o[h].x * inv), out[x + 1] = from_f32<IO>(s.o[h].y * inv);
+                out[x + 2] = from_f32<IO>(s.o[h].z * inv), out[x + 3] = from_f32<IO>(s.o[h].w * inv);
             }
-            *reinterpret_cast<float4 *>(&acc[warp][x]) = s;
+            return;
         }
-        __syncthreads();
-        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-        for (int x = tid; x < j.d; x += AJ_THREADS) {
-            float s = 0.0f;
+        if (lane == 0) ml[warp] = make_float2(s.m, s.l);
 #pragma unroll
-            for (int w = 0; w < AJ_THREADS / 32; w++) s += acc[w][x];
-            static_cast<IO *>(a.out)[b * a.out_stride + (int64_t)h * j.d + x] = from_f32<IO>(s * inv);
+        for (int h = 0; h < 2; h++)
+            if (128 * h + 4 * lane < j.d) *reinterpret_cast<float4 *>(&acc[warp][128 * h + 4 * lane]) = s.o[h];
+        __syncthreads();
+        float m = -INFINITY, l = 0.0f, v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < W; w++) m = fmaxf(m, ml[w].x);
+        const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+        for (int w = 0; w < W; w++) {
+            const float f = exp2_fast(ml[w].x - ref);
+            l += f * ml[w].y;
+            if (tid < j.d) v += f * acc[w][tid];
         }
+        if (tid < j.d) out[tid] = from_f32<IO>(l > 0.0f || l != l ? v / l : 0.0f);
         return;
     }
     // weights of entries [i0, i0 + AJ_CHUNK) of one (sequence, kv head), four
-    // consecutive ones per thread
+    // consecutive ones per thread and turn
     const int w = blockIdx.x - j.n_out, u = w / j.chunks, b = u / a.KVH, kvh = u - b * a.KVH, i0 = (w - u * j.chunks) * AJ_CHUNK;
-    const int len = attn_len(a, b), i = i0 + 4 * tid;
+    const int len = attn_len(a, b);
     if (i0 >= len) return;
     const int nt = a.prefix[b + 1] - a.prefix[b];
-    float4 add = make_float4(0, 0, 0, 0);
+    float4 add[AJ_TURNS];
+#pragma unroll
+    for (int k = 0; k < AJ_TURNS; k++) add[k] = make_float4(0, 0, 0, 0);
     for (int g0 = 0; g0 < a.G; g0 += 128) {  // ml holds 128 heads at a time
         const int ng = min(a.G - g0, 128);
-        for (int g = warp; g < ng; g += AJ_THREADS / 32) {
+        for (int g = warp; g < ng; g += W) {
             const PartRange pr = part_range(j, b, kvh * a.NB + (g0 + g) / ATT_R, nt);
-            const float2 e = pr.c0 == pr.c1 ? a.ml[(int64_t)b * a.H + kvh * a.G + g0 + g] : warp_ml(j, pr, (g0 + g) % ATT_R, lane);
+            const float2 e = pr.n == 1 ? a.ml[(int64_t)b * a.H + kvh * a.G + g0 + g] : warp_ml(j, pr, (g0 + g) % ATT_R, lane);
             if (lane == 0) ml[g] = make_float2(e.x == -INFINITY ? 0.0f : e.x, e.y > 0.0f || e.y != e.y ? 1.0f / e.y : 0.0f);
         }
         __syncthreads();
         // scores are there up to the end of the last tile of 16
-        if (i < len) {
-            const float *z = a.z + ((int64_t)b * a.H + kvh * a.G + g0) * a.z_stride + i;
-#pragma unroll 4
-            for (int g = 0; g < ng; g++) {
-                const float2 e = ml[g];
-                const float4 x = *reinterpret_cast<const float4 *>(z + g * a.z_stride);
-                add.x += exp2_fast(x.x - e.x) * e.y, add.y += exp2_fast(x.y - e.x) * e.y;
-                add.z += exp2_fast(x.z - e.x) * e.y, add.w += exp2_fast(x.w - e.x) * e.y;
+        const float *z = a.z + ((int64_t)b * a.H + kvh * a.G + g0) * a.z_stride + i0 + 4 * tid;
+        for (int g = 0; g < ng; g++, z += a.z_stride) {
+            const float2 e = ml[g];
+            float4 x[AJ_TURNS];
+#pragma unroll
+            for (int k = 0; k < AJ_TURNS; k++)
+                if (i0 + 4 * tid + k * 4 * AJ_THREADS < len) x[k] = *reinterpret_cast<const float4 *>(z + k * 4 * AJ_THREADS);
+#pragma unroll
+            for (int k = 0; k < AJ_TURNS; k++) {
+                if (i0 + 4 * tid + k * 4 * AJ_THREADS >= len) break;
+                add[k].x += exp2_fast(x[k].x - e.x) * e.y, add[k].y += exp2_fast(x[k].y - e.x) * e.y;
+                add[k].z += exp2_fast(x[k].z - e.x) * e.y, add[k].w += exp2_fast(x[k].w - e.x) * e.y;
             }
         }
         __syncthreads();
     }
-    const float v[4] = {add.x, add.y, add.z, add.w};
 #pragma unroll
-    for (int k = 0; k < 4; k++) {
-        if (i + k >= len) break;
-        const int col = a.page.div(i + k), page = a.table[(int64_t)b * a.max_pages + col];
-        if (page < 0 || page >= a.n_pages) continue;
-        a.weight[((int64_t)page * a.KVH + kvh) * a.page_size + (i + k - col * a.page_size)] += v[k];
+    for (int k = 0; k < AJ_TURNS; k++) {
+        const int i = i0 + 4 * tid + k * 4 * AJ_THREADS;
+        if (i >= len) break;
+        if (a.quads && i + 3 < len) {  // four entries in one page, 16-byte aligned
+            const int col = a.page.div(i), page = a.table[(int64_t)b * a.max_pages + col];
+            if (page < 0 || page >= a.n_pages) continue;
+            float4 *const at = reinterpret_cast<float4 *>(a.weight + ((int64_t)page * a.KVH + kvh) * a.page_size + (i - col * a.page_size));
+            float4 x = *at;
+            x.x += add[k].x, x.y += add[k].y, x.z += add[k].z, x.w += add[k].w;
+            *at = x;
+        } else {
+            const float v[4] = {add[k].x, add[k].y, add[k].z, add[k].w};
+#pragma unroll
+            for (int x = 0; x < 4; x++) {
+                if (i + x >= len) break;
+                const int col = a.page.div(i + x), page = a.table[(int64_t)b * a.max_pages + col];
+                if (page < 0 || page >= a.n_pages) continue;
+                a.weight[((int64_t)page * a.KVH + kvh) * a.page_size + (i + x - col * a.page_size)] += v[x];
+            }
+        }
     }
 }
 
@@ -180,7 +238,7 @@ static int attn_plan(const ofb_kv_cache *c, int n_heads, int n_seqs, int max_len
     p.max_len = max_len && max_len < reach ? max_len : reach;
     const int64_t tiles = ((int64_t)p.max_len + ATT_TILE - 1) / ATT_TILE;
     p.NB = (n_heads / c->n_kv_heads + ATT_R - 1) / ATT_R;
-    if (tiles * n_seqs > INT32_MAX / ((int64_t)c->n_kv_heads * p.NB)) {
+    if (tiles * n_seqs > (1 << 30) / ((int64_t)c->n_kv_heads * p.NB)) {  // (sums of tile numbers stay within 31 bits)
         set_error("ofb_attn_decode: %d sequences of %d entries are too many tiles", n_seqs, p.max_len);
         return OFB_ETOOLARGE;
     }
@@ -192,26 +250,27 @@ static int attn_plan(const ofb_kv_cache *c, int n_heads, int n_seqs, int max_len
     case 192: p.v = attn_variant_192(bf, f32); break;
     default: p.v = attn_variant_256(bf, f32); break;
     }
-    const int64_t runs = (tiles * n_seqs * c->n_kv_heads * p.NB + ATT_W - 1) / ATT_W;
-    const int most = sm_count() * p.v.ctas < AJ_MAX_CTAS ? sm_count() * p.v.ctas : AJ_MAX_CTAS;
+    const int64_t runs = (tiles * n_seqs * c->n_kv_heads * p.NB + p.v.warps - 1) / p.v.warps;
+    const int most = sm_count() * p.v.ctas;
     // Short sequences: as many CTAs as give each warp ATT_SHORT tiles at most,
     // where all of them have room at once. Weights need all of a kv head's
     // query heads in one pass.
     p.cluster = 0;
     if (!accumulate || p.NB == 1) {
         int n = 1;
-        while (n < 8 && tiles > n * ATT_W) n *= 2;
-        if (tiles <= (int64_t)n * ATT_W * ATT_SHORT && (int64_t)n_seqs * c->n_kv_heads * p.NB * n <= most) p.cluster = n;
+        while (n < 8 && tiles > n * p.v.warps) n *= 2;
+        if (tiles <= (int64_t)n * p.v.warps * ATT_SHORT && (int64_t)n_seqs * c->n_kv_heads * p.NB * n <= most) p.cluster = n;
     }
     p.ctas = runs < 1 ? 1 : runs < most ? (int)runs : most;
+    const size_t parts = 2 * (size_t)most;
     p.z_stride = tiles * ATT_TILE;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t o = at; at += (bytes + 255) / 256 * 256; return o; };
     p.prefix = take((size_t)(n_seqs + 1) * 4);
     p.ml = take((size_t)n_seqs * n_heads * 8);
     // sized for a full grid, so that the size grows with n_seqs and max_len
-    p.part_ml = take((size_t)2 * most * ATT_R * 8);
-    p.part_o = take((size_t)2 * most * ATT_R * c->head_dim * 4);
+    p.part_ml = take(parts * ATT_R * 8);
+    p.part_o = take(parts * ATT_R * c->head_dim * 4);
     p.z = accumulate ? take((size_t)n_seqs * n_heads * p.z_stride * 4) : 0;
     p.total = at;
     return OFB_OK;
@@ -255,17 +314,20 @@ extern "C" int ofb_attn_decode(const ofb_kv_cache *cache, const void *q, int typ
     a.page_stride = cache_page_stride(cache), a.q_stride = q_stride, a.out_stride = out_stride;
     a.B = n_seqs, a.KVH = cache->n_kv_heads, a.G = n_heads / a.KVH, a.NB = p.NB, a.H = n_heads;
     a.page_size = cache->page_size, a.max_pages = cache->max_pages, a.n_pages = cache->n_pages, a.max_len = p.max_len;
-    a.page = fast_div(a.page_size), a.tiled = a.page_size % ATT_TILE == 0;
+    a.page = fast_div(a.page_size), a.halves = a.page_size % 16 == 0;
     a.scale = scale * 1.4426950408889634f;
     a.errors = cache->errors;
     a.prefix = reinterpret_cast<int *>(w + p.prefix), a.ml = reinterpret_cast<float2 *>(w + p.ml);
     a.part_o = reinterpret_cast<float *>(w + p.part_o), a.part_ml = reinterpret_cast<float2 *>(w + p.part_ml);
     a.z = accumulate ? reinterpret_cast<float *>(w + p.z) : nullptr;
     a.z_stride = p.z_stride, a.weight = cache->weight;
-    j.ctas = p.ctas, j.d = cache->head_dim;
-    j.n_out = n_seqs * n_heads;
+    a.quads = a.page_size % 4 == 0 && !misaligned(a.weight, 16);
+    j.ctas = p.ctas, j.warps = p.v.warps, j.d = cache->head_dim;
+    // parts of a head, about, when all sequences are of the largest length
+    j.wide = p.ctas >= 4 * n_seqs * a.KVH * a.NB;
+    j.n_out = j.wide ? n_seqs * n_heads : n_seqs * a.KVH * a.NB;
     j.chunks = (p.max_len + AJ_CHUNK - 1) / AJ_CHUNK;
-    const int64_t blocks = (int64_t)n_seqs * n_heads + (accumulate ? (int64_t)n_seqs * a.KVH * j.chunks : 0);
+    const int64_t blocks = j.n_out + (accumulate ? (int64_t)n_seqs * a.KVH * j.chunks : 0);
     if (blocks > INT32_MAX) { set_error("ofb_attn_decode: too many weight blocks"); return OFB_ETOOLARGE; }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     // a raised shared-memory limit per kernel and device
@@ -275,14 +337,14 @@ extern "C" int ofb_attn_decode(const ofb_kv_cache *cache, const void *q, int typ
     if (p.cluster) {
         cudaError_t e = ensure_dyn_smem(p.v.cluster, p.v.head, attr[vi + 1]);
         if (e != cudaSuccess) return cuda_status(e, "ofb_attn_decode smem attribute");
-        e = launch_pdl_cluster(p.v.cluster, dim3((unsigned)(n_seqs * a.KVH * a.NB * p.cluster)), dim3(ATT_W * 32), p.cluster,
+        e = launch_pdl_cluster(p.v.cluster, dim3((unsigned)(n_seqs * a.KVH * a.NB * p.cluster)), dim3(p.v.warps * 32), p.cluster,
                                p.v.head, s, a);
         return e == cudaSuccess ? OFB_OK : cuda_status(e, "ofb_attn_decode launch");
     }
     const size_t smem = p.v.head + (size_t)n_seqs * 4 + (n_seqs + 3) / 4 * 4;
     cudaError_t e = ensure_dyn_smem(p.v.run, smem, attr[vi]);
     if (e != cudaSuccess) return cuda_status(e, "ofb_attn_decode smem attribute");
-    e = launch_pdl(p.v.run, dim3(p.ctas), dim3(ATT_W * 32), smem, s, a);
+    e = launch_pdl(p.v.run, dim3(p.ctas), dim3(p.v.warps * 32), smem, s, a);
     if (e != cudaSuccess) return cuda_status(e, "ofb_attn_decode launch");
     if (p.ctas == 1 && !accumulate) return OFB_OK;  // every part is whole
     const dim3 grid((unsigned)blocks), block(AJ_THREADS);

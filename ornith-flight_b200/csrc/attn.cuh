@@ -6,17 +6,21 @@
 // HBM-bound: 4 * head_dim bytes per cached entry and kv head against
 // 4 * head_dim operations per query head.
 //
-// Work: the entries of each (sequence, kv head) are cut into tiles of 16, and
-// the tiles of all of them, laid end to end, are dealt to the CTAs in equal
-// runs, whatever the lengths. A run holds parts of one or more (sequence, kv
-// head)s; a part that is not whole goes to the scratch (sums, maximum, sum of
-// exponentials) and attn.cu joins it with the others.
+// Work: the entries of each (sequence, kv head) are cut into tiles of 32, and
+// the tiles of all of them, laid end to end, are dealt to the CTAs in equal runs,
+// whatever the lengths. A run holds parts of one or more (sequence, kv head)s; a
+// part that is not whole goes to the scratch (sums, maximum, sum of exponentials)
+// and attn.cu joins it with the others. (Runs of three quarters and the rest
+// taken in smaller ones by CTAs that finish early gained 4% on 48 ragged
+// sequences with head_dim 128 and lost 3% on 24 with 256: not kept.)
 //
-// Inside a CTA each warp takes every fourth tile of a part by itself: its own
+// Inside a CTA the warps take the tiles of a part in turn, each by itself: its own
 // ring of tiles in shared memory filled by 16-byte asynchronous copies (page
-// by page, ATT_S - 1 tiles ahead and across parts, the page numbers one tile
+// by page, a tile or two ahead and across parts, the page numbers one tile
 // before that), its own running maximum and sums, no barrier but one merge at
-// the end of a part. Rows are padded by 16 bytes, so that ldmatrix meets no
+// the end of a part. The 6 to 8 warps that an SM's shared memory has room for
+// leave latencies open, so a tile is 32 entries: its four chains of products, and
+// one softmax step for all, keep a warp busier than two tiles of 16 would. Rows are padded by 16 bytes, so that ldmatrix meets no
 // bank twice.
 //
 // Short sequences take a cluster of CTAs each instead of runs (CLUSTER): its
@@ -49,12 +53,7 @@ namespace cg = cooperative_groups;
 
 namespace ofb {
 
-#ifndef V_S
-#define V_S 3
-#define V_C 2
-#endif
-constexpr int ATT_W = 4;      // warps per CTA
-constexpr int ATT_TILE = 16;  // entries per tile
+constexpr int ATT_TILE = 32;  // entries per tile, one per lane
 constexpr int ATT_R = 8;      // query heads per pass
 constexpr int ATT_MAX_SEQS = 2048;
 
@@ -66,7 +65,8 @@ struct AttnArgs {
     int B, KVH, G, NB, H;  // NB: passes of at most ATT_R heads per kv head
     FastDiv page;  // by page_size
     int page_size, max_pages, n_pages, max_len;
-    int tiled;        // page_size is a multiple of ATT_TILE: a tile lies in one page
+    int halves;       // page_size is a multiple of 16: each half of a tile lies in one page
+    int quads;        // page_size is a multiple of 4 and weight 16-byte aligned
     float scale;      // times log2(e)
     uint32_t *errors;
     // scratch
@@ -79,6 +79,7 @@ struct AttnArgs {
     float *weight;
 };
 
+__device__ __forceinline__ void prefetch_l2_line(const void *p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
 __device__ __forceinline__ float exp2_fast(float x) {  // 2 steps at most; below 2^-126 it gives 0
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -86,26 +87,31 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2 steps at most; below
 }
 // How many entries of sequence b are attended to.
 __device__ __forceinline__ int attn_len(const AttnArgs &a, int b) { return min(max(a.lens[b], 0), a.max_len); }
-// Tiles per CTA when `total` tiles are dealt to `ctas` CTAs: at least one per
+// How the row of all tiles is cut into runs, one per CTA: at least a tile per
 // warp, so that few tiles do not leave many parts to join.
-__host__ __device__ __forceinline__ int attn_run(int total, int ctas) {
-    const int n = total / ctas + (total % ctas != 0);
-    return n < ATT_W ? ATT_W : n;
-}
+struct AttnSplit {
+    int total, run;
+    static __device__ __forceinline__ AttnSplit make(int total, int ctas, int warps) {
+        return {total, max(total / ctas + (total % ctas != 0), warps)};
+    }
+    __device__ __forceinline__ int first(int id) const { return (int)min((int64_t)id * run, (int64_t)total); }
+};
 
 template <int D> struct AttnShape {
     static constexpr int PITCH = D * 2 + 16;                 // bytes of a row in shared memory
     static constexpr int TILE_BYTES = 2 * ATT_TILE * PITCH;  // K, then V
-    static constexpr int S = D <= 64 ? 5 : D <= 96 ? 4 : D <= 128 ? V_S : D <= 192 ? 4 : 3;  // ring slots
-    static constexpr int CTAS = D <= 96 ? 2 : D <= 128 ? V_C : 1;            // per SM
-    static constexpr int RING = ATT_W * S * TILE_BYTES;
-    // behind the ring: the warps' and the CTA's (maximum, sum), then per sequence
+    static constexpr int W = D == 128 || D == 256 ? 3 : 4;   // warps per CTA
+    static constexpr int S = D <= 64 ? 3 : 2;                // ring slots
+    static constexpr int CTAS = D <= 128 ? 2 : 1;            // per SM
+    static constexpr int THREADS = W * 32;
+    static constexpr int RING = W * S * TILE_BYTES;
+    // behind the ring: the warps' and the cluster's (maximum, sum), then per sequence
     // the tiles before it and the entries of its last tile
-    static constexpr int HEAD = RING + (ATT_W + 2) * ATT_R * 8;
+    static constexpr int HEAD = RING + (W + 1) * ATT_R * 8;
     static constexpr int smem(int B) { return HEAD + (B + 1) * 4 + (B + 3) / 4 * 4; }
     static_assert(TILE_BYTES >= ATT_R * (D + 4) * 4, "a warp's sums must fit one ring slot");
-    static_assert(CTAS * (smem(512) + 1536) <= 228 * 1024, "shared memory of an SM");
-    static_assert(smem(ATT_MAX_SEQS) + 1536 <= 227 * 1024, "shared memory of a CTA");
+    static_assert(CTAS * (smem(384) + 2048) <= 228 * 1024, "shared memory of an SM");
+    static_assert(smem(ATT_MAX_SEQS) + 1024 <= 227 * 1024, "shared memory of a CTA");
 };
 
 template <typename T> struct Mma;
@@ -199,7 +205,7 @@ __device__ __forceinline__ AttnPart attn_part(const int *prefix, const uint8_t *
 }
 
 template <int D, typename CT, typename IO, bool CLUSTER>
-__global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_kernel(const __grid_constant__ AttnArgs a) {
+__global__ void __launch_bounds__(AttnShape<D>::THREADS, AttnShape<D>::CTAS) attn_split_kernel(const __grid_constant__ AttnArgs a) {
     using SH = AttnShape<D>;
     constexpr bool F32 = sizeof(IO) == 4, BF = std::is_same<CT, __nv_bfloat16>::value;
     constexpr int NQ = F32 ? (BF ? 3 : 2) : 1;       // parts of a query
@@ -208,17 +214,19 @@ __global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_ker
     constexpr bool DIRECT = !F32 && D <= 128;        // the tensor core accumulates (registers allow no more)
     constexpr int NO = DIRECT ? 4 : 2;               // accumulators of 8 columns
     constexpr int KS = D / 16, CH = D / 8;           // k steps; 16-byte chunks of a row
+    constexpr int W = SH::W, THREADS = SH::THREADS;
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c2 = (lane & 3) * 2;
     uint8_t *ring = smem + warp * SH::S * SH::TILE_BYTES;
     float2 *mml = reinterpret_cast<float2 *>(smem + SH::RING);  // [W][R]
-    float2 *cml = mml + ATT_W * ATT_R;                          // [2][R]: this CTA's, the cluster's
+    float2 *cml = mml + W * ATT_R;                          // [R]: the cluster's
     int *prefix = reinterpret_cast<int *>(smem + SH::HEAD);     // [B + 1]
     uint8_t *last = reinterpret_cast<uint8_t *>(prefix + a.B + 1);
-    __shared__ uint32_t valid[ATT_W][8];  // per ring slot: which of the 16 entries are there
-    __shared__ int wsum[ATT_W];
-    __shared__ float *mo[ATT_W];  // each warp's sums at the end of a part, [R][D + 4]
-    __shared__ int mo_at;         // CLUSTER: mo[0] as an offset, for the other CTAs
+    __shared__ uint32_t valid[W][4];  // per ring slot: which of the 32 entries are there
+    __shared__ int wsum[W];
+    __shared__ float *mo[W];  // each warp's sums at the end of a part, [R][D + 4]
+    __shared__ float2 all_ml[8][ATT_R];  // CLUSTER: every CTA's (maximum, sum) ...
+    __shared__ int all_at[8];            // ... and where its sums are in its shared memory
     cg::cluster_group cl = cg::this_cluster();
 
     pdl_wait();
@@ -228,6 +236,7 @@ __global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_ker
     int f0 = 0, f1 = 1;
     AttnPart first;
     if constexpr (CLUSTER) {
+        cl.barrier_arrive();  // waited for before the others' shared memory is written
         const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank(), u = blockIdx.x / C;
         first.b = u / nvh;
         first.vh = u - first.b * nvh;
@@ -237,8 +246,16 @@ __global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_ker
         first.t = (int)((int64_t)rank * first.nt / C);
         first.end = (int)((int64_t)(rank + 1) * first.nt / C);
     } else {
+        // the queries and the page table into L2 while the lengths are on their way
+        {
+            const int64_t i = ((int64_t)blockIdx.x * (THREADS) + tid) * 128;
+            if (i < (int64_t)a.H * D * (int)sizeof(IO))
+                for (int b = 0; b < min(a.B, 8); b++)
+                    prefetch_l2_line(static_cast<const char *>(a.q) + b * a.q_stride * (int)sizeof(IO) + i);
+            if (i < (int64_t)a.B * a.max_pages * 4) prefetch_l2_line(reinterpret_cast<const char *>(a.table) + i);
+        }
         // tiles before each sequence; every CTA forms them for itself
-        for (int base = 0; base < a.B; base += ATT_W * 32) {
+        for (int base = 0; base < a.B; base += THREADS) {
             const int b = base + tid;
             int n = 0;
             if (b < a.B) {
@@ -262,21 +279,20 @@ __global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_ker
             __syncthreads();
         }
         if (blockIdx.x == 0)
-            for (int b = tid; b <= a.B; b += ATT_W * 32) a.prefix[b] = prefix[b];
+            for (int b = tid; b <= a.B; b += THREADS) a.prefix[b] = prefix[b];
         // sequences without entries: zeros
         for (int b = blockIdx.x; b < a.B; b += gridDim.x)
             if (prefix[b + 1] == prefix[b])
-                for (int i = tid; i < a.H * D; i += ATT_W * 32) static_cast<IO *>(a.out)[b * a.out_stride + i] = from_f32<IO>(0.0f);
-        const int total = prefix[a.B] * nvh, run = attn_run(total, gridDim.x);
-        // (the last run's end may lie past 31 bits)
-        f0 = (int)min((int64_t)blockIdx.x * run, (int64_t)total), f1 = f0 + min(run, total - f0);
+                for (int i = tid; i < a.H * D; i += THREADS) static_cast<IO *>(a.out)[b * a.out_stride + i] = from_f32<IO>(0.0f);
+        const AttnSplit sp = AttnSplit::make(prefix[a.B] * nvh, (int)gridDim.x, W);
+        f0 = sp.first(blockIdx.x), f1 = sp.first(blockIdx.x + 1);
         if (f0 >= f1) return;
         first = attn_part(prefix, last, a.B, nvh, f0, f1);
     }
 
     const uint32_t ring_s = ax::smem_u32(ring);
-    // The tile that the ring is filled with next: its part, number, and its
-    // rows' entries (lanes 0..15) with the page numbers already asked for.
+    // The tile that the ring is filled with next: its part, number, and each
+    // lane's entry with the page number already asked for.
     AttnPart lp = first;
     int lf = f0;
     int lt = lp.t + warp, l_entry = 0, l_page = -1;
@@ -288,7 +304,7 @@ __global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_ker
             else lp = attn_part(prefix, last, a.B, nvh, lf, f1), lt = lp.t + warp;
         }
         if (more) {
-            l_entry = lt * ATT_TILE + (a.tiled ? 0 : lane & 15);
+            l_entry = lt * ATT_TILE + lane;
             if (l_entry < lp.len) l_page = a.table[(int64_t)lp.b * a.max_pages + a.page.div(l_entry)];
         }
     };
@@ -300,65 +316,73 @@ __global__ void __launch_bounds__(ATT_W * 32, AttnShape<D>::CTAS) attn_split_ker
             const bool there = l_entry < lp.len, ok = there && l_page >= 0 && l_page < a.n_pages;
             if (there && !ok) report(a.errors, OFB_CACHE_EPAGE);
             const int64_t off = ok ? l_page * a.page_stride + ((int64_t)kvh * a.page_size + in) * D : -1;
-            if (a.tiled) {  // 16 rows on end
-                const int rows = off < 0 ? 0 : min(ATT_TILE, lp.len - l_entry);
-                const CT *ks = k + (off < 0 ? 0 : off) + lane * 8, *vs = v + (off < 0 ? 0 : off) + lane * 8;
-                if (lane == 0) valid[warp][slot] = (1u << rows) - 1u;
-if (rows == ATT_TILE) {
+            const uint32_t mask = __ballot_sync(0xffffffffu, ok);
+            if (lane == 0) valid[warp][slot] = mask;
+            if (a.halves && mask == 0xffffffffu) {  // two times 16 rows on end
 #pragma unroll
-                    for (int j = 0; j < ATT_TILE * CH / 32; j++) {
-                        const int c = j * 32 + lane, r = c / CH, x = c - r * CH;
-                        cp16(dst + r * SH::PITCH + x * 16, ks + j * 256, 16);
-                        cp16(dst + (ATT_TILE + r) * SH::PITCH + x * 16, vs + j * 256, 16);
-                    }
-                } else {
+                for (int h = 0; h < 2; h++) {
+                    const int64_t o = __shfl_sync(0xffffffffu, off, 16 * h) + lane * 8;
+                    const CT *ks = k + o, *vs = v + o;
 #pragma unroll
-                    for (int j = 0; j < ATT_TILE * CH / 32; j++) {
+                    for (int j = 0; j < 16 * CH / 32; j++) {
                         const int c = j * 32 + lane, r = c / CH, x = c - r * CH;
-                        const bool in_row = r < rows;
-                        // a row that is not there is not read: its address need not exist
-                        cp16(dst + r * SH::PITCH + x * 16, in_row ? ks + j * 256 : k, in_row ? 16 : 0);
-                        cp16(dst + (ATT_TILE + r) * SH::PITCH + x * 16, in_row ? vs + j * 256 : v, in_row ? 16 : 0);
+                        cp16(dst + (16 * h + r) * SH::PITCH + x * 16, ks + j * 256, 16);
+                        cp16(dst + (ATT_TILE + 16 * h + r) * SH::PITCH + x * 16, vs + j * 256, 16);
                     }
                 }
             } else {
-                const uint32_t mask = __ballot_sync(0xffffffffu, off >= 0);
-                if (lane == 0) valid[warp][slot] = mask & 0xffffu;
-#pragma unroll
+#pragma unroll 4
                 for (int j = 0; j < ATT_TILE * CH / 32; j++) {
                     const int c = j * 32 + lane, r = c / CH, x = c - r * CH;
                     const int64_t o = __shfl_sync(0xffffffffu, off, r);
+                    // a row that is not there is not read: its address need not exist
                     const int64_t e = o < 0 ? 0 : o + x * 8;
                     const int n = o < 0 ? 0 : 16;
                     cp16(dst + r * SH::PITCH + x * 16, k + e, n);
                     cp16(dst + (ATT_TILE + r) * SH::PITCH + x * 16, v + e, n);
                 }
             }
-            lt += ATT_W;
+            lt += W;
             look_up();
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
     look_up();
+    // Queries: row g of A, parts as told at the top. The first part's are asked
+    // for before the rings fill, whose copies would keep them waiting.
+    IO qx[KS][2][2];
+    auto ask_queries = [&](const AttnPart &p) {
+        const int kvh = p.vh / a.NB, h0 = (p.vh - kvh * a.NB) * ATT_R;
+        const IO *qr = static_cast<const IO *>(a.q) + p.b * a.q_stride + (int64_t)(kvh * a.G + h0 + g) * D + c2;
+        const bool there = g < min(ATT_R, a.G - h0);
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                qx[ks][u][0] = there ? qr[ks * 16 + u * 8] : from_f32<IO>(0.0f);
+                qx[ks][u][1] = there ? qr[ks * 16 + u * 8 + 1] : from_f32<IO>(0.0f);
+            }
+    };
+    ask_queries(first);
 #pragma unroll
     for (int i = 0; i < SH::S - 1; i++) fill(i);
     int slot = 0;  // of the next tile to compute
 
     int npart = 0;
-    for (int f = f0; f < f1; npart++) {
-        const AttnPart p = npart ? attn_part(prefix, last, a.B, nvh, f, f1) : first;
+    AttnPart p = first;
+    for (;;) {
         const int kvh = p.vh / a.NB, h0 = (p.vh - kvh * a.NB) * ATT_R, rows = min(ATT_R, a.G - h0);
-        // queries: row g of A, parts as told at the top
         uint32_t qa[KS][2][NQ];
         float qscale = a.scale;
         {
-            const IO *qr = static_cast<const IO *>(a.q) + p.b * a.q_stride + (int64_t)(kvh * a.G + h0 + g) * D;
             float up = 1.0f;
             if constexpr (F32 && !BF) {
                 // a power of two that brings the row's largest element to [2^13, 2^14)
                 float m = 0.0f;
-                if (g < rows)
-                    for (int i = c2; i < D; i += 8) m = fmaxf(m, fmaxf(fabsf(qr[i]), fabsf(qr[i + 1])));
+#pragma unroll
+                for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) m = fmaxf(m, fmaxf(fabsf(qx[ks][u][0]), fabsf(qx[ks][u][1])));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
                 const int e = (int)(__float_as_uint(m) >> 23);  // 0: zero or subnormal, 255: not finite
@@ -371,14 +395,7 @@ if (rows == ATT_TILE) {
 #pragma unroll
             for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    float x = 0.0f, y = 0.0f;
-                    if (g < rows) {
-                        x = to_f32(qr[ks * 16 + u * 8 + c2]) * up;
-                        y = to_f32(qr[ks * 16 + u * 8 + c2 + 1]) * up;
-                    }
-                    split2<CT, NQ>(x, y, qa[ks][u]);
-                }
+                for (int u = 0; u < 2; u++) split2<CT, NQ>(to_f32(qx[ks][u][0]) * up, to_f32(qx[ks][u][1]) * up, qa[ks][u]);
         }
         float o[D / 8][NO], m = -INFINITY, l = 0.0f;
 #pragma unroll
@@ -386,7 +403,7 @@ if (rows == ATT_TILE) {
 #pragma unroll
             for (int u = 0; u < NO; u++) o[i][u] = 0.0f;
 
-        for (int t = p.t + warp; t < p.end; t += ATT_W) {
+        for (int t = p.t + warp; t < p.end; t += W) {
             asm volatile("cp.async.wait_group %0;" ::"n"(SH::S - 2) : "memory");
             __syncwarp();
             fill(slot == 0 ? SH::S - 1 : slot - 1);
@@ -394,50 +411,53 @@ if (rows == ATT_TILE) {
             const uint32_t ok = valid[warp][slot] >> c2;
             slot = slot == SH::S - 1 ? 0 : slot + 1;
 
-            float s[2][4] = {}, s2[2][4] = {};
+            // scores of 8 entries each; with three parts the lowest apart
+            float s[4][4] = {}, sl[NQ > 2 ? 4 : 1][4] = {};
             const uint32_t ka = ks_s + ((lane & 7) + ((lane >> 4) << 3)) * SH::PITCH + ((lane >> 3) & 1) * 16;
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
-                uint32_t b[4];
-                ldmatrix4(b, ka + ks * 32);
                 const uint32_t a0[4] = {qa[ks][0][0], NQ > 1 ? qa[ks][0][NQ > 1 ? 1 : 0] : 0u, qa[ks][1][0],
                                         NQ > 1 ? qa[ks][1][NQ > 1 ? 1 : 0] : 0u};
-                float(&c0)[4] = ks & 1 ? s2[0] : s[0];
-                float(&c1)[4] = ks & 1 ? s2[1] : s[1];
-                Mma<CT>::run(c0, a0, b[0], b[1]);
-                Mma<CT>::run(c1, a0, b[2], b[3]);
-                if constexpr (NQ > 2) {
-                    const uint32_t a1[4] = {qa[ks][0][2], 0u, qa[ks][1][2], 0u};
-                    Mma<CT>::run(c0, a1, b[0], b[1]);
-                    Mma<CT>::run(c1, a1, b[2], b[3]);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t b[4];
+                    ldmatrix4(b, ka + h * 16 * SH::PITCH + ks * 32);
+                    Mma<CT>::run(s[2 * h], a0, b[0], b[1]);
+                    Mma<CT>::run(s[2 * h + 1], a0, b[2], b[3]);
+                    if constexpr (NQ > 2) {
+                        const uint32_t a1[4] = {qa[ks][0][2], 0u, qa[ks][1][2], 0u};
+                        Mma<CT>::run(sl[2 * h], a1, b[0], b[1]);
+                        Mma<CT>::run(sl[2 * h + 1], a1, b[2], b[3]);
+                    }
                 }
             }
-            // scores of row g, entries 8j + c2 + {0, 1}, in log2
-            float z[2][2];
+            // row g, entries 8j + c2 + {0, 1}, in log2
+            float z[4][2], mt = -INFINITY;
 #pragma unroll
-            for (int j = 0; j < 2; j++)
+            for (int j = 0; j < 4; j++)
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    float x = s[j][u] + s2[j][u];
-                    if (NQ > 1) x += s[j][2 + u] + s2[j][2 + u];
+                    float x = s[j][u];
+                    if (NQ > 1) x += s[j][2 + u];
+                    if constexpr (NQ > 2) x += sl[j][u];
                     z[j][u] = (ok >> (8 * j + u)) & 1 ? x * qscale : -INFINITY;
+                    mt = fmaxf(mt, z[j][u]);
                 }
             if (a.z && g < rows) {
                 float *zr = a.z + ((int64_t)p.b * a.H + kvh * a.G + h0 + g) * a.z_stride + t * ATT_TILE + c2;
-                *reinterpret_cast<float2 *>(zr) = make_float2(z[0][0], z[0][1]);
-                *reinterpret_cast<float2 *>(zr + 8) = make_float2(z[1][0], z[1][1]);
+#pragma unroll
+                for (int j = 0; j < 4; j++) *reinterpret_cast<float2 *>(zr + 8 * j) = make_float2(z[j][0], z[j][1]);
             }
-            float mt = fmaxf(fmaxf(z[0][0], z[0][1]), fmaxf(z[1][0], z[1][1]));
             mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
             mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
             const float mn = fmaxf(m, mt), ref = mn == -INFINITY ? 0.0f : mn;
             const float alpha = exp2_fast(m - ref);  // 0 at the first tile
             const bool grown = __any_sync(0xffffffffu, mn != m);
             m = mn;
-            uint32_t pa[2][NP];  // [entries 0-7 / 8-15][part]
+            uint32_t pa[4][NP];  // [8 entries][part]
             float sum = 0.0f;
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
+            for (int j = 0; j < 4; j++) {
                 const float x = exp2_fast(z[j][0] - ref), y = exp2_fast(z[j][1] - ref);
                 sum += x + y;
                 split2<CT, NP>(x * PSCALE, y * PSCALE, pa[j]);
@@ -450,23 +470,28 @@ if (rows == ATT_TILE) {
                     for (int u = 0; u < NO; u++) o[i][u] *= alpha;
             }
             const uint32_t va = vs_s + ((lane & 7) + ((lane >> 3) & 1) * 8) * SH::PITCH + (lane >> 4) * 16;
-            const uint32_t a0[4] = {pa[0][0], pa[0][1], pa[1][0], pa[1][1]};
 #pragma unroll
             for (int n = 0; n < D / 16; n++) {
-                uint32_t b[4];
-                ldmatrix4_t(b, va + n * 32);
-                if constexpr (DIRECT) {
-                    Mma<CT>::run(o[2 * n], a0, b[0], b[1]);
-                    Mma<CT>::run(o[2 * n + 1], a0, b[2], b[3]);
-                } else {
-                    float x[4] = {}, y[4] = {};
-                    Mma<CT>::run(x, a0, b[0], b[1]);
-                    Mma<CT>::run(y, a0, b[2], b[3]);
-                    if constexpr (NP > 2) {
-                        const uint32_t a1[4] = {pa[0][2], 0u, pa[1][2], 0u};
-                        Mma<CT>::run(x, a1, b[0], b[1]);
-                        Mma<CT>::run(y, a1, b[2], b[3]);
+                float x[4] = {}, y[4] = {};
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t b[4];
+                    ldmatrix4_t(b, va + h * 16 * SH::PITCH + n * 32);
+                    const uint32_t a0[4] = {pa[2 * h][0], pa[2 * h][1], pa[2 * h + 1][0], pa[2 * h + 1][1]};
+                    if constexpr (DIRECT) {
+                        Mma<CT>::run(o[2 * n], a0, b[0], b[1]);
+                        Mma<CT>::run(o[2 * n + 1], a0, b[2], b[3]);
+                    } else {
+                        Mma<CT>::run(x, a0, b[0], b[1]);
+                        Mma<CT>::run(y, a0, b[2], b[3]);
+                        if constexpr (NP > 2) {
+                            const uint32_t a1[4] = {pa[2 * h][2], 0u, pa[2 * h + 1][2], 0u};
+                            Mma<CT>::run(x, a1, b[0], b[1]);
+                            Mma<CT>::run(y, a1, b[2], b[3]);
+                        }
                     }
+                }
+                if constexpr (!DIRECT) {
                     o[2 * n][0] = o[2 * n][0] * alpha + (x[0] + x[2]);
                     o[2 * n][1] = o[2 * n][1] * alpha + (x[1] + x[3]);
                     o[2 * n + 1][0] = o[2 * n + 1][0] * alpha + (y[0] + y[2]);
@@ -483,7 +508,9 @@ if (rows == ATT_TILE) {
         float *const mslot = reinterpret_cast<float *>(ring + (slot == 0 ? SH::S - 1 : slot - 1) * SH::TILE_BYTES);
         float *mw = mslot + g * (D + 4);
         if (lane == 0) mo[warp] = mslot;
-        if (CLUSTER && tid == 0) mo_at = (int)(reinterpret_cast<uint8_t *>(mslot) - smem);
+        if constexpr (CLUSTER) cl.barrier_wait();
+        if (CLUSTER && tid < (int)cl.num_blocks())  // tell every CTA where warp 0's sums are
+            *cl.map_shared_rank(&all_at[cl.block_rank()], tid) = (int)(reinterpret_cast<uint8_t *>(mslot) - smem);
 #pragma unroll
         for (int i = 0; i < D / 8; i++)
             *reinterpret_cast<float2 *>(mw + i * 8 + c2) =
@@ -492,16 +519,16 @@ if (rows == ATT_TILE) {
         __syncthreads();
         const bool whole = !CLUSTER && p.t == 0 && p.end == p.nt;
         const int64_t slot_id = 2 * (int64_t)blockIdx.x + (npart ? 1 : 0);
-        for (int i = tid; i < rows * (D / 4); i += ATT_W * 32) {
+        for (int i = tid; i < rows * (D / 4); i += THREADS) {
             const int r = i / (D / 4), x = (i - r * (D / 4)) * 4;
             float mm = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < ATT_W; w++) mm = fmaxf(mm, mml[w * ATT_R + r].x);
+            for (int w = 0; w < W; w++) mm = fmaxf(mm, mml[w * ATT_R + r].x);
             const float ref = mm == -INFINITY ? 0.0f : mm;
             float ll = 0.0f;
             float4 acc = make_float4(0, 0, 0, 0);
 #pragma unroll
-            for (int w = 0; w < ATT_W; w++) {
+            for (int w = 0; w < W; w++) {
                 const float2 e = mml[w * ATT_R + r];
                 const float s = exp2_fast(e.x - ref);
                 const float4 y = *reinterpret_cast<const float4 *>(mo[w] + r * (D + 4) + x);
@@ -511,7 +538,8 @@ if (rows == ATT_TILE) {
             const int64_t head = kvh * a.G + h0 + r;
             if (CLUSTER) {  // in place of warp 0's sums, whose elements only this thread reads
                 *reinterpret_cast<float4 *>(mo[0] + r * (D + 4) + x) = acc;
-                if (x == 0) cml[r] = make_float2(mm, ll);
+                if (x == 0)
+                    for (int c = 0; c < (int)cl.num_blocks(); c++) cl.map_shared_rank(&all_ml[0][0], c)[cl.block_rank() * ATT_R + r] = make_float2(mm, ll);
             } else if (whole) {
                 // no entry attended to (all on bad pages): zeros
                 const float inv = ll > 0.0f || ll != ll ? 1.0f / (ll * PSCALE) : 0.0f;
@@ -526,31 +554,32 @@ if (rows == ATT_TILE) {
             }
         }
         if constexpr (CLUSTER) {
-            // join the cluster's CTAs; each writes some of the columns
+            // join the cluster's CTAs, whose maxima and sums have been told to
+            // all; each writes some of the columns
             const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
             cl.sync();
             if (tid < rows) {
                 float mm = -INFINITY, ll = 0.0f;
-                for (int r = 0; r < C; r++) mm = fmaxf(mm, cl.map_shared_rank(cml, r)[tid].x);
+                for (int r = 0; r < C; r++) mm = fmaxf(mm, all_ml[r][tid].x);
                 const float ref = mm == -INFINITY ? 0.0f : mm;
-                for (int r = 0; r < C; r++) {
-                    const float2 e = cl.map_shared_rank(cml, r)[tid];
-                    ll += exp2_fast(e.x - ref) * e.y;
-                }
-                cml[ATT_R + tid] = make_float2(ref, ll > 0.0f || ll != ll ? 1.0f / ll : 0.0f);
+                for (int r = 0; r < C; r++) ll += exp2_fast(all_ml[r][tid].x - ref) * all_ml[r][tid].y;
+                cml[tid] = make_float2(ref, ll > 0.0f || ll != ll ? 1.0f / ll : 0.0f);
             }
             __syncthreads();
-            // (a CTA's sums are in the slot that its warp 0 came to: it says which)
-            for (int i = rank * ATT_W * 32 + tid; i < rows * (D / 4); i += C * ATT_W * 32) {
+            for (int i = rank * THREADS + tid; i < rows * (D / 4); i += C * THREADS) {
                 const int r = i / (D / 4), x = (i - r * (D / 4)) * 4;
-                const float2 fin = cml[ATT_R + r];
+                const float2 fin = cml[r];
+                float4 y[8];
+#pragma unroll
+                for (int c = 0; c < 8; c++)
+                    if (c < C) y[c] = *reinterpret_cast<const float4 *>(cl.map_shared_rank(smem, c) + all_at[c] + (r * (D + 4) + x) * 4);
                 float4 acc = make_float4(0, 0, 0, 0);
-                for (int c = 0; c < C; c++) {
-                    const float s = exp2_fast(cl.map_shared_rank(cml, c)[r].x - fin.x);
-                    const int at = *cl.map_shared_rank(&mo_at, c);
-                    const float4 y = *reinterpret_cast<const float4 *>(cl.map_shared_rank(smem, c) + at + (r * (D + 4) + x) * 4);
-                    acc.x += s * y.x, acc.y += s * y.y, acc.z += s * y.z, acc.w += s * y.w;
-                }
+#pragma unroll
+                for (int c = 0; c < 8; c++)
+                    if (c < C) {
+                        const float s = exp2_fast(all_ml[c][r].x - fin.x);
+                        acc.x += s * y[c].x, acc.y += s * y[c].y, acc.z += s * y[c].z, acc.w += s * y[c].w;
+                    }
                 const float inv = fin.y / PSCALE;
                 IO *dst = static_cast<IO *>(a.out) + p.b * a.out_stride + (int64_t)(kvh * a.G + h0 + r) * D + x;
                 dst[0] = from_f32<IO>(acc.x * inv), dst[1] = from_f32<IO>(acc.y * inv);
@@ -558,10 +587,10 @@ if (rows == ATT_TILE) {
             }
             if (a.z) {  // one pass per kv head here: this CTA's entries are its own
                 const int i1 = min(p.end * ATT_TILE, p.len);
-                for (int i = p.t * ATT_TILE + tid; i < i1; i += ATT_W * 32) {
+                for (int i = p.t * ATT_TILE + tid; i < i1; i += THREADS) {
                     const float *z = a.z + ((int64_t)p.b * a.H + kvh * a.G) * a.z_stride + i;
                     float add = 0.0f;
-                    for (int r = 0; r < rows; r++) add += exp2_fast(z[r * a.z_stride] - cml[ATT_R + r].x) * cml[ATT_R + r].y;
+                    for (int r = 0; r < rows; r++) add += exp2_fast(z[r * a.z_stride] - cml[r].x) * cml[r].y;
                     const int col = a.page.div(i), page = a.table[(int64_t)p.b * a.max_pages + col];
                     if (page >= 0 && page < a.n_pages) a.weight[((int64_t)page * a.KVH + kvh) * a.page_size + (i - col * a.page_size)] += add;
                 }
@@ -569,8 +598,12 @@ if (rows == ATT_TILE) {
             cl.sync();  // no CTA leaves while its sums are read
             break;
         }
+        f0 += p.end - p.t;
+        npart++;
+        if (f0 >= f1) break;
         __syncthreads();  // the slots may be filled again
-        f += p.end - p.t;
+        p = attn_part(prefix, last, a.B, nvh, f0, f1);
+        ask_queries(p);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
@@ -578,7 +611,7 @@ if (rows == ATT_TILE) {
 using AttnKernel = void (*)(AttnArgs);
 struct AttnVariant {
     AttnKernel run, cluster;
-    int head, ctas;  // shared memory without the per-sequence part, CTAs per SM
+    int head, ctas, warps;  // shared memory without the per-sequence part, CTAs per SM, warps per CTA
 };
 // The instances for a head width: cache type bf16 or fp16, activations f32 or the cache's.
 AttnVariant attn_variant_64(bool bf16, bool f32);
@@ -588,7 +621,7 @@ AttnVariant attn_variant_192(bool bf16, bool f32);
 AttnVariant attn_variant_256(bool bf16, bool f32);
 
 template <int D, typename CT, typename IO> AttnVariant attn_instances() {
-    return {attn_split_kernel<D, CT, IO, false>, attn_split_kernel<D, CT, IO, true>, AttnShape<D>::smem(0), AttnShape<D>::CTAS};
+    return {attn_split_kernel<D, CT, IO, false>, attn_split_kernel<D, CT, IO, true>, AttnShape<D>::smem(0), AttnShape<D>::CTAS, AttnShape<D>::W};
 }
 
 }  // namespace ofb
