@@ -6,23 +6,24 @@
 //   M = max m_i, out = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i,
 // so the result does not depend on which CTA took which run, nor on when. A CTA
 // takes one head, its warps every eighth part, where a head has many parts, and
-// eight heads of a kv head, a warp each, where it has few. With `accumulate`,
-// further CTAs add each entry's probability, summed over the query heads of its
-// kv head in their order, to the cache's weight: they read the scores the split
-// kernel left (4 bytes per entry and query head, an eighth of the entry's K and V
-// at 8 heads of 128; forming them again would read all of K a second time).
+// eight heads of a kv head, a warp each, where it has few.
+//
+// Third launch, with `accumulate`: each entry's probability, summed over the query
+// heads of its kv head in their order, is added to the cache's weight, four
+// entries per thread. It reads the scores the split kernel left (4 bytes per entry
+// and query head, an eighth of the entry's K and V at 8 heads of 128; forming them
+// again would read all of K a second time).
 #include "attn.cuh"
 
 namespace ofb {
 
 constexpr int AJ_THREADS = 256;
-constexpr int AJ_TURNS = 2;
-constexpr int AJ_CHUNK = AJ_TURNS * 4 * AJ_THREADS;  // entries of one weight CTA
+constexpr int AJ_CHUNK = 4 * AJ_THREADS;  // entries of one weight CTA
 
 struct AttnJoinArgs {
     AttnArgs a;
     int ctas, warps, d;       // of the split kernel: CTAs, warps of each; head_dim
-    int wide, n_out, chunks;  // one head per CTA; join CTAs; weight CTAs per (sequence, kv head)
+    int wide, chunks;         // one head per CTA; weight CTAs per (sequence, kv head)
 };
 
 // The runs that hold parts of (sequence b, pass vh): n of them from CTA c0's on.
@@ -32,28 +33,13 @@ struct PartRange {
     __device__ __forceinline__ int slot(int i) const { return 2 * (c0 + i) + (i == 0 && sp.first(c0) < f0 ? 1 : 0); }
 };
 __device__ __forceinline__ PartRange part_range(const AttnJoinArgs &j, int b, int vh, int nt) {
-    const int nvh = j.a.KVH * j.a.NB;
+    const int nvh = j.a.KVH * j.a.NB, places = nt + ATT_PART;
     PartRange r;
     r.sp = AttnSplit::make(j.a.prefix[j.a.B] * nvh, j.ctas, j.warps);
-    r.f0 = j.a.prefix[b] * nvh + vh * nt;
-    r.c0 = r.f0 / r.sp.run;
-    r.n = (r.f0 + nt - 1) / r.sp.run - r.c0 + 1;
+    r.f0 = j.a.prefix[b] * nvh + vh * places;
+    r.c0 = (r.f0 + ATT_PART) / r.sp.run;
+    r.n = (r.f0 + places - 1) / r.sp.run - r.c0 + 1;
     return r;
-}
-
-// Maximum and sum of exponentials over the parts of row r, by one warp.
-__device__ __forceinline__ float2 warp_ml(const AttnJoinArgs &j, const PartRange &pr, int r, int lane) {
-    float m = -INFINITY;
-    for (int i = lane; i < pr.n; i += 32) m = fmaxf(m, j.a.part_ml[pr.slot(i) * ATT_R + r].x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float ref = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f;
-    for (int i = lane; i < pr.n; i += 32) {
-        const float2 e = j.a.part_ml[pr.slot(i) * ATT_R + r];
-        l += exp2_fast(e.x - ref) * e.y;
-    }
-    return make_float2(ref, warp_sum(l));
 }
 
 // Sums over parts w, w + step, ... of row r, by one warp: lane x4 has columns
@@ -104,111 +90,117 @@ struct JoinSum {
 template <typename IO> __global__ void __launch_bounds__(AJ_THREADS) attn_join_kernel(const __grid_constant__ AttnJoinArgs j) {
     constexpr int W = AJ_THREADS / 32;
     __shared__ __align__(16) float acc[W][256 + 4];
-    __shared__ float2 ml[128];  // join: (maximum, sum) per warp; weights: (maximum, 1 / sum) of a head
+    __shared__ float2 ml[W];
     const AttnArgs &a = j.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_wait();
     pdl_trigger();
-    if (blockIdx.x < j.n_out) {
-        int b, vh, r;
-        if (j.wide) {
-            b = blockIdx.x / a.H;
-            const int h = blockIdx.x - b * a.H, kvh = h / a.G, g = h - kvh * a.G;
-            vh = kvh * a.NB + g / ATT_R, r = g % ATT_R;
-        } else {
-            b = blockIdx.x / (a.KVH * a.NB), vh = blockIdx.x - b * a.KVH * a.NB, r = warp;
+    int b, vh, r;
+    if (j.wide) {
+        b = blockIdx.x / a.H;
+        const int h = blockIdx.x - b * a.H, kvh = h / a.G, g = h - kvh * a.G;
+        vh = kvh * a.NB + g / ATT_R, r = g % ATT_R;
+    } else {
+        b = blockIdx.x / (a.KVH * a.NB), vh = blockIdx.x - b * a.KVH * a.NB, r = warp;
+    }
+    const int kvh = vh / a.NB, g = (vh - kvh * a.NB) * ATT_R + r, nt = a.prefix[b + 1] - a.prefix[b] - ATT_PART;
+    if (nt < 0) return;
+    const PartRange pr = part_range(j, b, vh, nt);
+    if (pr.n == 1 || g >= a.G) return;  // (`wide`: the CTA's only head, so all leave)
+    IO *const out = static_cast<IO *>(a.out) + b * a.out_stride + (int64_t)(kvh * a.G + g) * j.d;
+    JoinSum s;
+    s.add(j, pr, r, j.wide ? warp : 0, j.wide ? W : 1, lane);
+    if (!j.wide) {
+        if (lane == 0) a.ml[(int64_t)b * a.H + kvh * a.G + g] = make_float2(s.m, s.l);
+        const float inv = s.l > 0.0f || s.l != s.l ? 1.0f / s.l : 0.0f;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            const int x = 128 * h + 4 * lane;
+            if (x >= j.d) break;
+            out[x] = from_f32<IO>(s.o[h].x * inv), out[x + 1] = from_f32<IO>(s.o[h].y * inv);
+            out[x + 2] = from_f32<IO>(s.o[h].z * inv), out[x + 3] = from_f32<IO>(s.o[h].w * inv);
         }
-        const int kvh = vh / a.NB, g = (vh - kvh * a.NB) * ATT_R + r, nt = a.prefix[b + 1] - a.prefix[b];
-        if (!nt) return;
-        const PartRange pr = part_range(j, b, vh, nt);
-        if (pr.n == 1 || g >= a.G) return;  // (`wide`: the CTA's only head, so all leave)
-        IO *const out = static_cast<IO *>(a.out) + b * a.out_stride + (int64_t)(kvh * a.G + g) * j.d;
-        JoinSum s;
-        s.add(j, pr, r, j.wide ? warp : 0, j.wide ? W : 1, lane);
-        if (!j.wide) {
-            const float inv = s.l > 0.0f || s.l != s.l ? 1.0f / s.l : 0.0f;
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int x = 128 * h + 4 * lane;
-                if (x >= j.d) break;
-                out[x] = from_f32<IO>(s.o[h].x * inv), out[x + 1] = from_f32<IO>(s.o[h].y * inv);
-                out[x + 2] = from_f32<IO>(s.o[h].z * inv), out[x + 3] = from_f32<IO>(s.o[h].w * inv);
-            }
-            return;
-        }
-        if (lane == 0) ml[warp] = make_float2(s.m, s.l);
-#pragma unroll
-        for (int h = 0; h < 2; h++)
-            if (128 * h + 4 * lane < j.d) *reinterpret_cast<float4 *>(&acc[warp][128 * h + 4 * lane]) = s.o[h];
-        __syncthreads();
-        float m = -INFINITY, l = 0.0f, v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < W; w++) m = fmaxf(m, ml[w].x);
-        const float ref = m == -INFINITY ? 0.0f : m;
-#pragma unroll
-        for (int w = 0; w < W; w++) {
-            const float f = exp2_fast(ml[w].x - ref);
-            l += f * ml[w].y;
-            if (tid < j.d) v += f * acc[w][tid];
-        }
-        if (tid < j.d) out[tid] = from_f32<IO>(l > 0.0f || l != l ? v / l : 0.0f);
         return;
     }
-    // weights of entries [i0, i0 + AJ_CHUNK) of one (sequence, kv head), four
-    // consecutive ones per thread and turn
-    const int w = blockIdx.x - j.n_out, u = w / j.chunks, b = u / a.KVH, kvh = u - b * a.KVH, i0 = (w - u * j.chunks) * AJ_CHUNK;
-    const int len = attn_len(a, b);
+    if (lane == 0) ml[warp] = make_float2(s.m, s.l);
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+        if (128 * h + 4 * lane < j.d) *reinterpret_cast<float4 *>(&acc[warp][128 * h + 4 * lane]) = s.o[h];
+    __syncthreads();
+    float m = -INFINITY, l = 0.0f, v = 0.0f;
+#pragma unroll
+    for (int w = 0; w < W; w++) m = fmaxf(m, ml[w].x);
+    const float ref = m == -INFINITY ? 0.0f : m;
+#pragma unroll
+    for (int w = 0; w < W; w++) {
+        const float f = exp2_fast(ml[w].x - ref);
+        l += f * ml[w].y;
+        if (tid < j.d) v += f * acc[w][tid];
+    }
+    if (tid < j.d) out[tid] = from_f32<IO>(l > 0.0f || l != l ? v / l : 0.0f);
+    if (tid == 0) a.ml[(int64_t)b * a.H + kvh * a.G + g] = make_float2(m, l);
+}
+
+constexpr int AW_HEADS = 128;  // heads whose maximum and sum are in shared memory at a time
+__global__ void __launch_bounds__(AJ_THREADS) attn_weight_kernel(const __grid_constant__ AttnJoinArgs j) {
+    __shared__ float2 ml[AW_HEADS];  // (maximum, 1 / sum)
+    const AttnArgs &a = j.a;
+    const int tid = threadIdx.x;
+    const int u = blockIdx.x / j.chunks, b = u / a.KVH, kvh = u - b * a.KVH, i0 = (blockIdx.x - u * j.chunks) * AJ_CHUNK;
+    pdl_wait();
+    pdl_trigger();
+    const int len = attn_len(a, b), i = i0 + 4 * tid;
     if (i0 >= len) return;
-    const int nt = a.prefix[b + 1] - a.prefix[b];
-    float4 add[AJ_TURNS];
+    // the entries' weights, asked for beside the scores
+    const bool quad = a.quads && i + 3 < len;  // four entries in one page, 16-byte aligned
+    float *at[4] = {nullptr, nullptr, nullptr, nullptr};
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int k = 0; k < AJ_TURNS; k++) add[k] = make_float4(0, 0, 0, 0);
-    for (int g0 = 0; g0 < a.G; g0 += 128) {  // ml holds 128 heads at a time
-        const int ng = min(a.G - g0, 128);
-        for (int g = warp; g < ng; g += W) {
-            const PartRange pr = part_range(j, b, kvh * a.NB + (g0 + g) / ATT_R, nt);
-            const float2 e = pr.n == 1 ? a.ml[(int64_t)b * a.H + kvh * a.G + g0 + g] : warp_ml(j, pr, (g0 + g) % ATT_R, lane);
-            if (lane == 0) ml[g] = make_float2(e.x == -INFINITY ? 0.0f : e.x, e.y > 0.0f || e.y != e.y ? 1.0f / e.y : 0.0f);
+    for (int x = 0; x < 4; x++) {
+        if (i + x >= len || (quad && x)) break;
+        const int col = a.page.div(i + x), page = a.table[(int64_t)b * a.max_pages + col];
+        if (page < 0 || page >= a.n_pages) continue;
+        at[x] = a.weight + ((int64_t)page * a.KVH + kvh) * a.page_size + (i + x - col * a.page_size);
+        if (quad) {
+            const float4 y = *reinterpret_cast<const float4 *>(at[0]);
+            v[0] = y.x, v[1] = y.y, v[2] = y.z, v[3] = y.w;
+        } else {
+            v[x] = *at[x];
         }
+    }
+    float4 add = make_float4(0, 0, 0, 0);
+    for (int g0 = 0; g0 < a.G; g0 += AW_HEADS) {
+        const int ng = min(a.G - g0, AW_HEADS);
+        if (tid < ng) {
+            const float2 e = a.ml[(int64_t)b * a.H + kvh * a.G + g0 + tid];
+            ml[tid] = make_float2(e.x == -INFINITY ? 0.0f : e.x, e.y > 0.0f || e.y != e.y ? 1.0f / e.y : 0.0f);
+        }
+        // scores are there up to the end of the last tile
+        const float *z = a.z + ((int64_t)b * a.H + kvh * a.G + g0) * a.z_stride + i;
+        float4 x[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+            if (i < len && k < ng) x[k] = *reinterpret_cast<const float4 *>(z + k * a.z_stride);
         __syncthreads();
-        // scores are there up to the end of the last tile of 16
-        const float *z = a.z + ((int64_t)b * a.H + kvh * a.G + g0) * a.z_stride + i0 + 4 * tid;
-        for (int g = 0; g < ng; g++, z += a.z_stride) {
-            const float2 e = ml[g];
-            float4 x[AJ_TURNS];
+        for (int g = 0; i < len && g < ng; g += 4) {
 #pragma unroll
-            for (int k = 0; k < AJ_TURNS; k++)
-                if (i0 + 4 * tid + k * 4 * AJ_THREADS < len) x[k] = *reinterpret_cast<const float4 *>(z + k * 4 * AJ_THREADS);
-#pragma unroll
-            for (int k = 0; k < AJ_TURNS; k++) {
-                if (i0 + 4 * tid + k * 4 * AJ_THREADS >= len) break;
-                add[k].x += exp2_fast(x[k].x - e.x) * e.y, add[k].y += exp2_fast(x[k].y - e.x) * e.y;
-                add[k].z += exp2_fast(x[k].z - e.x) * e.y, add[k].w += exp2_fast(x[k].w - e.x) * e.y;
+            for (int k = 0; k < 4; k++) {
+                if (g + k >= ng) break;
+                const float2 e = ml[g + k];
+                add.x += exp2_fast(x[k].x - e.x) * e.y, add.y += exp2_fast(x[k].y - e.x) * e.y;
+                add.z += exp2_fast(x[k].z - e.x) * e.y, add.w += exp2_fast(x[k].w - e.x) * e.y;
+                if (g + 4 + k < ng) x[k] = *reinterpret_cast<const float4 *>(z + (g + 4 + k) * a.z_stride);
             }
         }
         __syncthreads();
     }
-#pragma unroll
-    for (int k = 0; k < AJ_TURNS; k++) {
-        const int i = i0 + 4 * tid + k * 4 * AJ_THREADS;
-        if (i >= len) break;
-        if (a.quads && i + 3 < len) {  // four entries in one page, 16-byte aligned
-            const int col = a.page.div(i), page = a.table[(int64_t)b * a.max_pages + col];
-            if (page < 0 || page >= a.n_pages) continue;
-            float4 *const at = reinterpret_cast<float4 *>(a.weight + ((int64_t)page * a.KVH + kvh) * a.page_size + (i - col * a.page_size));
-            float4 x = *at;
-            x.x += add[k].x, x.y += add[k].y, x.z += add[k].z, x.w += add[k].w;
-            *at = x;
-        } else {
-            const float v[4] = {add[k].x, add[k].y, add[k].z, add[k].w};
-#pragma unroll
-            for (int x = 0; x < 4; x++) {
-                if (i + x >= len) break;
-                const int col = a.page.div(i + x), page = a.table[(int64_t)b * a.max_pages + col];
-                if (page < 0 || page >= a.n_pages) continue;
-                a.weight[((int64_t)page * a.KVH + kvh) * a.page_size + (i + x - col * a.page_size)] += v[x];
-            }
-        }
+    if (quad) {
+        if (at[0]) *reinterpret_cast<float4 *>(at[0]) = make_float4(v[0] + add.x, v[1] + add.y, v[2] + add.z, v[3] + add.w);
+    } else {
+        if (at[0]) *at[0] = v[0] + add.x;
+        if (at[1]) *at[1] = v[1] + add.y;
+        if (at[2]) *at[2] = v[2] + add.z;
+        if (at[3]) *at[3] = v[3] + add.w;
     }
 }
 
@@ -238,7 +230,7 @@ static int attn_plan(const ofb_kv_cache *c, int n_heads, int n_seqs, int max_len
     p.max_len = max_len && max_len < reach ? max_len : reach;
     const int64_t tiles = ((int64_t)p.max_len + ATT_TILE - 1) / ATT_TILE;
     p.NB = (n_heads / c->n_kv_heads + ATT_R - 1) / ATT_R;
-    if (tiles * n_seqs > (1 << 30) / ((int64_t)c->n_kv_heads * p.NB)) {  // (sums of tile numbers stay within 31 bits)
+    if ((tiles + ATT_PART) * n_seqs > (1 << 30) / ((int64_t)c->n_kv_heads * p.NB)) {  // (sums of tile numbers stay within 31 bits)
         set_error("ofb_attn_decode: %d sequences of %d entries are too many tiles", n_seqs, p.max_len);
         return OFB_ETOOLARGE;
     }
@@ -325,10 +317,9 @@ extern "C" int ofb_attn_decode(const ofb_kv_cache *cache, const void *q, int typ
     j.ctas = p.ctas, j.warps = p.v.warps, j.d = cache->head_dim;
     // parts of a head, about, when all sequences are of the largest length
     j.wide = p.ctas >= 4 * n_seqs * a.KVH * a.NB;
-    j.n_out = j.wide ? n_seqs * n_heads : n_seqs * a.KVH * a.NB;
     j.chunks = (p.max_len + AJ_CHUNK - 1) / AJ_CHUNK;
-    const int64_t blocks = j.n_out + (accumulate ? (int64_t)n_seqs * a.KVH * j.chunks : 0);
-    if (blocks > INT32_MAX) { set_error("ofb_attn_decode: too many weight blocks"); return OFB_ETOOLARGE; }
+    const int64_t weight_ctas = (int64_t)n_seqs * a.KVH * j.chunks;
+    if (accumulate && weight_ctas > INT32_MAX) { set_error("ofb_attn_decode: too many weight blocks"); return OFB_ETOOLARGE; }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     // a raised shared-memory limit per kernel and device
     static size_t attr[40][64];
@@ -347,9 +338,12 @@ extern "C" int ofb_attn_decode(const ofb_kv_cache *cache, const void *q, int typ
     e = launch_pdl(p.v.run, dim3(p.ctas), dim3(p.v.warps * 32), smem, s, a);
     if (e != cudaSuccess) return cuda_status(e, "ofb_attn_decode launch");
     if (p.ctas == 1 && !accumulate) return OFB_OK;  // every part is whole
-    const dim3 grid((unsigned)blocks), block(AJ_THREADS);
+    const dim3 grid((unsigned)(n_seqs * (j.wide ? n_heads : a.KVH * a.NB))), block(AJ_THREADS);
     e = type == OFB_TYPE_F32              ? launch_pdl(attn_join_kernel<float>, grid, block, 0, s, j)
         : cache->type == OFB_TYPE_BF16 ? launch_pdl(attn_join_kernel<__nv_bfloat16>, grid, block, 0, s, j)
                                        : launch_pdl(attn_join_kernel<__half>, grid, block, 0, s, j);
-    return e == cudaSuccess ? OFB_OK : cuda_status(e, "ofb_attn_decode join launch");
+    if (e != cudaSuccess) return cuda_status(e, "ofb_attn_decode join launch");
+    if (!accumulate) return OFB_OK;
+    e = launch_pdl(attn_weight_kernel, dim3((unsigned)weight_ctas), block, 0, s, j);
+    return e == cudaSuccess ? OFB_OK : cuda_status(e, "ofb_attn_decode weight launch");
 }

@@ -70,8 +70,8 @@ struct AttnArgs {
     float scale;      // times log2(e)
     uint32_t *errors;
     // scratch
-    int *prefix;      // [B + 1] tiles before each sequence, per pass
-    float2 *ml;       // [B][H] maximum (log2) and sum of whole parts
+    int *prefix;      // [B + 1] places before each sequence, per pass
+    float2 *ml;       // [B][H] maximum (log2) and sum
     float *part_o;    // [2 * CTAs][ATT_R][d]
     float2 *part_ml;  // [2 * CTAs][ATT_R]
     float *z;         // [B][H][z_stride] scores in log2, or NULL
@@ -87,8 +87,11 @@ __device__ __forceinline__ float exp2_fast(float x) {  // 2 steps at most; below
 }
 // How many entries of sequence b are attended to.
 __device__ __forceinline__ int attn_len(const AttnArgs &a, int b) { return min(max(a.lens[b], 0), a.max_len); }
-// How the row of all tiles is cut into runs, one per CTA: at least a tile per
-// warp, so that few tiles do not leave many parts to join.
+// The row of all places: each (sequence, pass) with entries has ATT_PART places
+// that stand for the time a part costs besides its tiles (queries, the warps'
+// merge), then one per tile. It is cut into runs, one per CTA: at least a tile
+// per warp, so that few tiles do not leave many parts to join.
+constexpr int ATT_PART = 8;
 struct AttnSplit {
     int total, run;
     static __device__ __forceinline__ AttnSplit make(int total, int ctas, int warps) {
@@ -106,7 +109,7 @@ template <int D> struct AttnShape {
     static constexpr int THREADS = W * 32;
     static constexpr int RING = W * S * TILE_BYTES;
     // behind the ring: the warps' and the cluster's (maximum, sum), then per sequence
-    // the tiles before it and the entries of its last tile
+    // the places before it and the entries of its last tile
     static constexpr int HEAD = RING + (W + 1) * ATT_R * 8;
     static constexpr int smem(int B) { return HEAD + (B + 1) * 4 + (B + 3) / 4 * 4; }
     static_assert(TILE_BYTES >= ATT_R * (D + 4) * 4, "a warp's sums must fit one ring slot");
@@ -180,27 +183,28 @@ template <typename T, int N> __device__ __forceinline__ void split2(float x, flo
 }
 
 // A part: tiles [t, end) of (sequence b, pass vh), of nt tiles that hold len
-// entries.
+// entries; f_end: the place behind it in the row of all places.
 struct AttnPart {
-    int b, vh, t, end, nt, len;
+    int b, vh, t, end, nt, len, f_end;
 };
-// The part that begins at tile `f` of the row of all tiles, cut at f1.
+// The part that begins at place f, cut at f1 (it may then be without tiles).
 __device__ __forceinline__ AttnPart attn_part(const int *prefix, const uint8_t *last, int B, int nvh, int f, int f1) {
-    int lo = 0, hi = B - 1;  // the last sequence that begins at or before f (and has tiles)
+    int lo = 0, hi = B - 1;  // the last sequence that begins at or before f (and has places)
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (prefix[mid] * nvh <= f) lo = mid;
         else hi = mid - 1;
     }
     AttnPart p;
+    const int places = prefix[lo + 1] - prefix[lo], r = f - prefix[lo] * nvh;
     p.b = lo;
-    p.nt = prefix[lo + 1] - prefix[lo];
+    p.nt = places - ATT_PART;
     p.len = (p.nt - 1) * ATT_TILE + last[lo];
-    const int r = f - prefix[lo] * nvh;
-    p.vh = r / p.nt;
-    p.t = r - p.vh * p.nt;
-    const int left = f1 - f;
-    p.end = left < p.nt - p.t ? p.t + left : p.nt;
+    p.vh = r / places;
+    const int off = r - p.vh * places, n = min(f1 - f, places - off);
+    p.t = max(off - ATT_PART, 0);
+    p.end = max(off + n - ATT_PART, 0);
+    p.f_end = f + n;
     return p;
 }
 
@@ -245,6 +249,7 @@ __global__ void __launch_bounds__(AttnShape<D>::THREADS, AttnShape<D>::CTAS) att
         first.nt = (first.len + ATT_TILE - 1) / ATT_TILE;
         first.t = (int)((int64_t)rank * first.nt / C);
         first.end = (int)((int64_t)(rank + 1) * first.nt / C);
+        first.f_end = 1;
     } else {
         // the queries and the page table into L2 while the lengths are on their way
         {
@@ -254,7 +259,7 @@ __global__ void __launch_bounds__(AttnShape<D>::THREADS, AttnShape<D>::CTAS) att
                     prefetch_l2_line(static_cast<const char *>(a.q) + b * a.q_stride * (int)sizeof(IO) + i);
             if (i < (int64_t)a.B * a.max_pages * 4) prefetch_l2_line(reinterpret_cast<const char *>(a.table) + i);
         }
-        // tiles before each sequence; every CTA forms them for itself
+        // places before each sequence; every CTA forms them for itself
         for (int base = 0; base < a.B; base += THREADS) {
             const int b = base + tid;
             int n = 0;
@@ -263,6 +268,7 @@ __global__ void __launch_bounds__(AttnShape<D>::THREADS, AttnShape<D>::CTAS) att
                 if (a.lens[b] > a.max_len && blockIdx.x == 0) report(a.errors, OFB_CACHE_ELEN);
                 n = (len + ATT_TILE - 1) / ATT_TILE;
                 last[b] = (uint8_t)(len - (n - 1) * ATT_TILE);
+                if (n) n += ATT_PART;
             }
             int s = n;
 #pragma unroll
@@ -288,6 +294,7 @@ __global__ void __launch_bounds__(AttnShape<D>::THREADS, AttnShape<D>::CTAS) att
         f0 = sp.first(blockIdx.x), f1 = sp.first(blockIdx.x + 1);
         if (f0 >= f1) return;
         first = attn_part(prefix, last, a.B, nvh, f0, f1);
+        if (first.t >= first.end) return;
     }
 
     const uint32_t ring_s = ax::smem_u32(ring);
@@ -299,7 +306,7 @@ __global__ void __launch_bounds__(AttnShape<D>::THREADS, AttnShape<D>::CTAS) att
     bool more = true;
     auto look_up = [&]() {
         while (more && lt >= lp.end) {
-            lf += lp.end - lp.t;
+            lf = lp.f_end;
             if (CLUSTER || lf >= f1) more = false;
             else lp = attn_part(prefix, last, a.B, nvh, lf, f1), lt = lp.t + warp;
         }
@@ -516,6 +523,14 @@ __global__ void __launch_bounds__(AttnShape<D>::THREADS, AttnShape<D>::CTAS) att
             *reinterpret_cast<float2 *>(mw + i * 8 + c2) =
                 DIRECT ? make_float2(o[i][0] + o[i][NO - 2], o[i][1] + o[i][NO - 1]) : make_float2(o[i][0], o[i][1]);
         if ((lane & 3) == 0) mml[warp * ATT_R + g] = make_float2(m, l);
+        // the next part and its queries, on their way while the warps merge
+        AttnPart next = p;
+        bool go_on = false;
+        if (!CLUSTER && p.f_end < f1) {
+            next = attn_part(prefix, last, a.B, nvh, p.f_end, f1);
+            go_on = next.t < next.end;
+            if (go_on) ask_queries(next);
+        }
         __syncthreads();
         const bool whole = !CLUSTER && p.t == 0 && p.end == p.nt;
         const int64_t slot_id = 2 * (int64_t)blockIdx.x + (npart ? 1 : 0);
@@ -598,12 +613,10 @@ __global__ void __launch_bounds__(AttnShape<D>::THREADS, AttnShape<D>::CTAS) att
             cl.sync();  // no CTA leaves while its sums are read
             break;
         }
-        f0 += p.end - p.t;
+        if (!go_on) break;
         npart++;
-        if (f0 >= f1) break;
         __syncthreads();  // the slots may be filled again
-        p = attn_part(prefix, last, a.B, nvh, f0, f1);
-        ask_queries(p);
+        p = next;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
