@@ -330,8 +330,8 @@ int ofb_rope_append(const ofb_kv_cache *cache, const ofb_rope_config *rope, int 
  * joined in a fixed order (results are reproducible):
  *   out[b][h] = sum_n p_n v_n,  p = softmax over n < lens[b] of scale * q[b][h].k_n
  * where head h reads kv head h / (n_heads / n_kv_heads). lens: device int32
- * [n_seqs], n_seqs <= cache->n_seqs rows of the page table in order; a length
- * of 0 (or below) gives zeros. max_len bounds every length (0: the table's
+ * [n_seqs], n_seqs <= cache->n_seqs rows of the page table in order, at most
+ * OFB_ATTN_MAX_SEQS; a length of 0 (or below) gives zeros. max_len bounds every length (0: the table's
  * reach) and sizes the scratch. q and out: type OFB_TYPE_F32 or the cache's,
  * row b at b*q_stride (b*out_stride), heads consecutive; they must not overlap.
  * accumulate 1: cache->weight of entry n of kv head g grows by the sum of p_n
@@ -340,6 +340,7 @@ int ofb_rope_append(const ofb_kv_cache *cache, const ofb_rope_config *rope, int 
  * ofb_attn_scratch_size() bytes of device memory, 16-byte aligned, needing no
  * initialisation; calls whose GPU work may overlap (other streams, graphs
  * replayed side by side) need scratch of their own. */
+#define OFB_ATTN_MAX_SEQS 1536
 size_t ofb_attn_scratch_size(const ofb_kv_cache *cache, int n_heads, int n_seqs, int max_len, int accumulate);
 int ofb_attn_decode(const ofb_kv_cache *cache, const void *q, int type, int64_t q_stride, int n_heads, float scale,
                     const int32_t *lens, int n_seqs, int max_len, int accumulate, void *out, int64_t out_stride,

@@ -17,12 +17,12 @@
 
 namespace ofb {
 
-constexpr int AJ_THREADS = 256;
+constexpr int AJ_THREADS = 256;  // 8 warps, a row each where a CTA joins 8 rows
 constexpr int AJ_CHUNK = 4 * AJ_THREADS;  // entries of one weight CTA
 
 struct AttnJoinArgs {
     AttnArgs a;
-    int ctas, warps, d;       // of the split kernel: CTAs, warps of each; head_dim
+    int ctas, warps, rows, d; // of the split kernel: CTAs, warps of each, heads per pass; head_dim
     int wide, chunks;         // one head per CTA; weight CTAs per (sequence, kv head)
 };
 
@@ -60,7 +60,7 @@ struct JoinSum {
                 e[k] = make_float2(-INFINITY, 0.0f);
                 y[k][0] = y[k][1] = make_float4(0, 0, 0, 0);
                 if (i < pr.n) {
-                    const int p = pr.slot(i) * ATT_R + r;
+                    const int p = pr.slot(i) * j.rows + r;
                     const float *src = j.a.part_o + (int64_t)p * j.d;
                     e[k] = j.a.part_ml[p];
                     if (4 * lane < j.d) y[k][0] = *reinterpret_cast<const float4 *>(src + 4 * lane);
@@ -99,11 +99,12 @@ template <typename IO> __global__ void __launch_bounds__(AJ_THREADS) attn_join_k
     if (j.wide) {
         b = blockIdx.x / a.H;
         const int h = blockIdx.x - b * a.H, kvh = h / a.G, g = h - kvh * a.G;
-        vh = kvh * a.NB + g / ATT_R, r = g % ATT_R;
+        vh = kvh * a.NB + g / j.rows, r = g % j.rows;
     } else {
-        b = blockIdx.x / (a.KVH * a.NB), vh = blockIdx.x - b * a.KVH * a.NB, r = warp;
+        const int u = blockIdx.x / (j.rows / W);  // 8 rows per CTA
+        b = u / (a.KVH * a.NB), vh = u - b * a.KVH * a.NB, r = (blockIdx.x - u * (j.rows / W)) * W + warp;
     }
-    const int kvh = vh / a.NB, g = (vh - kvh * a.NB) * ATT_R + r, nt = a.prefix[b + 1] - a.prefix[b] - ATT_PART;
+    const int kvh = vh / a.NB, g = (vh - kvh * a.NB) * j.rows + r, nt = a.prefix[b + 1] - a.prefix[b] - ATT_PART;
     if (nt < 0) return;
     const PartRange pr = part_range(j, b, vh, nt);
     if (pr.n == 1 || g >= a.G) return;  // (`wide`: the CTA's only head, so all leave)
@@ -208,7 +209,7 @@ constexpr int ATT_SHORT = 4;
 
 struct AttnPlan {
     AttnVariant v;
-    int max_len, ctas, NB;
+    int max_len, ctas, NB, rows;
     int cluster;  // CTAs per (sequence, pass) that join by themselves, or 0: runs and a second launch
     int64_t z_stride;
     size_t prefix, ml, part_o, part_ml, z, total;
@@ -229,18 +230,20 @@ static int attn_plan(const ofb_kv_cache *c, int n_heads, int n_seqs, int max_len
     const int reach = cache_reach(c);
     p.max_len = max_len && max_len < reach ? max_len : reach;
     const int64_t tiles = ((int64_t)p.max_len + ATT_TILE - 1) / ATT_TILE;
-    p.NB = (n_heads / c->n_kv_heads + ATT_R - 1) / ATT_R;
+    const int group = n_heads / c->n_kv_heads;
+    p.rows = group > 8 && attn_wide_rows(c->head_dim, f32) ? 16 : 8;
+    p.NB = (group + p.rows - 1) / p.rows;
     if ((tiles + ATT_PART) * n_seqs > (1 << 30) / ((int64_t)c->n_kv_heads * p.NB)) {  // (sums of tile numbers stay within 31 bits)
         set_error("ofb_attn_decode: %d sequences of %d entries are too many tiles", n_seqs, p.max_len);
         return OFB_ETOOLARGE;
     }
     const bool bf = c->type == OFB_TYPE_BF16;
     switch (c->head_dim) {
-    case 64: p.v = attn_variant_64(bf, f32); break;
-    case 96: p.v = attn_variant_96(bf, f32); break;
-    case 128: p.v = attn_variant_128(bf, f32); break;
-    case 192: p.v = attn_variant_192(bf, f32); break;
-    default: p.v = attn_variant_256(bf, f32); break;
+    case 64: p.v = attn_variant_64(bf, f32, p.rows); break;
+    case 96: p.v = attn_variant_96(bf, f32, p.rows); break;
+    case 128: p.v = attn_variant_128(bf, f32, p.rows); break;
+    case 192: p.v = attn_variant_192(bf, f32, p.rows); break;
+    default: p.v = attn_variant_256(bf, f32, p.rows); break;
     }
     const int64_t runs = (tiles * n_seqs * c->n_kv_heads * p.NB + p.v.warps - 1) / p.v.warps;
     const int most = sm_count() * p.v.ctas;
@@ -254,15 +257,15 @@ static int attn_plan(const ofb_kv_cache *c, int n_heads, int n_seqs, int max_len
         if (tiles <= (int64_t)n * p.v.warps * ATT_SHORT && (int64_t)n_seqs * c->n_kv_heads * p.NB * n <= most) p.cluster = n;
     }
     p.ctas = runs < 1 ? 1 : runs < most ? (int)runs : most;
-    const size_t parts = 2 * (size_t)most;
+    const size_t parts = 2 * (size_t)ATT_MAX_CTAS * sm_count();  // whatever the type: one scratch serves both
     p.z_stride = tiles * ATT_TILE;
     size_t at = 0;
     auto take = [&](size_t bytes) { const size_t o = at; at += (bytes + 255) / 256 * 256; return o; };
     p.prefix = take((size_t)(n_seqs + 1) * 4);
     p.ml = take((size_t)n_seqs * n_heads * 8);
     // sized for a full grid, so that the size grows with n_seqs and max_len
-    p.part_ml = take(parts * ATT_R * 8);
-    p.part_o = take(parts * ATT_R * c->head_dim * 4);
+    p.part_ml = take(parts * 16 * 8);
+    p.part_o = take(parts * 16 * c->head_dim * 4);
     p.z = accumulate ? take((size_t)n_seqs * n_heads * p.z_stride * 4) : 0;
     p.total = at;
     return OFB_OK;
@@ -314,7 +317,7 @@ extern "C" int ofb_attn_decode(const ofb_kv_cache *cache, const void *q, int typ
     a.z = accumulate ? reinterpret_cast<float *>(w + p.z) : nullptr;
     a.z_stride = p.z_stride, a.weight = cache->weight;
     a.quads = a.page_size % 4 == 0 && !misaligned(a.weight, 16);
-    j.ctas = p.ctas, j.warps = p.v.warps, j.d = cache->head_dim;
+    j.ctas = p.ctas, j.warps = p.v.warps, j.rows = p.rows, j.d = cache->head_dim;
     // parts of a head, about, when all sequences are of the largest length
     j.wide = p.ctas >= 4 * n_seqs * a.KVH * a.NB;
     j.chunks = (p.max_len + AJ_CHUNK - 1) / AJ_CHUNK;
@@ -322,9 +325,9 @@ extern "C" int ofb_attn_decode(const ofb_kv_cache *cache, const void *q, int typ
     if (accumulate && weight_ctas > INT32_MAX) { set_error("ofb_attn_decode: too many weight blocks"); return OFB_ETOOLARGE; }
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     // a raised shared-memory limit per kernel and device
-    static size_t attr[40][64];
-    const int vi = (cache->head_dim == 64 ? 0 : cache->head_dim == 96 ? 1 : cache->head_dim == 128 ? 2 : cache->head_dim == 192 ? 3 : 4) * 8 +
-                   (cache->type == OFB_TYPE_BF16 ? 4 : 0) + (type == OFB_TYPE_F32 ? 2 : 0);
+    static size_t attr[80][64];
+    const int vi = (cache->head_dim == 64 ? 0 : cache->head_dim == 96 ? 1 : cache->head_dim == 128 ? 2 : cache->head_dim == 192 ? 3 : 4) * 16 +
+                   (cache->type == OFB_TYPE_BF16 ? 8 : 0) + (type == OFB_TYPE_F32 ? 4 : 0) + (p.rows == 16 ? 2 : 0);
     if (p.cluster) {
         cudaError_t e = ensure_dyn_smem(p.v.cluster, p.v.head, attr[vi + 1]);
         if (e != cudaSuccess) return cuda_status(e, "ofb_attn_decode smem attribute");
@@ -338,7 +341,7 @@ extern "C" int ofb_attn_decode(const ofb_kv_cache *cache, const void *q, int typ
     e = launch_pdl(p.v.run, dim3(p.ctas), dim3(p.v.warps * 32), smem, s, a);
     if (e != cudaSuccess) return cuda_status(e, "ofb_attn_decode launch");
     if (p.ctas == 1 && !accumulate) return OFB_OK;  // every part is whole
-    const dim3 grid((unsigned)(n_seqs * (j.wide ? n_heads : a.KVH * a.NB))), block(AJ_THREADS);
+    const dim3 grid((unsigned)(n_seqs * (j.wide ? n_heads : a.KVH * a.NB * (p.rows / (AJ_THREADS / 32))))), block(AJ_THREADS);
     e = type == OFB_TYPE_F32              ? launch_pdl(attn_join_kernel<float>, grid, block, 0, s, j)
         : cache->type == OFB_TYPE_BF16 ? launch_pdl(attn_join_kernel<__nv_bfloat16>, grid, block, 0, s, j)
                                        : launch_pdl(attn_join_kernel<__half>, grid, block, 0, s, j);

@@ -28,16 +28,19 @@
 // distributed shared memory, which saves the second launch.
 //
 // The products run on mma.sync m16n8k16 (bf16 or fp16, f32 sums): 16 rows of A
-// by 8 entries or 8 output columns. Query heads of one kv head fill 8 rows at
-// most; the other 8 take the low-order parts of the same numbers, so that
-// neither an f32 query nor a probability is rounded to the cache's type:
+// by 8 entries or 8 output columns. Neither an f32 query nor a probability is
+// rounded to the cache's type; both go in as parts of that type:
 //   query: in the cache's type one part, exact. f32: bf16 hi + mid + low (24
-//     bits, two mma) or fp16 hi + low (22 bits, one mma) of q scaled by a power
-//     of two into fp16's range.
-//   probability: bf16 hi + low (16 bits) or, for f32 output, + lowest (24
-//     bits, a second mma); fp16 hi + low of 2^14 p (22 bits).
-// A row's parts end in the same thread (accumulators c0, c1 and c2, c3), which
-// adds them in f32. With f32 output each tile's product starts at zero and is
+//     bits) or fp16 hi + low (22 bits) of q scaled by a power of two into fp16's
+//     range.
+//   probability: bf16 hi + low (16 bits) or, for f32 output, + lowest (24 bits);
+//     fp16 hi + low of 2^14 p (22 bits).
+// Up to 8 query heads of a kv head fill 8 rows; the other 8 rows take the next
+// part of the same numbers, so that two parts cost one product. 9 to 16 heads
+// (R = 16) fill all rows, with a product per part; more take several passes over
+// K and V, and so do 9 to 16 f32 heads of 192 or 256, whose queries and sums are
+// more than the registers hold.
+// A number's parts end in the same thread, which adds them in f32. With f32 output each tile's product starts at zero and is
 // added to the running sum by an FFMA, since the tensor core's own accumulation
 // cuts off where an addition rounds; with 16-bit output, whose own rounding is
 // coarser than that by far, the tensor core accumulates up to head_dim 128.
@@ -54,15 +57,15 @@ namespace cg = cooperative_groups;
 namespace ofb {
 
 constexpr int ATT_TILE = 32;  // entries per tile, one per lane
-constexpr int ATT_R = 8;      // query heads per pass
-constexpr int ATT_MAX_SEQS = 2048;
+constexpr int ATT_MAX_SEQS = OFB_ATTN_MAX_SEQS;
+constexpr int ATT_MAX_CTAS = 2;  // per SM, of any instance
 
 struct AttnArgs {
     const void *k, *v, *q;
     void *out;
     const int32_t *table, *lens;
     int64_t page_stride, q_stride, out_stride;
-    int B, KVH, G, NB, H;  // NB: passes of at most ATT_R heads per kv head
+    int B, KVH, G, NB, H;  // NB: passes of at most R heads per kv head
     FastDiv page;  // by page_size
     int page_size, max_pages, n_pages, max_len;
     int halves;       // page_size is a multiple of 16: each half of a tile lies in one page
@@ -72,8 +75,8 @@ struct AttnArgs {
     // scratch
     int *prefix;      // [B + 1] places before each sequence, per pass
     float2 *ml;       // [B][H] maximum (log2) and sum
-    float *part_o;    // [2 * CTAs][ATT_R][d]
-    float2 *part_ml;  // [2 * CTAs][ATT_R]
+    float *part_o;    // [2 * CTAs][R][d]
+    float2 *part_ml;  // [2 * CTAs][R]
     float *z;         // [B][H][z_stride] scores in log2, or NULL
     int64_t z_stride;
     float *weight;
@@ -100,7 +103,19 @@ struct AttnSplit {
     __device__ __forceinline__ int first(int id) const { return (int)min((int64_t)id * run, (int64_t)total); }
 };
 
-template <int D> struct AttnShape {
+// How the queries of an instance go in (see the top): parts, fragments of A, and
+// whether the fragments are in shared memory, one copy for all warps, instead of
+// each warp's registers. That is where registers cannot hold them beside the
+// sums: 8 heads of 256, f32, bf16 cache (24 sequences of 8 to 40 thousand entries
+// 268 -> 209 us).
+template <int D, int R, typename CT, typename IO> struct AttnQuery {
+    static constexpr bool F32 = sizeof(IO) == 4, BF = std::is_same<CT, __nv_bfloat16>::value;
+    static constexpr int NQ = F32 ? (BF ? 3 : 2) : 1;
+    static constexpr int QF = R == 8 ? (NQ + 1) / 2 : NQ;
+    static constexpr bool QS = F32 && BF && R == 8 && D == 256;
+    static constexpr int QB = QS ? D / 16 * 32 * 24 : 0;  // bytes
+};
+template <int D, int QB> struct AttnShape {
     static constexpr int PITCH = D * 2 + 16;                 // bytes of a row in shared memory
     static constexpr int TILE_BYTES = 2 * ATT_TILE * PITCH;  // K, then V
     static constexpr int W = D == 128 || D == 256 ? 3 : 4;   // warps per CTA
@@ -108,11 +123,13 @@ template <int D> struct AttnShape {
     static constexpr int CTAS = D <= 128 ? 2 : 1;            // per SM
     static constexpr int THREADS = W * 32;
     static constexpr int RING = W * S * TILE_BYTES;
-    // behind the ring: the warps' and the cluster's (maximum, sum), then per sequence
+    // behind the ring: the warps' and the cluster's (maximum, sum), the queries'
+    // fragments, then per sequence
     // the places before it and the entries of its last tile
-    static constexpr int HEAD = RING + (W + 1) * ATT_R * 8;
+    static constexpr int HEAD = RING + (W + 1) * 16 * 8 + QB;
     static constexpr int smem(int B) { return HEAD + (B + 1) * 4 + (B + 3) / 4 * 4; }
-    static_assert(TILE_BYTES >= ATT_R * (D + 4) * 4, "a warp's sums must fit one ring slot");
+    static_assert(CTAS <= ATT_MAX_CTAS, "parts in the scratch");
+    static_assert(TILE_BYTES >= 16 * (D + 4) * 4, "a warp's sums must fit one ring slot");
     static_assert(CTAS * (smem(384) + 2048) <= 228 * 1024, "shared memory of an SM");
     static_assert(smem(ATT_MAX_SEQS) + 1024 <= 227 * 1024, "shared memory of a CTA");
 };
@@ -208,28 +225,38 @@ __device__ __forceinline__ AttnPart attn_part(const int *prefix, const uint8_t *
     return p;
 }
 
-template <int D, typename CT, typename IO, bool CLUSTER>
-__global__ void __launch_bounds__(AttnShape<D>::THREADS, AttnShape<D>::CTAS) attn_split_kernel(const __grid_constant__ AttnArgs a) {
-    using SH = AttnShape<D>;
-    constexpr bool F32 = sizeof(IO) == 4, BF = std::is_same<CT, __nv_bfloat16>::value;
-    constexpr int NQ = F32 ? (BF ? 3 : 2) : 1;       // parts of a query
+template <int D, int R, typename CT, typename IO, bool CLUSTER>
+__global__ void __launch_bounds__(AttnShape<D, AttnQuery<D, R, CT, IO>::QB>::THREADS,
+                                  AttnShape<D, AttnQuery<D, R, CT, IO>::QB>::CTAS) attn_split_kernel(const __grid_constant__ AttnArgs a) {
+    using Q = AttnQuery<D, R, CT, IO>;
+    using SH = AttnShape<D, Q::QB>;
+    constexpr bool F32 = Q::F32, BF = Q::BF, QS = Q::QS;
+    constexpr int NQ = Q::NQ, QF = Q::QF;            // parts of a query; fragments
     constexpr int NP = BF && F32 ? 3 : 2;            // parts of a probability
     constexpr float PSCALE = BF ? 1.0f : 16384.0f;   // fp16 holds 2^14 p
+    constexpr int NR = R / 8;                        // query heads of a thread: g, g + 8
+    constexpr int PF = R == 8 ? (NP + 1) / 2 : NP;   // fragments: two parts of 8 heads, or a part of 16
     constexpr bool DIRECT = !F32 && D <= 128;        // the tensor core accumulates (registers allow no more)
-    constexpr int NO = DIRECT ? 4 : 2;               // accumulators of 8 columns
+    constexpr int NO = DIRECT || R == 16 ? 4 : 2;    // accumulators of 8 columns
     constexpr int KS = D / 16, CH = D / 8;           // k steps; 16-byte chunks of a row
     constexpr int W = SH::W, THREADS = SH::THREADS;
+    // the next part's queries are asked for while registers hold them beside the sums
+    constexpr bool AHEAD = NR * D * sizeof(IO) <= 512;
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c2 = (lane & 3) * 2;
     uint8_t *ring = smem + warp * SH::S * SH::TILE_BYTES;
     float2 *mml = reinterpret_cast<float2 *>(smem + SH::RING);  // [W][R]
-    float2 *cml = mml + W * ATT_R;                          // [R]: the cluster's
+    float2 *cml = mml + W * R;                          // [R]: the cluster's
     int *prefix = reinterpret_cast<int *>(smem + SH::HEAD);     // [B + 1]
     uint8_t *last = reinterpret_cast<uint8_t *>(prefix + a.B + 1);
+    // fragments: [KS][32] of four registers, then [KS][32] of the two of the second
+    // fragment that are not zero
+    uint4 *const q4 = reinterpret_cast<uint4 *>(smem + SH::RING + (W + 1) * 16 * 8);
+    uint2 *const q2 = reinterpret_cast<uint2 *>(q4 + KS * 32);
     __shared__ uint32_t valid[W][4];  // per ring slot: which of the 32 entries are there
     __shared__ int wsum[W];
     __shared__ float *mo[W];  // each warp's sums at the end of a part, [R][D + 4]
-    __shared__ float2 all_ml[8][ATT_R];  // CLUSTER: every CTA's (maximum, sum) ...
+    __shared__ float2 all_ml[8][R];  // CLUSTER: every CTA's (maximum, sum) ...
     __shared__ int all_at[8];            // ... and where its sums are in its shared memory
     cg::cluster_group cl = cg::this_cluster();
 
@@ -357,18 +384,21 @@ __global__ void __launch_bounds__(AttnShape<D>::THREADS, AttnShape<D>::CTAS) att
     look_up();
     // Queries: row g of A, parts as told at the top. The first part's are asked
     // for before the rings fill, whose copies would keep them waiting.
-    IO qx[KS][2][2];
+    IO qx[NR][KS][2][2];
     auto ask_queries = [&](const AttnPart &p) {
-        const int kvh = p.vh / a.NB, h0 = (p.vh - kvh * a.NB) * ATT_R;
-        const IO *qr = static_cast<const IO *>(a.q) + p.b * a.q_stride + (int64_t)(kvh * a.G + h0 + g) * D + c2;
-        const bool there = g < min(ATT_R, a.G - h0);
+        const int kvh = p.vh / a.NB, h0 = (p.vh - kvh * a.NB) * R;
 #pragma unroll
-        for (int ks = 0; ks < KS; ks++)
+        for (int n = 0; n < NR; n++) {
+            const IO *qr = static_cast<const IO *>(a.q) + p.b * a.q_stride + (int64_t)(kvh * a.G + h0 + g + 8 * n) * D + c2;
+            const bool there = g + 8 * n < min(R, a.G - h0);
 #pragma unroll
-            for (int u = 0; u < 2; u++) {
-                qx[ks][u][0] = there ? qr[ks * 16 + u * 8] : from_f32<IO>(0.0f);
-                qx[ks][u][1] = there ? qr[ks * 16 + u * 8 + 1] : from_f32<IO>(0.0f);
-            }
+            for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    qx[n][ks][u][0] = there ? qr[ks * 16 + u * 8] : from_f32<IO>(0.0f);
+                    qx[n][ks][u][1] = there ? qr[ks * 16 + u * 8 + 1] : from_f32<IO>(0.0f);
+                }
+        }
     };
     ask_queries(first);
 #pragma unroll
@@ -378,33 +408,60 @@ __global__ void __launch_bounds__(AttnShape<D>::THREADS, AttnShape<D>::CTAS) att
     int npart = 0;
     AttnPart p = first;
     for (;;) {
-        const int kvh = p.vh / a.NB, h0 = (p.vh - kvh * a.NB) * ATT_R, rows = min(ATT_R, a.G - h0);
-        uint32_t qa[KS][2][NQ];
-        float qscale = a.scale;
-        {
-            float up = 1.0f;
+        const int kvh = p.vh / a.NB, h0 = (p.vh - kvh * a.NB) * R, rows = min(R, a.G - h0);
+        uint32_t qa[QS ? 1 : KS][2][QF][2];  // [k step][k half][fragment][row g, row g + 8]
+        float qscale[NR];
+        float up[NR];
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+            up[n] = 1.0f;
+            qscale[n] = a.scale;
             if constexpr (F32 && !BF) {
                 // a power of two that brings the row's largest element to [2^13, 2^14)
                 float m = 0.0f;
 #pragma unroll
                 for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-                    for (int u = 0; u < 2; u++) m = fmaxf(m, fmaxf(fabsf(qx[ks][u][0]), fabsf(qx[ks][u][1])));
+                    for (int u = 0; u < 2; u++) m = fmaxf(m, fmaxf(fabsf(qx[n][ks][u][0]), fabsf(qx[n][ks][u][1])));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
                 m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
                 const int e = (int)(__float_as_uint(m) >> 23);  // 0: zero or subnormal, 255: not finite
                 if (e > 0 && e < 255) {
                     const int sh = min(max(13 + 127 - e, -100), 100);
-                    up = __uint_as_float((uint32_t)(127 + sh) << 23);
-                    qscale = a.scale * __uint_as_float((uint32_t)(127 - sh) << 23);
+                    up[n] = __uint_as_float((uint32_t)(127 + sh) << 23);
+                    qscale[n] = a.scale * __uint_as_float((uint32_t)(127 - sh) << 23);
                 }
             }
-#pragma unroll
-            for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-                for (int u = 0; u < 2; u++) split2<CT, NQ>(to_f32(qx[ks][u][0]) * up, to_f32(qx[ks][u][1]) * up, qa[ks][u]);
         }
-        float o[D / 8][NO], m = -INFINITY, l = 0.0f;
+#pragma unroll
+        for (int ks = 0; ks < KS; ks++) {
+            if (QS && ks % W != warp) continue;
+            uint32_t(&to)[2][QF][2] = qa[QS ? 0 : ks];
+#pragma unroll
+            for (int n = 0; n < NR; n++)
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    uint32_t part[NQ];
+                    split2<CT, NQ>(to_f32(qx[n][ks][u][0]) * up[n], to_f32(qx[n][ks][u][1]) * up[n], part);
+#pragma unroll
+                    for (int f = 0; f < QF; f++) {
+                        if (R == 8) {
+                            to[u][f][0] = part[2 * f];
+                            to[u][f][1] = 2 * f + 1 < NQ ? part[2 * f + 1 < NQ ? 2 * f + 1 : 0] : 0u;
+                        } else {
+                            to[u][f][n] = part[f];
+                        }
+                    }
+                }
+            if constexpr (QS) {
+                q4[ks * 32 + lane] = make_uint4(to[0][0][0], to[0][0][1], to[1][0][0], to[1][0][1]);
+                q2[ks * 32 + lane] = make_uint2(to[0][1][0], to[1][1][0]);
+            }
+        }
+        if (QS) __syncthreads();
+        float o[D / 8][NO], m[NR], l[NR];
+#pragma unroll
+        for (int n = 0; n < NR; n++) m[n] = -INFINITY, l[n] = 0.0f;
 #pragma unroll
         for (int i = 0; i < D / 8; i++)
 #pragma unroll
@@ -418,99 +475,121 @@ __global__ void __launch_bounds__(AttnShape<D>::THREADS, AttnShape<D>::CTAS) att
             const uint32_t ok = valid[warp][slot] >> c2;
             slot = slot == SH::S - 1 ? 0 : slot + 1;
 
-            // scores of 8 entries each; with three parts the lowest apart
-            float s[4][4] = {}, sl[NQ > 2 ? 4 : 1][4] = {};
+            // scores of 8 entries each; the second fragment on apart, so that small
+            // numbers are not cut off against large ones
+            float s[4][4] = {}, sl[QF > 1 ? 4 : 1][4] = {};
             const uint32_t ka = ks_s + ((lane & 7) + ((lane >> 4) << 3)) * SH::PITCH + ((lane >> 3) & 1) * 16;
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
-                const uint32_t a0[4] = {qa[ks][0][0], NQ > 1 ? qa[ks][0][NQ > 1 ? 1 : 0] : 0u, qa[ks][1][0],
-                                        NQ > 1 ? qa[ks][1][NQ > 1 ? 1 : 0] : 0u};
+                uint4 x = {};
+                uint2 y = {};
+                if constexpr (QS) x = q4[ks * 32 + lane], y = q2[ks * 32 + lane];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     uint32_t b[4];
                     ldmatrix4(b, ka + h * 16 * SH::PITCH + ks * 32);
-                    Mma<CT>::run(s[2 * h], a0, b[0], b[1]);
-                    Mma<CT>::run(s[2 * h + 1], a0, b[2], b[3]);
-                    if constexpr (NQ > 2) {
-                        const uint32_t a1[4] = {qa[ks][0][2], 0u, qa[ks][1][2], 0u};
-                        Mma<CT>::run(sl[2 * h], a1, b[0], b[1]);
-                        Mma<CT>::run(sl[2 * h + 1], a1, b[2], b[3]);
+#pragma unroll
+                    for (int f = 0; f < QF; f++) {
+                        const int k = QS ? 0 : ks;
+                        const uint32_t af[4] = {QS ? (f ? y.x : x.x) : qa[k][0][f][0], QS ? (f ? 0u : x.y) : qa[k][0][f][1],
+                                                QS ? (f ? y.y : x.z) : qa[k][1][f][0], QS ? (f ? 0u : x.w) : qa[k][1][f][1]};
+                        Mma<CT>::run(f ? sl[QF > 1 ? 2 * h : 0] : s[2 * h], af, b[0], b[1]);
+                        Mma<CT>::run(f ? sl[QF > 1 ? 2 * h + 1 : 0] : s[2 * h + 1], af, b[2], b[3]);
                     }
                 }
             }
-            // row g, entries 8j + c2 + {0, 1}, in log2
-            float z[4][2], mt = -INFINITY;
+            // rows g (and g + 8), entries 8j + c2 + {0, 1}, in log2
+            float z[NR][4][2], alpha[NR];
+            uint32_t pa[4][PF][2];  // [8 entries][fragment][row g, row g + 8]
+            bool grown = false;
 #pragma unroll
-            for (int j = 0; j < 4; j++)
+            for (int n = 0; n < NR; n++) {
+                float mt = -INFINITY;
 #pragma unroll
-                for (int u = 0; u < 2; u++) {
-                    float x = s[j][u];
-                    if (NQ > 1) x += s[j][2 + u];
-                    if constexpr (NQ > 2) x += sl[j][u];
-                    z[j][u] = (ok >> (8 * j + u)) & 1 ? x * qscale : -INFINITY;
-                    mt = fmaxf(mt, z[j][u]);
+                for (int j = 0; j < 4; j++)
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        float x = s[j][2 * n + u];
+                        if (R == 8 && NQ > 1) x += s[j][2 + u];
+                        if constexpr (QF > 1) x += sl[j][2 * n + u];
+                        z[n][j][u] = (ok >> (8 * j + u)) & 1 ? x * qscale[n] : -INFINITY;
+                        mt = fmaxf(mt, z[n][j][u]);
+                    }
+                if (a.z && g + 8 * n < rows) {
+                    float *zr = a.z + ((int64_t)p.b * a.H + kvh * a.G + h0 + g + 8 * n) * a.z_stride + t * ATT_TILE + c2;
+#pragma unroll
+                    for (int j = 0; j < 4; j++) *reinterpret_cast<float2 *>(zr + 8 * j) = make_float2(z[n][j][0], z[n][j][1]);
                 }
-            if (a.z && g < rows) {
-                float *zr = a.z + ((int64_t)p.b * a.H + kvh * a.G + h0 + g) * a.z_stride + t * ATT_TILE + c2;
+                mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
+                mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
+                const float mn = fmaxf(m[n], mt), ref = mn == -INFINITY ? 0.0f : mn;
+                alpha[n] = exp2_fast(m[n] - ref);  // 0 at the first tile
+                grown |= mn != m[n];
+                m[n] = mn;
+                float sum = 0.0f;
 #pragma unroll
-                for (int j = 0; j < 4; j++) *reinterpret_cast<float2 *>(zr + 8 * j) = make_float2(z[j][0], z[j][1]);
-            }
-            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 1));
-            mt = fmaxf(mt, __shfl_xor_sync(0xffffffffu, mt, 2));
-            const float mn = fmaxf(m, mt), ref = mn == -INFINITY ? 0.0f : mn;
-            const float alpha = exp2_fast(m - ref);  // 0 at the first tile
-            const bool grown = __any_sync(0xffffffffu, mn != m);
-            m = mn;
-            uint32_t pa[4][NP];  // [8 entries][part]
-            float sum = 0.0f;
+                for (int j = 0; j < 4; j++) {
+                    const float x = exp2_fast(z[n][j][0] - ref), y = exp2_fast(z[n][j][1] - ref);
+                    sum += x + y;
+                    uint32_t part[NP];
+                    split2<CT, NP>(x * PSCALE, y * PSCALE, part);
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float x = exp2_fast(z[j][0] - ref), y = exp2_fast(z[j][1] - ref);
-                sum += x + y;
-                split2<CT, NP>(x * PSCALE, y * PSCALE, pa[j]);
+                    for (int f = 0; f < PF; f++) {
+                        if (R == 8) {
+                            pa[j][f][0] = part[2 * f];
+                            pa[j][f][1] = 2 * f + 1 < NP ? part[2 * f + 1 < NP ? 2 * f + 1 : 0] : 0u;
+                        } else {
+                            pa[j][f][n] = part[f];
+                        }
+                    }
+                }
+                l[n] = l[n] * alpha[n] + sum;
             }
-            l = l * alpha + sum;
-            if (DIRECT && grown) {
+            if (DIRECT && __any_sync(0xffffffffu, grown)) {
 #pragma unroll
                 for (int i = 0; i < D / 8; i++)
 #pragma unroll
-                    for (int u = 0; u < NO; u++) o[i][u] *= alpha;
+                    for (int u = 0; u < NO; u++) o[i][u] *= alpha[R == 8 ? 0 : u / 2];
             }
             const uint32_t va = vs_s + ((lane & 7) + ((lane >> 3) & 1) * 8) * SH::PITCH + (lane >> 4) * 16;
 #pragma unroll
             for (int n = 0; n < D / 16; n++) {
-                float x[4] = {}, y[4] = {};
+                float x[2][4] = {};  // of 8 columns each
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     uint32_t b[4];
                     ldmatrix4_t(b, va + h * 16 * SH::PITCH + n * 32);
-                    const uint32_t a0[4] = {pa[2 * h][0], pa[2 * h][1], pa[2 * h + 1][0], pa[2 * h + 1][1]};
-                    if constexpr (DIRECT) {
-                        Mma<CT>::run(o[2 * n], a0, b[0], b[1]);
-                        Mma<CT>::run(o[2 * n + 1], a0, b[2], b[3]);
-                    } else {
-                        Mma<CT>::run(x, a0, b[0], b[1]);
-                        Mma<CT>::run(y, a0, b[2], b[3]);
-                        if constexpr (NP > 2) {
-                            const uint32_t a1[4] = {pa[2 * h][2], 0u, pa[2 * h + 1][2], 0u};
-                            Mma<CT>::run(x, a1, b[0], b[1]);
-                            Mma<CT>::run(y, a1, b[2], b[3]);
+#pragma unroll
+                    for (int f = 0; f < PF; f++) {
+                        const uint32_t af[4] = {pa[2 * h][f][0], pa[2 * h][f][1], pa[2 * h + 1][f][0], pa[2 * h + 1][f][1]};
+                        if constexpr (DIRECT) {
+                            Mma<CT>::run(o[2 * n], af, b[0], b[1]);
+                            Mma<CT>::run(o[2 * n + 1], af, b[2], b[3]);
+                        } else {
+                            Mma<CT>::run(x[0], af, b[0], b[1]);
+                            Mma<CT>::run(x[1], af, b[2], b[3]);
                         }
                     }
                 }
                 if constexpr (!DIRECT) {
-                    o[2 * n][0] = o[2 * n][0] * alpha + (x[0] + x[2]);
-                    o[2 * n][1] = o[2 * n][1] * alpha + (x[1] + x[3]);
-                    o[2 * n + 1][0] = o[2 * n + 1][0] * alpha + (y[0] + y[2]);
-                    o[2 * n + 1][1] = o[2 * n + 1][1] * alpha + (y[1] + y[3]);
+#pragma unroll
+                    for (int i = 0; i < 2; i++)
+#pragma unroll
+                        for (int u = 0; u < NO; u++) {
+                            const float y = R == 8 ? x[i][u] + x[i][u + 2 < 4 ? u + 2 : 0] : x[i][u];
+                            o[2 * n + i][u] = o[2 * n + i][u] * alpha[R == 8 ? 0 : u / 2] + y;
+                        }
                 }
             }
         }
         // merge the warps: their sums, maxima and sums of exponentials. A warp
         // leaves its sums in the ring slot it computed last, which the next
         // fill is for (at the start: the one not filled yet).
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
+#pragma unroll
+        for (int n = 0; n < NR; n++) {
+            l[n] += __shfl_xor_sync(0xffffffffu, l[n], 1);
+            l[n] += __shfl_xor_sync(0xffffffffu, l[n], 2);
+        }
         __syncwarp();
         float *const mslot = reinterpret_cast<float *>(ring + (slot == 0 ? SH::S - 1 : slot - 1) * SH::TILE_BYTES);
         float *mw = mslot + g * (D + 4);
@@ -519,17 +598,25 @@ __global__ void __launch_bounds__(AttnShape<D>::THREADS, AttnShape<D>::CTAS) att
         if (CLUSTER && tid < (int)cl.num_blocks())  // tell every CTA where warp 0's sums are
             *cl.map_shared_rank(&all_at[cl.block_rank()], tid) = (int)(reinterpret_cast<uint8_t *>(mslot) - smem);
 #pragma unroll
-        for (int i = 0; i < D / 8; i++)
-            *reinterpret_cast<float2 *>(mw + i * 8 + c2) =
-                DIRECT ? make_float2(o[i][0] + o[i][NO - 2], o[i][1] + o[i][NO - 1]) : make_float2(o[i][0], o[i][1]);
-        if ((lane & 3) == 0) mml[warp * ATT_R + g] = make_float2(m, l);
+        for (int i = 0; i < D / 8; i++) {
+            if (R == 16) {
+                *reinterpret_cast<float2 *>(mw + i * 8 + c2) = make_float2(o[i][0], o[i][1]);
+                *reinterpret_cast<float2 *>(mw + 8 * (D + 4) + i * 8 + c2) = make_float2(o[i][NO - 2], o[i][NO - 1]);
+            } else {
+                *reinterpret_cast<float2 *>(mw + i * 8 + c2) =
+                    DIRECT ? make_float2(o[i][0] + o[i][NO - 2], o[i][1] + o[i][NO - 1]) : make_float2(o[i][0], o[i][1]);
+            }
+        }
+        if ((lane & 3) == 0)
+#pragma unroll
+            for (int n = 0; n < NR; n++) mml[warp * R + g + 8 * n] = make_float2(m[n], l[n]);
         // the next part and its queries, on their way while the warps merge
         AttnPart next = p;
         bool go_on = false;
         if (!CLUSTER && p.f_end < f1) {
             next = attn_part(prefix, last, a.B, nvh, p.f_end, f1);
             go_on = next.t < next.end;
-            if (go_on) ask_queries(next);
+            if (AHEAD && go_on) ask_queries(next);
         }
         __syncthreads();
         const bool whole = !CLUSTER && p.t == 0 && p.end == p.nt;
@@ -538,13 +625,13 @@ __global__ void __launch_bounds__(AttnShape<D>::THREADS, AttnShape<D>::CTAS) att
             const int r = i / (D / 4), x = (i - r * (D / 4)) * 4;
             float mm = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < W; w++) mm = fmaxf(mm, mml[w * ATT_R + r].x);
+            for (int w = 0; w < W; w++) mm = fmaxf(mm, mml[w * R + r].x);
             const float ref = mm == -INFINITY ? 0.0f : mm;
             float ll = 0.0f;
             float4 acc = make_float4(0, 0, 0, 0);
 #pragma unroll
             for (int w = 0; w < W; w++) {
-                const float2 e = mml[w * ATT_R + r];
+                const float2 e = mml[w * R + r];
                 const float s = exp2_fast(e.x - ref);
                 const float4 y = *reinterpret_cast<const float4 *>(mo[w] + r * (D + 4) + x);
                 ll += s * e.y;
@@ -554,7 +641,7 @@ __global__ void __launch_bounds__(AttnShape<D>::THREADS, AttnShape<D>::CTAS) att
             if (CLUSTER) {  // in place of warp 0's sums, whose elements only this thread reads
                 *reinterpret_cast<float4 *>(mo[0] + r * (D + 4) + x) = acc;
                 if (x == 0)
-                    for (int c = 0; c < (int)cl.num_blocks(); c++) cl.map_shared_rank(&all_ml[0][0], c)[cl.block_rank() * ATT_R + r] = make_float2(mm, ll);
+                    for (int c = 0; c < (int)cl.num_blocks(); c++) cl.map_shared_rank(&all_ml[0][0], c)[cl.block_rank() * R + r] = make_float2(mm, ll);
             } else if (whole) {
                 // no entry attended to (all on bad pages): zeros
                 const float inv = ll > 0.0f || ll != ll ? 1.0f / (ll * PSCALE) : 0.0f;
@@ -564,8 +651,8 @@ __global__ void __launch_bounds__(AttnShape<D>::THREADS, AttnShape<D>::CTAS) att
                 if (x == 0) a.ml[(int64_t)p.b * a.H + head] = make_float2(mm, ll);
             } else {
                 const float u = 1.0f / PSCALE;
-                *reinterpret_cast<float4 *>(a.part_o + (slot_id * ATT_R + r) * D + x) = make_float4(acc.x * u, acc.y * u, acc.z * u, acc.w * u);
-                if (x == 0) a.part_ml[slot_id * ATT_R + r] = make_float2(mm, ll);
+                *reinterpret_cast<float4 *>(a.part_o + (slot_id * R + r) * D + x) = make_float4(acc.x * u, acc.y * u, acc.z * u, acc.w * u);
+                if (x == 0) a.part_ml[slot_id * R + r] = make_float2(mm, ll);
             }
         }
         if constexpr (CLUSTER) {
@@ -617,6 +704,7 @@ __global__ void __launch_bounds__(AttnShape<D>::THREADS, AttnShape<D>::CTAS) att
         npart++;
         __syncthreads();  // the slots may be filled again
         p = next;
+        if (!AHEAD) ask_queries(p);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
@@ -626,23 +714,36 @@ struct AttnVariant {
     AttnKernel run, cluster;
     int head, ctas, warps;  // shared memory without the per-sequence part, CTAs per SM, warps per CTA
 };
-// The instances for a head width: cache type bf16 or fp16, activations f32 or the cache's.
-AttnVariant attn_variant_64(bool bf16, bool f32);
-AttnVariant attn_variant_96(bool bf16, bool f32);
-AttnVariant attn_variant_128(bool bf16, bool f32);
-AttnVariant attn_variant_192(bool bf16, bool f32);
-AttnVariant attn_variant_256(bool bf16, bool f32);
+// Whether there are instances for 16 heads per pass: not where registers cannot
+// hold 16 f32 queries and sums.
+constexpr bool attn_wide_rows(int d, bool f32) { return !f32 || d <= 128; }
+// The instances for a head width: cache type bf16 or fp16, activations f32 or the
+// cache's, 8 or 16 query heads per pass.
+AttnVariant attn_variant_64(bool bf16, bool f32, int rows);
+AttnVariant attn_variant_96(bool bf16, bool f32, int rows);
+AttnVariant attn_variant_128(bool bf16, bool f32, int rows);
+AttnVariant attn_variant_192(bool bf16, bool f32, int rows);
+AttnVariant attn_variant_256(bool bf16, bool f32, int rows);
 
-template <int D, typename CT, typename IO> AttnVariant attn_instances() {
-    return {attn_split_kernel<D, CT, IO, false>, attn_split_kernel<D, CT, IO, true>, AttnShape<D>::smem(0), AttnShape<D>::CTAS, AttnShape<D>::W};
+template <int D, int R, typename CT, typename IO> AttnVariant attn_instance() {
+    if constexpr (R == 8 || attn_wide_rows(D, sizeof(IO) == 4)) {
+        using SH = AttnShape<D, AttnQuery<D, R, CT, IO>::QB>;
+        return {attn_split_kernel<D, R, CT, IO, false>, attn_split_kernel<D, R, CT, IO, true>, SH::smem(0), SH::CTAS, SH::W};
+    } else {
+        return {};
+    }
+}
+template <int D, typename CT, typename IO> AttnVariant attn_instances(int rows) {
+    return rows == 8 ? attn_instance<D, 8, CT, IO>() : attn_instance<D, 16, CT, IO>();
 }
 
 }  // namespace ofb
 
 #define OFB_ATTN_INSTANCES(D)                                                                                   \
     namespace ofb {                                                                                             \
-    AttnVariant attn_variant_##D(bool bf16, bool f32) {                                                         \
-        if (bf16) return f32 ? attn_instances<D, __nv_bfloat16, float>() : attn_instances<D, __nv_bfloat16, __nv_bfloat16>(); \
-        return f32 ? attn_instances<D, __half, float>() : attn_instances<D, __half, __half>();                  \
+    AttnVariant attn_variant_##D(bool bf16, bool f32, int rows) {                                               \
+        if (bf16)                                                                                               \
+            return f32 ? attn_instances<D, __nv_bfloat16, float>(rows) : attn_instances<D, __nv_bfloat16, __nv_bfloat16>(rows); \
+        return f32 ? attn_instances<D, __half, float>(rows) : attn_instances<D, __half, __half>(rows);          \
     }                                                                                                           \
     }
