@@ -25,16 +25,12 @@ namespace ofb {
 constexpr int RP_THREADS = 256;
 constexpr int RP_PAIRS = 128;
 constexpr int RP_TOKENS = 1 << 30;
-#ifndef V_RP
-#define V_RP 2
-#endif
-constexpr int RP_CTAS = V_RP;  // per SM
 
 struct RopeArgs {
     int T, H, KVH, d, rot, tpb;  // heads of q; kv heads (0: no cache); tokens of a group
-    int shared;                  // floats of RopeShared
+    int slots;                   // first kernel: rows under way, threads / per_row
     int n_pages, page_size, n_seqs, max_pages;
-    FastDiv page, rows;  // by page_size, by H + 2 KVH
+    FastDiv page, rows, per_row;  // by page_size, by H + 2 KVH, by chunk pairs of a row
     const void *q, *k, *v;
     void *q_out, *ck, *cv;
     int64_t qs, ks, vs, qos, page_stride, pos_stride;
@@ -48,9 +44,29 @@ struct RopeArgs {
 
 // Where a CTA's tokens go (a page below 0: nowhere) and their order numbers.
 struct RopeEntry {
-    int page, slot, number, asked;
+    int page, slot, number;
 };
-// Shared memory: cosines [tpb][rot/2], sines [tpb][rot/2], entries [tpb].
+// The place of token t's rows; reports what is wrong with it.
+__device__ __forceinline__ RopeEntry rope_entry(const RopeArgs &a, int t) {
+    const int b = a.seq[t], i = a.index[t];
+    RopeEntry e = {-1, 0, a.number ? a.number[t] : i};
+    if (b < 0) return e;
+    const int col = i < 0 ? 0 : a.page.div(i);
+    if (b >= a.n_seqs || i < 0 || col >= a.max_pages) {
+        report(a.errors, OFB_CACHE_EINDEX);
+        return e;
+    }
+    const int p = a.table[(int64_t)b * a.max_pages + col];
+    if (p < 0 || p >= a.n_pages) {
+        report(a.errors, OFB_CACHE_EPAGE);
+        return e;
+    }
+    e.page = p;
+    e.slot = i - col * a.page_size;
+    return e;
+}
+
+// Shared memory of the second kernel: cosines [tpb][rot/2], sines [tpb][rot/2], entries [tpb].
 struct RopeShared {
     float *c, *s;
     RopeEntry *entry;
@@ -73,29 +89,14 @@ __device__ __forceinline__ void rope_setup(const RopeArgs &a, int t0, int nt, co
         sh.c[i] = c;
         sh.s[i] = s;
     }
-    if (a.KVH && threadIdx.x < nt) {
-        const int t = t0 + threadIdx.x, b = a.seq[t], i = a.index[t];
-        RopeEntry e = {-1, 0, 0, 0};
-        if (b >= 0) {
-            const int col = i < 0 ? 0 : a.page.div(i);
-            if (b >= a.n_seqs || i < 0 || col >= a.max_pages) {
-                report(a.errors, OFB_CACHE_EINDEX);
-            } else {
-                const int p = a.table[(int64_t)b * a.max_pages + col];
-                if (p < 0 || p >= a.n_pages) report(a.errors, OFB_CACHE_EPAGE);
-                else e = {p, i - col * a.page_size, a.number ? a.number[t] : i, 0};
-            }
-        }
-        sh.entry[threadIdx.x] = e;
-    }
+    if (a.KVH && threadIdx.x < nt) sh.entry[threadIdx.x] = rope_entry(a, t0 + threadIdx.x);
     __syncthreads();
 }
 
 // Weight 0 and the order number of the CTA's new entries.
 __device__ __forceinline__ void rope_meta(const RopeArgs &a, int nt, const RopeEntry *entry) {
     if (!a.weight && !a.order) return;
-    // from the last thread down: the first ones look pages up
-    for (int i = RP_THREADS - 1 - threadIdx.x; i < nt * a.KVH; i += RP_THREADS) {
+    for (int i = threadIdx.x; i < nt * a.KVH; i += RP_THREADS) {
         const int t = i / a.KVH, h = i - t * a.KVH;
         const RopeEntry e = entry[t];
         if (e.page < 0) continue;
@@ -137,21 +138,24 @@ template <typename IO> struct RopeRaw {
     }
 };
 
-// CTAs go round over the groups of tpb tokens. Thread (slot, j) takes chunk
-// pair j of rows slot, slot + slots, ... of a group in batches; as soon as an
-// item is unpacked the same item of the next batch (or of the next group's
-// first) is asked for, so that loads never run dry. A group's cosines are formed
-// from positions that were asked for a group earlier (and page numbers, from
-// places asked for two groups earlier), into the half of the shared memory that
-// the group before does not read: one barrier per group.
-template <typename IO, typename CT, bool ADJ>
-__global__ void __launch_bounds__(RP_THREADS, RP_CTAS) rope_vec_kernel(const __grid_constant__ RopeArgs a) {
-    constexpr int BATCH = sizeof(IO) == 2 ? 4 : 2;
-    extern __shared__ __align__(16) float rope_smem[];
-    const int half = a.rot / 2, tid = threadIdx.x;
-    pdl_wait();
-    pdl_trigger();
-    const int per_row = a.d / 16, slots = RP_THREADS / per_row, slot = tid / per_row, j = tid - slot * per_row;
+// A CTA has tpb tokens (most often one). Thread (slot, j) takes chunk pair j of rows
+// slot, slot + slots, ...: it asks for its first three (f32: two) items at once;
+// while they are on their way the last threads find the tokens' places in the cache
+// and the first ones form the cosines, so that the three waits are one. Measured on
+// 8190 tokens with 32 + 2 x 8 heads of 128, bf16: 39.5 us, 5.1 TB/s, where adding a
+// number to as many bytes takes 32 (16383 tokens x 16 heads alone: 24.4 and 21.7).
+// 8 CTAs per SM 39.8, 6 41.2, 4 items at once 43, 2 x 192 threads 42, 3 x 256 41;
+// CTAs that stay and ask for the next group's loads, positions and pages ahead 45.
+constexpr int RV_THREADS = 128, RV_CTAS = 7;  // CTAs per SM that registers allow
+template <typename IO> constexpr int RV_BATCH = sizeof(IO) == 2 ? 3 : 2;  // items asked for at once
+template <typename IO, typename CT, bool ADJ, bool CACHE>
+__global__ void __launch_bounds__(RV_THREADS, RV_CTAS) rope_vec_kernel(const __grid_constant__ RopeArgs a) {
+    constexpr int BATCH = RV_BATCH<IO>;
+    extern __shared__ __align__(16) float rope_smem[];  // cosines, sines [tpb][rot/2], places [tpb]
+    const int half = a.rot / 2, tid = threadIdx.x, t0 = blockIdx.x * a.tpb, nt = min(a.tpb, a.T - t0);
+    float *const cosines = rope_smem, *const sines = rope_smem + a.tpb * half;
+    RopeEntry *const entry = reinterpret_cast<RopeEntry *>(rope_smem + a.tpb * a.rot);
+    const int slot = a.per_row.div(tid), j = tid - slot * (int)a.per_row.d, total = slot < a.slots ? nt * (int)a.rows.d : 0;
     // The thread's two chunks of 8 elements and where their cosines are. HALVES:
     // the two halves of 8 pairs, or two chunks behind rot; ADJACENT: 4 pairs
     // each, half a row apart. Neighbouring threads have neighbouring chunks.
@@ -165,154 +169,86 @@ __global__ void __launch_bounds__(RP_THREADS, RP_CTAS) rope_vec_kernel(const __g
         turn_a = turn_b = j < pr;
         ta = turn_a ? 8 * j : a.rot + 8 * (j - pr), tb = ta + (turn_a ? half : rest);
     }
-    const int dt = slots / (int)a.rows.d, drow = slots - dt * (int)a.rows.d;  // from one item's row to the next's
-    // the (token, pair)s whose cosines this thread forms: tpb * rot/2 <= 2 RP_THREADS
-    const int n_cs = a.tpb * half;
-    int ct[2] = {0, 0};
-    int64_t cpos[2] = {0, 0};
-    double cf[2] = {0.0, 0.0};
+    pdl_wait();
+    pdl_trigger();
+    RopeRaw<IO> raw[BATCH];
+    auto fetch = [&](int vr) {
+#pragma unroll
+        for (int k = 0; k < BATCH; k++)
+            if (vr + k * a.slots < total) {
+                const RopeRow r = rope_row(a, vr + k * a.slots);
+                if constexpr (CACHE) raw[k].load(rope_src<IO>(a, r, t0), ta, tb);
+                else raw[k].load(static_cast<const IO *>(a.q) + (t0 + r.t) * a.qs + (int64_t)r.row * a.d, ta, tb);
+            }
+    };
+    fetch(slot);
+    // (by the last threads: the first ones have the cosines)
+    if (CACHE && RV_THREADS - 1 - tid < nt) entry[RV_THREADS - 1 - tid] = rope_entry(a, t0 + RV_THREADS - 1 - tid);
     {
         const double *freq = a.half_turns;  // see rope_setup
         const uint8_t *axis = a.axis;
         asm("" : "+l"(freq), "+l"(axis));
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const int i = tid + k * RP_THREADS;
-            if (i < n_cs) {
-                ct[k] = i / half;
-                const int p = i - ct[k] * half;
-                cpos[k] = axis[p] * a.pos_stride + ct[k];
-                cf[k] = freq[p];
-            }
-        }
-    }
-    int pos[2] = {0, 0}, seq = -1, index = 0, number = 0;
-    auto ask_pos = [&](int t0) {
-#pragma unroll
-        for (int k = 0; k < 2; k++)
-            if (tid + k * RP_THREADS < n_cs && t0 + ct[k] < a.T) pos[k] = a.pos[cpos[k] + t0];
-    };
-    auto ask_place = [&](int t0) {
-        seq = -1;
-        if (a.KVH && tid < a.tpb && t0 + tid < a.T) {
-            seq = a.seq[t0 + tid], index = a.index[t0 + tid];
-            if (a.number) number = a.number[t0 + tid];
-        }
-    };
-    RopeEntry at = {-1, 0, 0, 0};
-    auto ask_page = [&]() {  // uses seq, index and number
-        at.page = -1;
-        if (seq < 0) return;
-        const int col = index < 0 ? 0 : a.page.div(index);
-        if (seq >= a.n_seqs || index < 0 || col >= a.max_pages) {
-            report(a.errors, OFB_CACHE_EINDEX);
-        } else {
-            at = {a.table[(int64_t)seq * a.max_pages + col], index - col * a.page_size, a.number ? number : index, 1};
-        }
-    };
-    const int step = gridDim.x * a.tpb;
-    int t0 = blockIdx.x * a.tpb, half_at = 0;
-    ask_pos(t0);
-    ask_place(t0);
-    ask_page();
-    ask_place(t0 + step);
-    RopeRaw<IO> raw[BATCH];
-    auto rows_of = [&](int t) { return slot < slots && t < a.T ? min(a.tpb, a.T - t) * (int)a.rows.d : 0; };
-    auto advance = [&](RopeRow &r) {
-        r.t += dt, r.row += drow;
-        if (r.row >= (int)a.rows.d) r.row -= (int)a.rows.d, r.t++;
-    };
-    RopeRow ask, now;  // the row asked for next, the row worked on
-    int total = rows_of(t0);
-    now = ask = rope_row(a, slot);
-#pragma unroll
-    for (int k = 0; k < BATCH; k++) {
-        if (slot + k * slots < total) raw[k].load(rope_src<IO>(a, ask, t0), ta, tb);
-        advance(ask);
-    }
-    for (; t0 < a.T; t0 += step, half_at ^= 1) {
-        const int nt = min(a.tpb, a.T - t0), total_next = rows_of(t0 + step);
-        const RopeShared sh(a, rope_smem + half_at * a.shared);
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            const int i = tid + k * RP_THREADS;
-            if (i >= n_cs) break;
-            const double h = (double)pos[k] * cf[k];
+        for (int i = tid; i < nt * half; i += RV_THREADS) {
+            const int t = a.tpb == 1 ? 0 : i / half, p = i - t * half;
+            const double h = (double)a.pos[axis[p] * a.pos_stride + t0 + t] * freq[p];
             float s, c;
             sincospif((float)(h - 2.0 * rint(0.5 * h)), &s, &c);
-            sh.c[i] = c;
-            sh.s[i] = s;
+            cosines[i] = c;
+            sines[i] = s;
         }
-        if (tid < nt) {
-            if (at.asked && (at.page < 0 || at.page >= a.n_pages)) {
-                report(a.errors, OFB_CACHE_EPAGE);
-                at.page = -1;
-            }
-            sh.entry[tid] = at;
-            at.asked = 0;
-        }
-        __syncthreads();
-        ask_pos(t0 + step);
-        ask_page();
-        ask_place(t0 + 2 * step);
-        for (int vr = slot; vr < total; vr += BATCH * slots) {
-            // the batch after this one: of this group, or the next group's first
-            const bool here = vr + BATCH * slots < total;
-            const int t_next = here ? t0 : t0 + step, n_next = here ? total : total_next;
-            int v_next = here ? vr + BATCH * slots : slot;
-            if (!here) ask = rope_row(a, slot);
+    }
+    __syncthreads();
+    for (int vr = slot; vr < total; vr += BATCH * a.slots) {
+        if (vr > slot) fetch(vr);
 #pragma unroll
-            for (int k = 0; k < BATCH; k++, v_next += slots) {
-                float x[8], y[8];
-                load8(reinterpret_cast<const IO *>(raw[k].x), x);
-                load8(reinterpret_cast<const IO *>(raw[k].y), y);
-                if (v_next < n_next) raw[k].load(rope_src<IO>(a, ask, t_next), ta, tb);
-                advance(ask);
-                const RopeRow r = now;
-                advance(now);
-                if (vr + k * slots >= total) continue;
-                const bool is_q = r.row < a.H, is_v = r.row >= a.H + a.KVH;
-                const float *cs = sh.c + r.t * half, *sn = sh.s + r.t * half;
-                if (ADJ) {
-                    auto turn4 = [&](float(&z)[8], int at) {
-                        const float4 c = *reinterpret_cast<const float4 *>(cs + at), s = *reinterpret_cast<const float4 *>(sn + at);
-                        const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
+        for (int k = 0; k < BATCH; k++) {
+            if (vr + k * a.slots >= total) break;
+            const RopeRow r = rope_row(a, vr + k * a.slots);
+            const bool is_q = !CACHE || r.row < a.H, is_v = CACHE && r.row >= a.H + a.KVH;
+            float x[8], y[8];
+            load8(reinterpret_cast<const IO *>(raw[k].x), x);
+            load8(reinterpret_cast<const IO *>(raw[k].y), y);
+            const float *cs = cosines + r.t * half, *sn = sines + r.t * half;
+            if (ADJ) {
+                auto turn4 = [&](float(&z)[8], int at) {
+                    const float4 c = *reinterpret_cast<const float4 *>(cs + at), s = *reinterpret_cast<const float4 *>(sn + at);
+                    const float cc[4] = {c.x, c.y, c.z, c.w}, ss[4] = {s.x, s.y, s.z, s.w};
 #pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const float u = z[2 * i], v = z[2 * i + 1];
-                            z[2 * i] = u * cc[i] - v * ss[i];
-                            z[2 * i + 1] = v * cc[i] + u * ss[i];
-                        }
-                    };
-                    if (turn_a && !is_v) turn4(x, ta / 2);
-                    if (turn_b && !is_v) turn4(y, tb / 2);
-                } else if (turn_a && !is_v) {
-                    float c[8], s[8];
-                    load8(cs + 8 * j, c);
-                    load8(sn + 8 * j, s);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        const float u = x[i], v = y[i];
-                        x[i] = u * c[i] - v * s[i];
-                        y[i] = v * c[i] + u * s[i];
+                    for (int i = 0; i < 4; i++) {
+                        const float u = z[2 * i], v = z[2 * i + 1];
+                        z[2 * i] = u * cc[i] - v * ss[i];
+                        z[2 * i + 1] = v * cc[i] + u * ss[i];
                     }
+                };
+                if (turn_a && !is_v) turn4(x, ta / 2);
+                if (turn_b && !is_v) turn4(y, tb / 2);
+            } else if (turn_a && !is_v) {
+                float c[8], s[8];
+                load8(cs + 8 * j, c);
+                load8(sn + 8 * j, s);
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float u = x[i], v = y[i];
+                    x[i] = u * c[i] - v * s[i];
+                    y[i] = v * c[i] + u * s[i];
                 }
-                if (is_q) {
-                    IO *dst = static_cast<IO *>(a.q_out) + (t0 + r.t) * a.qos + (int64_t)r.row * a.d;
-                    store8(dst + ta, x);
-                    store8(dst + tb, y);
-                } else {
-                    const RopeEntry e = sh.entry[r.t];
-                    if (e.page < 0) continue;
-                    CT *dst = static_cast<CT *>(is_v ? a.cv : a.ck) + rope_cache_at(a, e, r.row - a.H - (is_v ? a.KVH : 0));
-                    store8(dst + ta, x);
-                    store8(dst + tb, y);
+            }
+            if (is_q) {
+                IO *dst = static_cast<IO *>(a.q_out) + (t0 + r.t) * a.qos + (int64_t)r.row * a.d;
+                store8(dst + ta, x);
+                store8(dst + tb, y);
+            } else if (const RopeEntry e = entry[r.t]; e.page >= 0) {
+                const int h = r.row - a.H - (is_v ? a.KVH : 0);
+                CT *dst = static_cast<CT *>(is_v ? a.cv : a.ck) + rope_cache_at(a, e, h);
+                store8(dst + ta, x);
+                store8(dst + tb, y);
+                if (!is_v && j == 0) {  // with its key row: weight 0 and the order number
+                    const int64_t m = ((int64_t)e.page * a.KVH + h) * a.page_size + e.slot;
+                    if (a.weight) a.weight[m] = 0.0f;
+                    if (a.order) a.order[m] = e.number;
                 }
             }
         }
-        now = rope_row(a, slot);
-        rope_meta(a, nt, sh.entry);
-        total = total_next;
     }
 }
 
@@ -403,24 +339,27 @@ static int rope_tables(const ofb_rope_config *r, int head_dim, const char *who, 
 }
 
 template <typename IO, typename CT> static cudaError_t rope_launch(RopeArgs &a, bool vec, bool adjacent, cudaStream_t s) {
-    const int rows = a.H + 2 * a.KVH;
+    const int rows = a.H + 2 * a.KVH, threads = vec ? RV_THREADS : RP_THREADS;
     const int64_t per_tok = (int64_t)rows * (vec ? a.d / 16 : a.d - a.rot / 2);
     // one batch of items per thread where a token alone does not give them, at
     // most 8 tokens (2 KB of cosines and sines each), and two CTAs per SM first
-    int tpb = (int)((sizeof(IO) == 2 ? 4 : 2) * RP_THREADS / per_tok);
+    int tpb = (int)(RV_BATCH<IO> * threads / per_tok);
     tpb = tpb < 1 ? 1 : tpb > 8 ? 8 : tpb;
-    while (tpb > 1 && tpb * (a.rot / 2) > 2 * RP_THREADS) tpb--;
     while (tpb > 1 && (a.T + tpb - 1) / tpb < 2 * sm_count()) tpb--;
     a.tpb = tpb;
     a.rows = fast_div(rows);
     a.page = fast_div(a.page_size ? a.page_size : 1);
-    a.shared = (tpb * a.rot + 3) / 4 * 4 + tpb * (int)(sizeof(RopeEntry) / sizeof(float));
-    const size_t smem = (size_t)(vec ? 2 : 1) * a.shared * sizeof(float);
-    const int groups = (a.T + tpb - 1) / tpb, most = RP_CTAS * sm_count();
-    const dim3 grid(vec && groups > most ? most : groups), block(RP_THREADS);
+    a.per_row = fast_div(vec ? a.d / 16 : 1);
+    a.slots = RV_THREADS / (int)a.per_row.d;
+    // (a.rot is a multiple of 4 for the first kernel)
+    const size_t smem = ((size_t)tpb * a.rot + 3) / 4 * 16 + tpb * sizeof(RopeEntry);
+    const dim3 grid((a.T + tpb - 1) / tpb), block(threads);
     if (!vec) return launch_pdl(rope_any_kernel<IO, CT>, grid, block, smem, s, a, (int)adjacent);
-    return adjacent ? launch_pdl(rope_vec_kernel<IO, CT, true>, grid, block, smem, s, a)
-                    : launch_pdl(rope_vec_kernel<IO, CT, false>, grid, block, smem, s, a);
+    if (!a.KVH)
+        return adjacent ? launch_pdl(rope_vec_kernel<IO, IO, true, false>, grid, block, smem, s, a)
+                        : launch_pdl(rope_vec_kernel<IO, IO, false, false>, grid, block, smem, s, a);
+    return adjacent ? launch_pdl(rope_vec_kernel<IO, CT, true, true>, grid, block, smem, s, a)
+                    : launch_pdl(rope_vec_kernel<IO, CT, false, true>, grid, block, smem, s, a);
 }
 
 static bool row_ok(const void *p, int64_t stride) { return !misaligned(p, 16) && stride % 8 == 0; }

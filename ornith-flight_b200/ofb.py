@@ -251,20 +251,26 @@ def _rows(t: torch.Tensor, shape, dtype, device, name: str) -> int:
     """Elements from one row of t [rows, heads, head_dim] to the next; heads dense."""
     if t.shape != shape or t.dtype != dtype or t.device != device:
         raise OfbError(EINVAL, f"{name} must be {dtype} {tuple(shape)} on {device}")
-    st = t.stride()
-    if (st[2] != 1 and shape[2] > 1) or (st[1] != shape[2] and shape[1] > 1):
+    row, head, one = t.stride()
+    if (one != 1 and shape[2] > 1) or (head != shape[2] and shape[1] > 1):
         raise OfbError(EINVAL, f"{name}: the heads of a row must be consecutive")
-    return st[0]
+    return row
 
 
-def _on(device: torch.device, stream, body):
-    """body() with `device` and `stream` current."""
+_get_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+
+
+def _elsewhere(device: torch.device, stream, call, *args, **kw):
+    """call(...) with `device` and `stream` current."""
     if device.type != "cuda":
         raise OfbError(EINVAL, "tensors must be on a CUDA device")
-    if stream is None and device.index == torch.cuda.current_device():
-        return body(torch.cuda.current_stream().cuda_stream)
     with torch.cuda.device(device), torch.cuda.stream(stream):
-        return body(torch.cuda.current_stream().cuda_stream)
+        return call(*args, **kw)
+
+
+def _away(device: torch.device, stream) -> bool:
+    """Whether a call has to change the current device or stream first."""
+    return stream is not None or device.type != "cuda" or device.index != _get_device()
 
 
 class KvCache:
@@ -309,18 +315,19 @@ class KvCache:
 def rope(x: torch.Tensor, pos: torch.Tensor, cfg: RopeConfig, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
     """x [tokens, heads, head_dim] (f32, bf16 or fp16) turned by its tokens'
     positions pos int32 [axes, tokens] (ofb_rope); out may be x."""
-    _need(x.dim() == 3 and x.dtype in _TYPE_OF, "rope: x must be f32, bf16 or fp16 [tokens, heads, head_dim]")
-    T, H, d = shape = x.shape
-    xs = _rows(x, shape, x.dtype, x.device, "rope: x")
-    p = _ints(pos, (cfg.n_axes, T), x.device, "rope: pos")
-
-    def body(s):
-        y = torch.empty(shape, dtype=x.dtype, device=x.device) if out is None else out
-        ys = _rows(y, shape, x.dtype, x.device, "rope: out")
-        _check(lib.ofb_rope(ctypes.byref(cfg), x.data_ptr(), _TYPE_OF[x.dtype], T, H, d, xs, p, T, y.data_ptr(), ys, s))
-        return y
-
-    return _on(x.device, stream, body)
+    dev, dt, shape = x.device, x.dtype, x.shape
+    _need(x.dim() == 3 and dt in _TYPE_OF, "rope: x must be f32, bf16 or fp16 [tokens, heads, head_dim]")
+    T, H, d = shape
+    xs = _rows(x, shape, dt, dev, "rope: x")
+    p = _ints(pos, (cfg.n_axes, T), dev, "rope: pos")
+    if _away(dev, stream):
+        return _elsewhere(dev, stream, rope, x, pos, cfg, out)
+    if out is None:
+        out = torch.empty_like(x)
+    os_ = _rows(out, shape, dt, dev, "rope: out")
+    _check(lib.ofb_rope(ctypes.byref(cfg), x.data_ptr(), _TYPE_OF[dt], T, H, d, xs, p, T, out.data_ptr(), os_,
+                        _raw_stream(dev.index)))
+    return out
 
 
 def rope_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, seq: torch.Tensor, index: torch.Tensor,
@@ -333,29 +340,30 @@ def rope_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, seq: torch.Ten
     head_dim] (in q_out, which may be q), None without q."""
     _need(k.dim() == 3, "rope_append: k must be [tokens, kv heads, head_dim]")
     T, d, dev, dt = k.shape[0], cache.head_dim, cache.device, k.dtype
-    _need(dt in (torch.float32, cache.dtype), "rope_append: k, v and q must be f32 or of the cache's type")
+    _need(dt is torch.float32 or dt is cache.dtype, "rope_append: k, v and q must be f32 or of the cache's type")
     shape = (T, cache.n_kv_heads, d)
     ks, vs = _rows(k, shape, dt, dev, "rope_append: k"), _rows(v, shape, dt, dev, "rope_append: v")
     _need((rope is None) == (pos is None), "rope_append: rope and pos go together")
     pp = None if rope is None else _ints(pos, (rope.n_axes, T), dev, "rope_append: pos")
     sp, ip = _ints(seq, (T,), dev, "rope_append: seq"), _ints(index, (T,), dev, "rope_append: index")
     np_ = None if number is None else _ints(number, (T,), dev, "rope_append: number")
-    H = qs = 0
+    H = qs = os_ = 0
     if q is not None:
         _need(q.dim() == 3, "rope_append: q must be [tokens, heads, head_dim]")
         H = q.shape[1]
         qs = _rows(q, (T, H, d), dt, dev, "rope_append: q")
-
-    def body(s):
-        y, ys = None, 0
-        if q is not None:
-            y = torch.empty((T, H, d), dtype=dt, device=dev) if q_out is None else q_out
-            ys = _rows(y, (T, H, d), dt, dev, "rope_append: q_out")
-        _check(lib.ofb_rope_append(cache._ref, None if rope is None else ctypes.byref(rope), _TYPE_OF[dt], T, H, _ptr(q), qs,
-                                   k.data_ptr(), ks, v.data_ptr(), vs, pp, T, sp, ip, np_, _ptr(y), ys, s))
-        return y
-
-    return _on(dev, stream, body)
+    if _away(dev, stream):
+        return _elsewhere(dev, stream, rope_append, cache, k, v, seq, index, number, q, pos, rope, q_out)
+    if q is None:
+        q_out = None
+    else:
+        if q_out is None:
+            q_out = torch.empty((T, H, d), dtype=dt, device=dev)
+        os_ = _rows(q_out, (T, H, d), dt, dev, "rope_append: q_out")
+    _check(lib.ofb_rope_append(cache._ref, None if rope is None else ctypes.byref(rope), _TYPE_OF[dt], T, H, _ptr(q), qs,
+                               k.data_ptr(), ks, v.data_ptr(), vs, pp, T, sp, ip, np_, _ptr(q_out), os_,
+                               _raw_stream(dev.index)))
+    return q_out
 
 
 def _scratch(size: int, device) -> torch.Tensor:
@@ -366,8 +374,9 @@ def _scratch(size: int, device) -> torch.Tensor:
 
 def attn_scratch(cache: KvCache, n_heads: int, n_seqs: int, max_len: int = 0, accumulate: bool = False) -> torch.Tensor:
     """Scratch for attn_decode calls of up to these sizes that do not overlap."""
-    with torch.cuda.device(cache.device):
-        return _scratch(lib.ofb_attn_scratch_size(cache._ref, n_heads, n_seqs, max_len, int(accumulate)), cache.device)
+    if _away(cache.device, None):
+        return _elsewhere(cache.device, None, attn_scratch, cache, n_heads, n_seqs, max_len, accumulate)
+    return _scratch(lib.ofb_attn_scratch_size(cache._ref, n_heads, n_seqs, max_len, int(accumulate)), cache.device)
 
 
 def attn_decode(cache: KvCache, q: torch.Tensor, lens: torch.Tensor, scale: float | None = None, max_len: int = 0,
@@ -378,23 +387,24 @@ def attn_decode(cache: KvCache, q: torch.Tensor, lens: torch.Tensor, scale: floa
     (ofb_attn_decode). scale: 1/sqrt(head_dim) by default; max_len: a bound on
     lens (0: the page table's reach); accumulate: add the weights to cache.weight."""
     _need(q.dim() == 3, "attn_decode: q must be [sequences, heads, head_dim]")
-    dev, d = cache.device, cache.head_dim
+    dev, d, dt = cache.device, cache.head_dim, q.dtype
     B, H = q.shape[0], q.shape[1]
     shape = (B, H, d)
-    _need(q.dtype in (torch.float32, cache.dtype), "attn_decode: q must be f32 or of the cache's type")
-    qs, lp = _rows(q, shape, q.dtype, dev, "attn_decode: q"), _ints(lens, (B,), dev, "attn_decode: lens")
-
-    def body(s):
-        w = attn_scratch(cache, H, B, max_len, accumulate) if scratch is None else scratch
-        _need(w.device == dev and w.is_contiguous(), "attn_decode: scratch must be contiguous beside the cache")
-        y = torch.empty(shape, dtype=q.dtype, device=dev) if out is None else out
-        ys = _rows(y, shape, q.dtype, dev, "attn_decode: out")
-        _check(lib.ofb_attn_decode(cache._ref, q.data_ptr(), _TYPE_OF[q.dtype], qs, H, d ** -0.5 if scale is None else scale,
-                                   lp, B, max_len, int(accumulate), y.data_ptr(), ys, w.data_ptr(),
-                                   w.numel() * w.element_size(), s))
-        return y
-
-    return _on(dev, stream, body)
+    _need(dt is torch.float32 or dt is cache.dtype, "attn_decode: q must be f32 or of the cache's type")
+    qs, lp = _rows(q, shape, dt, dev, "attn_decode: q"), _ints(lens, (B,), dev, "attn_decode: lens")
+    if _away(dev, stream):
+        return _elsewhere(dev, stream, attn_decode, cache, q, lens, scale, max_len, accumulate, out, scratch)
+    if scratch is None:
+        scratch = attn_scratch(cache, H, B, max_len, accumulate)
+    elif scratch.device != dev or not scratch.is_contiguous():
+        raise OfbError(EINVAL, "attn_decode: scratch must be contiguous beside the cache")
+    if out is None:
+        out = torch.empty(shape, dtype=dt, device=dev)
+    os_ = _rows(out, shape, dt, dev, "attn_decode: out")
+    _check(lib.ofb_attn_decode(cache._ref, q.data_ptr(), _TYPE_OF[dt], qs, H, d ** -0.5 if scale is None else scale, lp, B,
+                               max_len, int(accumulate), out.data_ptr(), os_, scratch.data_ptr(), scratch.nbytes,
+                               _raw_stream(dev.index)))
+    return out
 
 
 def evict_scratch(cache: KvCache, n_seqs: int, keep: int) -> torch.Tensor:
@@ -413,18 +423,21 @@ def kv_evict(cache: KvCache, lens: torch.Tensor, keep: int, recent: int = 0, max
     _need(lens.dim() == 1, "kv_evict: lens must be [sequences]")
     B = lens.shape[0]
     lp = _ints(lens, (B,), dev, "kv_evict: lens")
-
-    def body(s):
-        w = evict_scratch(cache, B, keep) if scratch is None else scratch
-        _need(w.device == dev and w.is_contiguous(), "kv_evict: scratch must be contiguous beside the cache")
-        shape = (B, cache.n_kv_heads, keep)
-        src = torch.empty(shape, dtype=torch.int32, device=dev) if kept is None else kept
-        new = torch.empty(B, dtype=torch.int32, device=dev) if lens_out is None else lens_out
-        _check(lib.ofb_kv_evict(cache._ref, lp, B, max_len, keep, recent, _ints(new, (B,), dev, "kv_evict: lens_out"),
-                                _ints(src, shape, dev, "kv_evict: kept"), w.data_ptr(), w.numel() * w.element_size(), s))
-        return src, new
-
-    return _on(dev, stream, body)
+    if _away(dev, stream):
+        return _elsewhere(dev, stream, kv_evict, cache, lens, keep, recent, max_len, kept, lens_out, scratch)
+    if scratch is None:
+        scratch = evict_scratch(cache, B, keep)
+    elif scratch.device != dev or not scratch.is_contiguous():
+        raise OfbError(EINVAL, "kv_evict: scratch must be contiguous beside the cache")
+    shape = (B, cache.n_kv_heads, keep)
+    if kept is None:
+        kept = torch.empty(shape, dtype=torch.int32, device=dev)
+    if lens_out is None:
+        lens_out = torch.empty_like(lens)
+    _check(lib.ofb_kv_evict(cache._ref, lp, B, max_len, keep, recent, _ints(lens_out, (B,), dev, "kv_evict: lens_out"),
+                            _ints(kept, shape, dev, "kv_evict: kept"), scratch.data_ptr(), scratch.nbytes,
+                            _raw_stream(dev.index)))
+    return kept, lens_out
 
 
 # ---- synthetic inputs ---------------------------------------------------------
