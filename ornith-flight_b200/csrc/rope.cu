@@ -381,7 +381,7 @@ extern "C" int ofb_rope(const ofb_rope_config *rope, const void *x, int type, in
         return OFB_EUNSUPPORTED;
     }
     const int64_t width = (int64_t)n_heads * head_dim;
-    if ((n_tokens > 1 && (x_stride < width || out_stride < width || (rope->n_axes > 1 && pos_stride < n_tokens))) ||
+    if ((n_tokens > 1 && (x_stride < width || out_stride < width)) || (rope->n_axes > 1 && pos_stride < n_tokens) ||
         (x == out && n_tokens > 1 && x_stride != out_stride) || misaligned(x, type_size(type)) ||
         misaligned(out, type_size(type)) || misaligned(pos, 4)) {
         set_error("ofb_rope: strides or alignment (x %lld, out %lld, pos %lld)", (long long)x_stride, (long long)out_stride,
@@ -423,8 +423,8 @@ extern "C" int ofb_rope_append(const ofb_kv_cache *cache, const ofb_rope_config 
     const int d = cache->head_dim;
     const int64_t qw = (int64_t)n_heads * d, kw = (int64_t)cache->n_kv_heads * d;
     const size_t ts = type_size(type);
-    if ((n_tokens > 1 && ((q && (q_stride < qw || q_out_stride < qw)) || k_stride < kw || v_stride < kw ||
-                          (rope && rope->n_axes > 1 && pos_stride < n_tokens))) ||
+    if ((n_tokens > 1 && ((q && (q_stride < qw || q_out_stride < qw)) || k_stride < kw || v_stride < kw)) ||
+        (rope && rope->n_axes > 1 && pos_stride < n_tokens) ||
         (q && q == q_out && n_tokens > 1 && q_stride != q_out_stride) || misaligned(q, ts) || misaligned(q_out, ts) ||
         misaligned(k, ts) || misaligned(v, ts) || misaligned(pos, 4) || misaligned(seq, 4) || misaligned(index, 4) ||
         misaligned(number, 4)) {

@@ -290,7 +290,7 @@ class KvCache:
         _need(k.numel() > 0, "KvCache: empty k")
         for t in (k, v):
             _need(t[0].is_contiguous(), "KvCache: a page must be dense")
-        _need(n == 1 or k.stride(0) == v.stride(0), "KvCache: the pages of k and v must lie alike")
+        _need(n == 1 or k.stride(0) == v.stride(0) >= h * p * d, "KvCache: the pages of k and v must lie alike, and apart")
         _need(page_table.dim() == 2 and page_table.numel() > 0, "KvCache: page_table must be [sequences, pages]")
         self.device = k.device
         table = _ints(page_table, page_table.shape, k.device, "KvCache: page_table")

@@ -72,7 +72,7 @@ def test_rope_config_axes(ofb):
 @pytest.mark.parametrize("kw,want", [
     (dict(x=None), 1), (dict(pos=None), 1), (dict(out=None), 1), (dict(T=-1), 1), (dict(H=0), 1), (dict(d=0), 1), (dict(d=2048), 1),
     (dict(type=12), 4), (dict(xs=511), 1), (dict(os=100), 1), (dict(ps=4), 1), (dict(out=P, os=1024), 1), (dict(x=P + 2), 1),
-    (dict(pos=P + 1), 1), (dict(xs=-512), 1)], ids=str)
+    (dict(pos=P + 1), 1), (dict(xs=-512), 1), (dict(T=1, ps=0), 1), (dict(T=1, ps=-3), 1), (dict(T=(1 << 30) + 1, ps=1 << 40), 5)], ids=str)
 def test_rope_refused(ofb, kw, want):
     refused(ofb, call_rope(ofb, **kw), want)
 
@@ -97,7 +97,8 @@ def test_cache_refused(ofb, kw, want):
 @pytest.mark.parametrize("kw,want", [
     (dict(type=1), 4), (dict(type=14), 4), (dict(T=-1), 1), (dict(H=-1), 1), (dict(H=0), 1), (dict(k=None), 1), (dict(v=None), 1),
     (dict(seq=None), 1), (dict(index=None), 1), (dict(pos=None), 1), (dict(qo=None), 1), (dict(qs=511), 1), (dict(ks=255), 1),
-    (dict(vs=0), 1), (dict(qos=1), 1), (dict(ps=3), 1), (dict(qo=P, qos=1024), 1), (dict(k=P + 1), 1), (dict(seq=P + 2), 1)], ids=str)
+    (dict(vs=0), 1), (dict(qos=1), 1), (dict(ps=3), 1), (dict(qo=P, qos=1024), 1), (dict(k=P + 1), 1), (dict(seq=P + 2), 1),
+    (dict(T=1, ps=-1), 1), (dict(T=(1 << 30) + 1, ps=1 << 40), 5)], ids=str)
 def test_append_refused(ofb, kw, want):
     refused(ofb, call_append(ofb, **kw), want)
 
@@ -150,6 +151,8 @@ def test_binding_refuses_host_tensors_and_wrong_shapes(ofb):
     for bad in (lambda: ofb.KvCache(z(3, 2, 16, 64), z(3, 2, 16, 32), z(1, 2, dt=i32)),
                 lambda: ofb.KvCache(z(3, 2, 16, 64, dt=torch.float32), z(3, 2, 16, 64, dt=torch.float32), z(1, 2, dt=i32)),
                 lambda: ofb.KvCache(z(3, 2, 64, 16).transpose(2, 3), z(3, 2, 64, 16).transpose(2, 3), z(1, 2, dt=i32)),
+                lambda: ofb.KvCache(z(1, 2, 16, 64).expand(3, -1, -1, -1), z(1, 2, 16, 64).expand(3, -1, -1, -1), z(1, 2, dt=i32)),
+                lambda: ofb.KvCache(z(3, 2, 16, 64), z(3, 4, 16, 64)[:, :2], z(1, 2, dt=i32)),
                 lambda: ofb.KvCache(z(3, 2, 16, 64), z(3, 2, 16, 64), z(1, 2, dt=torch.int64)),
                 lambda: ofb.KvCache(z(3, 2, 16, 64), z(3, 2, 16, 64), z(1, 2, dt=i32), weight=z(3, 16, 2, dt=torch.float32)),
                 lambda: ofb.attn_decode(c, q, lens),  # host tensors
