@@ -205,11 +205,16 @@ __global__ void __launch_bounds__(AJ_THREADS) attn_weight_kernel(const __grid_co
     }
 }
 
-constexpr int ATT_SHORT = 4;
+// Tiles per warp up to which a sequence is left to a cluster: 2 heads of 16 over one
+// sequence of 1500 entries (two tiles) 7.9 us, as runs and a join 8.6; of 2500 10.9
+// and 9.3. CTAs of one warp, up to 4 tiles: 64 x 8 kv heads of 100 entries with
+// weights 18.0 us against 21.7, 95 x 3 of 15 entries (256) 12.4 against 27.7.
+constexpr int ATT_SHORT = 3, ATT_ONE_WARP = 4;
 
 struct AttnPlan {
     AttnVariant v;
     int max_len, ctas, NB, rows;
+    int warps;    // of a CTA of those
     int cluster;  // CTAs per (sequence, pass) that join by themselves, or 0: runs and a second launch
     int64_t z_stride;
     size_t prefix, ml, part_o, part_ml, z, total;
@@ -245,16 +250,23 @@ static int attn_plan(const ofb_kv_cache *c, int n_heads, int n_seqs, int max_len
     case 192: p.v = attn_variant_192(bf, f32, p.rows); break;
     default: p.v = attn_variant_256(bf, f32, p.rows); break;
     }
-    const int64_t runs = (tiles * n_seqs * c->n_kv_heads * p.NB + p.v.warps - 1) / p.v.warps;
+    const int64_t runs = (int64_t)n_seqs * c->n_kv_heads * p.NB * ((tiles + p.v.warps - 1) / p.v.warps);
     const int most = sm_count() * p.v.ctas;
-    // Short sequences: as many CTAs as give each warp ATT_SHORT tiles at most,
-    // where all of them have room at once. Weights need all of a kv head's
-    // query heads in one pass.
+    const int64_t units = (int64_t)n_seqs * c->n_kv_heads * p.NB;
+    // Short sequences: clusters of as many CTAs as give each warp a tile, while all
+    // have room at once and no warp more than ATT_SHORT; for so many sequences that
+    // they have no room at once a CTA of one warp each, of which an SM holds more.
+    // Weights need all of a kv head's query heads in one pass.
     p.cluster = 0;
     if (!accumulate || p.NB == 1) {
         int n = 1;
-        while (n < 8 && tiles > n * p.v.warps) n *= 2;
-        if (tiles <= (int64_t)n * p.v.warps * ATT_SHORT && (int64_t)n_seqs * c->n_kv_heads * p.NB * n <= most) p.cluster = n;
+        while (n < 8 && tiles > n * p.v.warps && 2 * n * units <= most) n *= 2;
+        if (units <= most && tiles <= (int64_t)n * p.v.warps * ATT_SHORT) {
+            p.cluster = n;
+            p.warps = p.v.warps;
+        } else if (units > most && tiles <= ATT_ONE_WARP) {
+            p.cluster = p.warps = 1;
+        }
     }
     p.ctas = runs < 1 ? 1 : runs < most ? (int)runs : most;
     const size_t parts = 2 * (size_t)ATT_MAX_CTAS * sm_count();  // whatever the type: one scratch serves both
@@ -329,13 +341,14 @@ extern "C" int ofb_attn_decode(const ofb_kv_cache *cache, const void *q, int typ
     const int vi = (cache->head_dim == 64 ? 0 : cache->head_dim == 96 ? 1 : cache->head_dim == 128 ? 2 : cache->head_dim == 192 ? 3 : 4) * 16 +
                    (cache->type == OFB_TYPE_BF16 ? 8 : 0) + (type == OFB_TYPE_F32 ? 4 : 0) + (p.rows == 16 ? 2 : 0);
     if (p.cluster) {
+        const size_t smem = p.v.head - (size_t)(p.v.warps - p.warps) * p.v.ring;
         cudaError_t e = ensure_dyn_smem(p.v.cluster, p.v.head, attr[vi + 1]);
         if (e != cudaSuccess) return cuda_status(e, "ofb_attn_decode smem attribute");
-        e = launch_pdl_cluster(p.v.cluster, dim3((unsigned)(n_seqs * a.KVH * a.NB * p.cluster)), dim3(p.v.warps * 32), p.cluster,
-                               p.v.head, s, a);
+        e = launch_pdl_cluster(p.v.cluster, dim3((unsigned)(n_seqs * a.KVH * a.NB * p.cluster)), dim3(p.warps * 32), p.cluster,
+                               smem, s, a);
         return e == cudaSuccess ? OFB_OK : cuda_status(e, "ofb_attn_decode launch");
     }
-    const size_t smem = p.v.head + (size_t)n_seqs * 4 + (n_seqs + 3) / 4 * 4;
+    const size_t smem = p.v.head + (size_t)(n_seqs + 1) * 4 + (n_seqs + 3) / 4 * 4;
     cudaError_t e = ensure_dyn_smem(p.v.run, smem, attr[vi]);
     if (e != cudaSuccess) return cuda_status(e, "ofb_attn_decode smem attribute");
     e = launch_pdl(p.v.run, dim3(p.ctas), dim3(p.v.warps * 32), smem, s, a);

@@ -122,12 +122,12 @@ template <int D, int QB> struct AttnShape {
     static constexpr int S = D <= 64 ? 3 : 2;                // ring slots
     static constexpr int CTAS = D <= 128 ? 2 : 1;            // per SM
     static constexpr int THREADS = W * 32;
-    static constexpr int RING = W * S * TILE_BYTES;
     // behind the ring: the warps' and the cluster's (maximum, sum), the queries'
     // fragments, then per sequence
     // the places before it and the entries of its last tile
-    static constexpr int HEAD = RING + (W + 1) * 16 * 8 + QB;
-    static constexpr int smem(int B) { return HEAD + (B + 1) * 4 + (B + 3) / 4 * 4; }
+    static __host__ __device__ constexpr int ring(int w) { return w * S * TILE_BYTES; }
+    static __host__ __device__ constexpr int head(int w) { return ring(w) + (W + 1) * 16 * 8 + QB; }
+    static constexpr int smem(int B) { return head(W) + (B + 1) * 4 + (B + 3) / 4 * 4; }
     static_assert(CTAS <= ATT_MAX_CTAS, "parts in the scratch");
     static_assert(TILE_BYTES >= 16 * (D + 4) * 4, "a warp's sums must fit one ring slot");
     static_assert(CTAS * (smem(384) + 2048) <= 228 * 1024, "shared memory of an SM");
@@ -239,26 +239,28 @@ __global__ void __launch_bounds__(AttnShape<D, AttnQuery<D, R, CT, IO>::QB>::THR
     constexpr bool DIRECT = !F32 && D <= 128;        // the tensor core accumulates (registers allow no more)
     constexpr int NO = DIRECT || R == 16 ? 4 : 2;    // accumulators of 8 columns
     constexpr int KS = D / 16, CH = D / 8;           // k steps; 16-byte chunks of a row
-    constexpr int W = SH::W, THREADS = SH::THREADS;
+    // CLUSTER: fewer warps where there are fewer tiles
+    const int W = CLUSTER ? (int)blockDim.x >> 5 : SH::W, THREADS = W * 32;
     // the next part's queries are asked for while registers hold them beside the sums
     constexpr bool AHEAD = NR * D * sizeof(IO) <= 512;
     extern __shared__ __align__(128) uint8_t smem[];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, c2 = (lane & 3) * 2;
     uint8_t *ring = smem + warp * SH::S * SH::TILE_BYTES;
-    float2 *mml = reinterpret_cast<float2 *>(smem + SH::RING);  // [W][R]
-    float2 *cml = mml + W * R;                          // [R]: the cluster's
-    int *prefix = reinterpret_cast<int *>(smem + SH::HEAD);     // [B + 1]
+    float2 *mml = reinterpret_cast<float2 *>(smem + SH::ring(W));  // [W][R]
+    float2 *cml = mml + SH::W * R;                          // [R]: the cluster's
+    int *prefix = reinterpret_cast<int *>(smem + SH::head(W));  // [B + 1]
     uint8_t *last = reinterpret_cast<uint8_t *>(prefix + a.B + 1);
     // fragments: [KS][32] of four registers, then [KS][32] of the two of the second
     // fragment that are not zero
-    uint4 *const q4 = reinterpret_cast<uint4 *>(smem + SH::RING + (W + 1) * 16 * 8);
+    uint4 *const q4 = reinterpret_cast<uint4 *>(smem + SH::ring(W) + (SH::W + 1) * 16 * 8);
     uint2 *const q2 = reinterpret_cast<uint2 *>(q4 + KS * 32);
-    __shared__ uint32_t valid[W][4];  // per ring slot: which of the 32 entries are there
-    __shared__ int wsum[W];
-    __shared__ float *mo[W];  // each warp's sums at the end of a part, [R][D + 4]
+    __shared__ uint32_t valid[SH::W][4];  // per ring slot: which of the 32 entries are there
+    __shared__ int wsum[SH::W];
+    __shared__ float *mo[SH::W];  // each warp's sums at the end of a part, [R][D + 4]
     __shared__ float2 all_ml[8][R];  // CLUSTER: every CTA's (maximum, sum) ...
     __shared__ int all_at[8];            // ... and where its sums are in its shared memory
     cg::cluster_group cl = cg::this_cluster();
+    const int C = CLUSTER ? (int)cl.num_blocks() : 1, rank = CLUSTER ? (int)cl.block_rank() : 0;
 
     pdl_wait();
     pdl_trigger();
@@ -267,8 +269,8 @@ __global__ void __launch_bounds__(AttnShape<D, AttnQuery<D, R, CT, IO>::QB>::THR
     int f0 = 0, f1 = 1;
     AttnPart first;
     if constexpr (CLUSTER) {
-        cl.barrier_arrive();  // waited for before the others' shared memory is written
-        const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank(), u = blockIdx.x / C;
+        if (C > 1) cl.barrier_arrive();  // waited for before the others' shared memory is written
+        const int u = blockIdx.x / C;
         first.b = u / nvh;
         first.vh = u - first.b * nvh;
         if (a.lens[first.b] > a.max_len && first.vh == 0 && rank == 0 && tid == 0) report(a.errors, OFB_CACHE_ELEN);
@@ -594,9 +596,11 @@ __global__ void __launch_bounds__(AttnShape<D, AttnQuery<D, R, CT, IO>::QB>::THR
         float *const mslot = reinterpret_cast<float *>(ring + (slot == 0 ? SH::S - 1 : slot - 1) * SH::TILE_BYTES);
         float *mw = mslot + g * (D + 4);
         if (lane == 0) mo[warp] = mslot;
-        if constexpr (CLUSTER) cl.barrier_wait();
-        if (CLUSTER && tid < (int)cl.num_blocks())  // tell every CTA where warp 0's sums are
-            *cl.map_shared_rank(&all_at[cl.block_rank()], tid) = (int)(reinterpret_cast<uint8_t *>(mslot) - smem);
+        if (CLUSTER && C > 1) {
+            cl.barrier_wait();
+            if (tid < C)  // tell every CTA where warp 0's sums are
+                *cl.map_shared_rank(&all_at[rank], tid) = (int)(reinterpret_cast<uint8_t *>(mslot) - smem);
+        }
 #pragma unroll
         for (int i = 0; i < D / 8; i++) {
             if (R == 16) {
@@ -619,18 +623,20 @@ __global__ void __launch_bounds__(AttnShape<D, AttnQuery<D, R, CT, IO>::QB>::THR
             if (AHEAD && go_on) ask_queries(next);
         }
         __syncthreads();
-        const bool whole = !CLUSTER && p.t == 0 && p.end == p.nt;
+        const bool whole = CLUSTER ? C == 1 : p.t == 0 && p.end == p.nt;
         const int64_t slot_id = 2 * (int64_t)blockIdx.x + (npart ? 1 : 0);
         for (int i = tid; i < rows * (D / 4); i += THREADS) {
             const int r = i / (D / 4), x = (i - r * (D / 4)) * 4;
             float mm = -INFINITY;
 #pragma unroll
-            for (int w = 0; w < W; w++) mm = fmaxf(mm, mml[w * R + r].x);
+            for (int w = 0; w < SH::W; w++)
+                if (w < W) mm = fmaxf(mm, mml[w * R + r].x);
             const float ref = mm == -INFINITY ? 0.0f : mm;
             float ll = 0.0f;
             float4 acc = make_float4(0, 0, 0, 0);
 #pragma unroll
-            for (int w = 0; w < W; w++) {
+            for (int w = 0; w < SH::W; w++) {
+                if (w >= W) break;
                 const float2 e = mml[w * R + r];
                 const float s = exp2_fast(e.x - ref);
                 const float4 y = *reinterpret_cast<const float4 *>(mo[w] + r * (D + 4) + x);
@@ -638,17 +644,19 @@ __global__ void __launch_bounds__(AttnShape<D, AttnQuery<D, R, CT, IO>::QB>::THR
                 acc.x += s * y.x, acc.y += s * y.y, acc.z += s * y.z, acc.w += s * y.w;
             }
             const int64_t head = kvh * a.G + h0 + r;
-            if (CLUSTER) {  // in place of warp 0's sums, whose elements only this thread reads
+            if (CLUSTER && C > 1) {  // in place of warp 0's sums, whose elements only this thread reads
                 *reinterpret_cast<float4 *>(mo[0] + r * (D + 4) + x) = acc;
-                if (x == 0)
-                    for (int c = 0; c < (int)cl.num_blocks(); c++) cl.map_shared_rank(&all_ml[0][0], c)[cl.block_rank() * R + r] = make_float2(mm, ll);
+                if (x < 4 * C) cl.map_shared_rank(&all_ml[0][0], x / 4)[rank * R + r] = make_float2(mm, ll);  // to CTA x / 4
             } else if (whole) {
                 // no entry attended to (all on bad pages): zeros
                 const float inv = ll > 0.0f || ll != ll ? 1.0f / (ll * PSCALE) : 0.0f;
                 IO *dst = static_cast<IO *>(a.out) + p.b * a.out_stride + head * D + x;
                 dst[0] = from_f32<IO>(acc.x * inv), dst[1] = from_f32<IO>(acc.y * inv);
                 dst[2] = from_f32<IO>(acc.z * inv), dst[3] = from_f32<IO>(acc.w * inv);
-                if (x == 0) a.ml[(int64_t)p.b * a.H + head] = make_float2(mm, ll);
+                if (x == 0) {
+                    if (CLUSTER) cml[r] = make_float2(ref, inv * PSCALE);
+                    else a.ml[(int64_t)p.b * a.H + head] = make_float2(mm, ll);
+                }
             } else {
                 const float u = 1.0f / PSCALE;
                 *reinterpret_cast<float4 *>(a.part_o + (slot_id * R + r) * D + x) = make_float4(acc.x * u, acc.y * u, acc.z * u, acc.w * u);
@@ -658,36 +666,41 @@ __global__ void __launch_bounds__(AttnShape<D, AttnQuery<D, R, CT, IO>::QB>::THR
         if constexpr (CLUSTER) {
             // join the cluster's CTAs, whose maxima and sums have been told to
             // all; each writes some of the columns
-            const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
-            cl.sync();
-            if (tid < rows) {
-                float mm = -INFINITY, ll = 0.0f;
-                for (int r = 0; r < C; r++) mm = fmaxf(mm, all_ml[r][tid].x);
-                const float ref = mm == -INFINITY ? 0.0f : mm;
-                for (int r = 0; r < C; r++) ll += exp2_fast(all_ml[r][tid].x - ref) * all_ml[r][tid].y;
-                cml[tid] = make_float2(ref, ll > 0.0f || ll != ll ? 1.0f / ll : 0.0f);
-            }
-            __syncthreads();
-            for (int i = rank * THREADS + tid; i < rows * (D / 4); i += C * THREADS) {
+            if (C > 1) cl.sync();
+            for (int i = rank * THREADS + tid; C > 1 && i < rows * (D / 4); i += C * THREADS) {
                 const int r = i / (D / 4), x = (i - r * (D / 4)) * 4;
-                const float2 fin = cml[r];
                 float4 y[8];
+                float mm = -INFINITY, ll = 0.0f;
 #pragma unroll
                 for (int c = 0; c < 8; c++)
-                    if (c < C) y[c] = *reinterpret_cast<const float4 *>(cl.map_shared_rank(smem, c) + all_at[c] + (r * (D + 4) + x) * 4);
+                    if (c < C) {
+                        y[c] = *reinterpret_cast<const float4 *>(cl.map_shared_rank(smem, c) + all_at[c] + (r * (D + 4) + x) * 4);
+                        mm = fmaxf(mm, all_ml[c][r].x);
+                    }
+                const float ref = mm == -INFINITY ? 0.0f : mm;
                 float4 acc = make_float4(0, 0, 0, 0);
 #pragma unroll
                 for (int c = 0; c < 8; c++)
                     if (c < C) {
-                        const float s = exp2_fast(all_ml[c][r].x - fin.x);
+                        const float2 e = all_ml[c][r];
+                        const float s = exp2_fast(e.x - ref);
+                        ll += s * e.y;
                         acc.x += s * y[c].x, acc.y += s * y[c].y, acc.z += s * y[c].z, acc.w += s * y[c].w;
                     }
-                const float inv = fin.y / PSCALE;
+                const float inv = ll > 0.0f || ll != ll ? 1.0f / (ll * PSCALE) : 0.0f;
                 IO *dst = static_cast<IO *>(a.out) + p.b * a.out_stride + (int64_t)(kvh * a.G + h0 + r) * D + x;
                 dst[0] = from_f32<IO>(acc.x * inv), dst[1] = from_f32<IO>(acc.y * inv);
                 dst[2] = from_f32<IO>(acc.z * inv), dst[3] = from_f32<IO>(acc.w * inv);
             }
             if (a.z) {  // one pass per kv head here: this CTA's entries are its own
+                if (C > 1 && tid < rows) {
+                    float mm = -INFINITY, ll = 0.0f;
+                    for (int c = 0; c < C; c++) mm = fmaxf(mm, all_ml[c][tid].x);
+                    const float ref = mm == -INFINITY ? 0.0f : mm;
+                    for (int c = 0; c < C; c++) ll += exp2_fast(all_ml[c][tid].x - ref) * all_ml[c][tid].y;
+                    cml[tid] = make_float2(ref, ll > 0.0f || ll != ll ? 1.0f / ll : 0.0f);
+                }
+                __syncthreads();
                 const int i1 = min(p.end * ATT_TILE, p.len);
                 for (int i = p.t * ATT_TILE + tid; i < i1; i += THREADS) {
                     const float *z = a.z + ((int64_t)p.b * a.H + kvh * a.G) * a.z_stride + i;
@@ -697,7 +710,7 @@ __global__ void __launch_bounds__(AttnShape<D, AttnQuery<D, R, CT, IO>::QB>::THR
                     if (page >= 0 && page < a.n_pages) a.weight[((int64_t)page * a.KVH + kvh) * a.page_size + (i - col * a.page_size)] += add;
                 }
             }
-            cl.sync();  // no CTA leaves while its sums are read
+            if (C > 1) cl.sync();  // no CTA leaves while its sums are read
             break;
         }
         if (!go_on) break;
@@ -712,7 +725,8 @@ __global__ void __launch_bounds__(AttnShape<D, AttnQuery<D, R, CT, IO>::QB>::THR
 using AttnKernel = void (*)(AttnArgs);
 struct AttnVariant {
     AttnKernel run, cluster;
-    int head, ctas, warps;  // shared memory without the per-sequence part, CTAs per SM, warps per CTA
+    int ctas, warps;            // CTAs per SM, warps per CTA
+    int ring, head;             // shared memory: a warp's ring; all rings and what follows, but for the per-sequence part
 };
 // Whether there are instances for 16 heads per pass: not where registers cannot
 // hold 16 f32 queries and sums.
@@ -728,7 +742,8 @@ AttnVariant attn_variant_256(bool bf16, bool f32, int rows);
 template <int D, int R, typename CT, typename IO> AttnVariant attn_instance() {
     if constexpr (R == 8 || attn_wide_rows(D, sizeof(IO) == 4)) {
         using SH = AttnShape<D, AttnQuery<D, R, CT, IO>::QB>;
-        return {attn_split_kernel<D, R, CT, IO, false>, attn_split_kernel<D, R, CT, IO, true>, SH::smem(0), SH::CTAS, SH::W};
+        return {attn_split_kernel<D, R, CT, IO, false>, attn_split_kernel<D, R, CT, IO, true>, SH::CTAS, SH::W,
+                SH::ring(1), SH::head(SH::W)};
     } else {
         return {};
     }

@@ -43,7 +43,13 @@ constexpr int EV_WARPS = EV_THREADS / 32;
 constexpr int EV_CLUSTER = 8;   // CTAs of a cluster at most
 constexpr int EV_BINS = 1024;
 constexpr int EV_SLICE = 64;    // moves of one CTA of the second launch
-constexpr int EV_FUSED = 4096;  // moves that may be, up to which there is none
+// moves per row that may be, up to which there is no second launch: 2 rows of 1100
+// entries down to 1024 take 10.4 us without and 11.4 with it, of 1536 16.2 and 12.2
+constexpr int EV_FUSED = 128;
+// entries per CTA from which a cluster is worth its barriers: 2 rows of 8000 take
+// 17.2 us with one CTA each and 20.1 with seven, of 16000 19.3 with three and 22.1
+// with one
+constexpr int EV_RUN = 4096;
 constexpr int EV_CAND = 256;    // entries ranked directly (at most one per thread)
 constexpr int EV_STATIC = 5120;  // bytes of the kernel's static arrays, rounded up
 constexpr int EV_KEYS = 49152;  // keys a CTA holds at most: OFB_EVICT_MAX_LEN / EV_CLUSTER
@@ -561,7 +567,7 @@ __global__ void __launch_bounds__(EV_MOVE_THREADS) evict_move_kernel(const __gri
 
 // CTAs per (sequence, kv head) and threads per CTA: what brings the most threads
 // onto the GPU with all CTAs there at once (an SM runs 1024 threads of this
-// kernel), as long as a CTA has 1024 entries and a thread two; fewer, larger
+// kernel), as long as a CTA has EV_RUN entries and a thread two; fewer, larger
 // CTAs where that is nearly the same.
 static void evict_shape(int rows, int max_len, int &ctas, int &threads) {
     ctas = 0;
@@ -572,7 +578,7 @@ static void evict_shape(int rows, int max_len, int &ctas, int &threads) {
         // a cluster lies within one of the GPU's eight groups of 16 SMs or more
         int c = slots / rows;
         while (c > 1 && 8 * (16 * per_sm / c) < rows) c--;
-        if (c > max_len / 1024) c = max_len / 1024;
+        if (c > max_len / EV_RUN) c = max_len / EV_RUN;
         c = c < 1 ? 1 : c > EV_CLUSTER ? EV_CLUSTER : c;
         while (c < EV_CLUSTER && (max_len + c - 1) / c > EV_KEYS) c++;
         const int64_t n = rows > slots ? 0 : (int64_t)rows * c * t;
@@ -645,7 +651,7 @@ extern "C" int ofb_kv_evict(const ofb_kv_cache *cache, const int32_t *lens, int 
     a.counts = a.lists + rows * 2 * keep;
     const int most = bound <= keep ? 0 : bound - keep < keep ? bound - keep : keep;  // moves of a row
     a.kept_quads = keep % 4 == 0 && !misaligned(kept, 16);
-    a.fused = rows * most <= EV_FUSED;
+    a.fused = most <= EV_FUSED;
     a.slices = (most + EV_SLICE - 1) / EV_SLICE;
     if (!a.fused && rows * a.slices > INT32_MAX) { set_error("ofb_kv_evict: too many moves"); return OFB_ETOOLARGE; }
     int C, threads = 256;
