@@ -6,12 +6,13 @@
 //
 // HBM-bound: every element is read and written once, in one launch for q, k
 // and v. A CTA owns a few tokens. It first forms the cosine and sine of each
-// (token, pair) once in shared memory, for all heads: pos * f / pi in f64 (a
-// position of a million turns with f = 1 would lose its place in f32), less
-// the nearest even integer, so that the f32 that goes to sincospif is within
-// [-1, 1] and off by at most 2^-25 half turns. f(i)/pi comes with the launch:
-// the host forms it by one powl and repeated products, 1 KB of arguments.
-// Then each thread takes items of two 8-element chunks (the two halves of 8
+// (token, pair) once in shared memory, for all heads. A far position times a
+// frequency would lose its place in the turn in f32; here f(i) / 2 pi comes as a
+// 64-bit fraction of a turn, and since positions are integers, the product's low
+// 64 bits are the exact place: its top word, as f32 half turns within [-1, 1], is
+// off by at most 2^-25 + 2^-31 (and by 2^-34 for the fraction's own rounding at
+// position 2^31). The host forms the fractions by one powl and repeated products,
+// 1 KB of arguments. Then each thread takes items of two 8-element chunks (the two halves of 8
 // pairs, or 16 neighbours), read and written 16 bytes at a time. Sizes or addresses
 // that do not allow it (head_dim or rot_dim no multiple of 16, strides no
 // multiple of 8, pointers off 16 bytes) take the second kernel, a pair per
@@ -28,7 +29,8 @@ constexpr int RP_TOKENS = 1 << 30;
 
 struct RopeArgs {
     int T, H, KVH, d, rot, tpb;  // heads of q; kv heads (0: no cache); tokens of a group
-    int slots;                   // first kernel: rows under way, threads / per_row
+    // first kernel: rows of a CTA under way, CTAs that share a group's rows
+    int slots, split;
     int n_pages, page_size, n_seqs, max_pages;
     FastDiv page, rows, per_row;  // by page_size, by H + 2 KVH, by chunk pairs of a row
     const void *q, *k, *v;
@@ -38,7 +40,7 @@ struct RopeArgs {
     float *weight;
     int32_t *order;
     uint32_t *errors;
-    double half_turns[RP_PAIRS];  // f(i) / pi
+    uint64_t turns[RP_PAIRS];     // f(i) / 2 pi, a fraction of 2^64
     uint8_t axis[RP_PAIRS];
 };
 
@@ -46,6 +48,14 @@ struct RopeArgs {
 struct RopeEntry {
     int page, slot, number;
 };
+// Cosine and sine of position pos at a frequency.
+__device__ __forceinline__ float2 rope_angle(int pos, uint64_t turns) {
+    const uint64_t place = (uint64_t)(int64_t)pos * turns;
+    float s, c;
+    sincospif((float)(int)(place >> 32) * 0x1p-31f, &s, &c);
+    return make_float2(c, s);
+}
+
 // The place of token t's rows; reports what is wrong with it.
 __device__ __forceinline__ RopeEntry rope_entry(const RopeArgs &a, int t) {
     const int b = a.seq[t], i = a.index[t];
@@ -78,16 +88,14 @@ __device__ __forceinline__ void rope_setup(const RopeArgs &a, int t0, int nt, co
     const int pairs = a.rot / 2;
     // read through a plain address: lanes want different pairs, which the
     // constant bank would serve one at a time
-    const double *freq = a.half_turns;
+    const uint64_t *freq = a.turns;
     const uint8_t *axis = a.axis;
     asm("" : "+l"(freq), "+l"(axis));
     for (int i = threadIdx.x; i < nt * pairs; i += RP_THREADS) {
         const int t = i / pairs, p = i - t * pairs;
-        const double h = (double)a.pos[axis[p] * a.pos_stride + t0 + t] * freq[p];
-        float s, c;
-        sincospif((float)(h - 2.0 * rint(0.5 * h)), &s, &c);
-        sh.c[i] = c;
-        sh.s[i] = s;
+        const float2 cs = rope_angle(a.pos[axis[p] * a.pos_stride + t0 + t], freq[p]);
+        sh.c[i] = cs.x;
+        sh.s[i] = cs.y;
     }
     if (a.KVH && threadIdx.x < nt) sh.entry[threadIdx.x] = rope_entry(a, t0 + threadIdx.x);
     __syncthreads();
@@ -152,10 +160,12 @@ template <typename IO, typename CT, bool ADJ, bool CACHE>
 __global__ void __launch_bounds__(RV_THREADS, RV_CTAS) rope_vec_kernel(const __grid_constant__ RopeArgs a) {
     constexpr int BATCH = RV_BATCH<IO>;
     extern __shared__ __align__(16) float rope_smem[];  // cosines, sines [tpb][rot/2], places [tpb]
-    const int half = a.rot / 2, tid = threadIdx.x, t0 = blockIdx.x * a.tpb, nt = min(a.tpb, a.T - t0);
+    const int half = a.rot / 2, tid = threadIdx.x, part = blockIdx.x % a.split;
+    const int t0 = blockIdx.x / a.split * a.tpb, nt = min(a.tpb, a.T - t0);
     float *const cosines = rope_smem, *const sines = rope_smem + a.tpb * half;
     RopeEntry *const entry = reinterpret_cast<RopeEntry *>(rope_smem + a.tpb * a.rot);
-    const int slot = a.per_row.div(tid), j = tid - slot * (int)a.per_row.d, total = slot < a.slots ? nt * (int)a.rows.d : 0;
+    const int in = a.per_row.div(tid), j = tid - in * (int)a.per_row.d, total = in < a.slots ? nt * (int)a.rows.d : 0;
+    const int slot = part * a.slots + in, step = a.split * a.slots;  // first row, from one item to the next
     // The thread's two chunks of 8 elements and where their cosines are. HALVES:
     // the two halves of 8 pairs, or two chunks behind rot; ADJACENT: 4 pairs
     // each, half a row apart. Neighbouring threads have neighbouring chunks.
@@ -175,8 +185,8 @@ __global__ void __launch_bounds__(RV_THREADS, RV_CTAS) rope_vec_kernel(const __g
     auto fetch = [&](int vr) {
 #pragma unroll
         for (int k = 0; k < BATCH; k++)
-            if (vr + k * a.slots < total) {
-                const RopeRow r = rope_row(a, vr + k * a.slots);
+            if (vr + k * step < total) {
+                const RopeRow r = rope_row(a, vr + k * step);
                 if constexpr (CACHE) raw[k].load(rope_src<IO>(a, r, t0), ta, tb);
                 else raw[k].load(static_cast<const IO *>(a.q) + (t0 + r.t) * a.qs + (int64_t)r.row * a.d, ta, tb);
             }
@@ -185,25 +195,23 @@ __global__ void __launch_bounds__(RV_THREADS, RV_CTAS) rope_vec_kernel(const __g
     // (by the last threads: the first ones have the cosines)
     if (CACHE && RV_THREADS - 1 - tid < nt) entry[RV_THREADS - 1 - tid] = rope_entry(a, t0 + RV_THREADS - 1 - tid);
     {
-        const double *freq = a.half_turns;  // see rope_setup
+        const uint64_t *freq = a.turns;  // see rope_setup
         const uint8_t *axis = a.axis;
         asm("" : "+l"(freq), "+l"(axis));
         for (int i = tid; i < nt * half; i += RV_THREADS) {
             const int t = a.tpb == 1 ? 0 : i / half, p = i - t * half;
-            const double h = (double)a.pos[axis[p] * a.pos_stride + t0 + t] * freq[p];
-            float s, c;
-            sincospif((float)(h - 2.0 * rint(0.5 * h)), &s, &c);
-            cosines[i] = c;
-            sines[i] = s;
+            const float2 cs = rope_angle(a.pos[axis[p] * a.pos_stride + t0 + t], freq[p]);
+            cosines[i] = cs.x;
+            sines[i] = cs.y;
         }
     }
     __syncthreads();
-    for (int vr = slot; vr < total; vr += BATCH * a.slots) {
+    for (int vr = slot; vr < total; vr += BATCH * step) {
         if (vr > slot) fetch(vr);
 #pragma unroll
         for (int k = 0; k < BATCH; k++) {
-            if (vr + k * a.slots >= total) break;
-            const RopeRow r = rope_row(a, vr + k * a.slots);
+            if (vr + k * step >= total) break;
+            const RopeRow r = rope_row(a, vr + k * step);
             const bool is_q = !CACHE || r.row < a.H, is_v = CACHE && r.row >= a.H + a.KVH;
             float x[8], y[8];
             load8(reinterpret_cast<const IO *>(raw[k].x), x);
@@ -289,7 +297,7 @@ __global__ void __launch_bounds__(RP_THREADS) rope_any_kernel(const __grid_const
     rope_meta(a, nt, sh.entry);
 }
 
-// Checks a rotary form and lays out its pairs: axis and frequency / pi.
+// Checks a rotary form and lays out its pairs: axis and frequency / 2 pi.
 static int rope_tables(const ofb_rope_config *r, int head_dim, const char *who, RopeArgs &a) {
     if (r->rot_dim < 2 || r->rot_dim > 2 * RP_PAIRS || r->rot_dim % 2 || r->rot_dim > head_dim || r->n_axes < 1 ||
         r->n_axes > 4 || (r->pairing != OFB_ROPE_HALVES && r->pairing != OFB_ROPE_ADJACENT) ||
@@ -316,15 +324,15 @@ static int rope_tables(const ofb_rope_config *r, int head_dim, const char *who, 
     if (sum != pairs) { set_error("%s: the sections have %lld pairs, rot_dim/2 is %d", who, (long long)sum, pairs); return OFB_EINVAL; }
     a.rot = r->rot_dim;
     // powers by repeated products: with 64 bits of mantissa 127 of them stay
-    // within 2^-56, below what the f64 result can hold, for one powl per call
-    const long double inv_pi = 0.318309886183790671537767526745028724L;
+    // within 2^-56 of the frequency, for one powl per call
+    const long double inv_2pi = 0.159154943091895335768883763372514362L;
     int x = 0, left = r->section[0];
-    long double f = inv_pi, step = powl(r->base, -1.0L / (r->per_axis && left ? left : pairs));
+    long double f = inv_2pi, step = powl(r->base, -1.0L / (r->per_axis && left ? left : pairs));
     for (int i = 0; i < pairs; i++) {
         if (r->order == OFB_ROPE_BLOCKED) {
             while (!left) {
                 left = r->section[++x];
-                if (r->per_axis && left) f = inv_pi, step = powl(r->base, -1.0L / left);
+                if (r->per_axis && left) f = inv_2pi, step = powl(r->base, -1.0L / left);
             }
             left--;
             a.axis[i] = (uint8_t)x;
@@ -332,7 +340,9 @@ static int rope_tables(const ofb_rope_config *r, int head_dim, const char *who, 
             const int y = i % r->n_axes;
             a.axis[i] = (uint8_t)(i / r->n_axes < r->section[y] ? y : 0);
         }
-        a.half_turns[i] = (double)f;
+        // whole turns (frequencies above 2 pi) leave no trace at integer positions
+        const long double part = f - floorl(f);
+        a.turns[i] = part * 0x1p64L < 0x1p64L ? (uint64_t)(part * 0x1p64L) : 0;
         f *= step;
     }
     return OFB_OK;
@@ -351,9 +361,13 @@ template <typename IO, typename CT> static cudaError_t rope_launch(RopeArgs &a, 
     a.page = fast_div(a.page_size ? a.page_size : 1);
     a.per_row = fast_div(vec ? a.d / 16 : 1);
     a.slots = RV_THREADS / (int)a.per_row.d;
+    // few tokens with many rows: several CTAs share a token's rows
+    const int groups = (a.T + tpb - 1) / tpb, batches = (tpb * rows + a.slots * RV_BATCH<IO> - 1) / (a.slots * RV_BATCH<IO>);
+    a.split = 1;
+    while (vec && 2 * a.split <= batches && (int64_t)2 * a.split * groups <= 2 * sm_count()) a.split *= 2;
     // (a.rot is a multiple of 4 for the first kernel)
     const size_t smem = ((size_t)tpb * a.rot + 3) / 4 * 16 + tpb * sizeof(RopeEntry);
-    const dim3 grid((a.T + tpb - 1) / tpb), block(threads);
+    const dim3 grid(groups * a.split), block(threads);
     if (!vec) return launch_pdl(rope_any_kernel<IO, CT>, grid, block, smem, s, a, (int)adjacent);
     if (!a.KVH)
         return adjacent ? launch_pdl(rope_vec_kernel<IO, IO, true, false>, grid, block, smem, s, a)
