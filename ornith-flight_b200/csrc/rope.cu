@@ -341,8 +341,8 @@ static int rope_tables(const ofb_rope_config *r, int head_dim, const char *who, 
             a.axis[i] = (uint8_t)(i / r->n_axes < r->section[y] ? y : 0);
         }
         // whole turns (frequencies above 2 pi) leave no trace at integer positions
-        const long double part = f - floorl(f);
-        a.turns[i] = part * 0x1p64L < 0x1p64L ? (uint64_t)(part * 0x1p64L) : 0;
+        const long double part = f < 1.0L ? f : f - floorl(f);
+        a.turns[i] = (uint64_t)(part * 0x1p64L);
         f *= step;
     }
     return OFB_OK;

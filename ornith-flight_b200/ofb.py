@@ -242,14 +242,14 @@ def _need(ok: bool, what: str) -> None:
 
 
 def _ints(t: torch.Tensor, shape, device, name: str) -> int:
-    if t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous() or t.device != device:
+    if t.dtype is not torch.int32 or t.shape != shape or not t.is_contiguous() or t.device != device:
         raise OfbError(EINVAL, f"{name} must be contiguous int32 {tuple(shape)} on {device}")
     return t.data_ptr()
 
 
 def _rows(t: torch.Tensor, shape, dtype, device, name: str) -> int:
     """Elements from one row of t [rows, heads, head_dim] to the next; heads dense."""
-    if t.shape != shape or t.dtype != dtype or t.device != device:
+    if t.dtype is not dtype or t.shape != shape or t.device != device:
         raise OfbError(EINVAL, f"{name} must be {dtype} {tuple(shape)} on {device}")
     row, head, one = t.stride()
     if (one != 1 and shape[2] > 1) or (head != shape[2] and shape[1] > 1):
@@ -270,7 +270,8 @@ def _elsewhere(device: torch.device, stream, call, *args, **kw):
 
 def _away(device: torch.device, stream) -> bool:
     """Whether a call has to change the current device or stream first."""
-    return stream is not None or device.type != "cuda" or device.index != _get_device()
+    index = device.index  # None for host tensors
+    return stream is not None or index is None or index != _get_device()
 
 
 class KvCache:
@@ -323,7 +324,7 @@ def rope(x: torch.Tensor, pos: torch.Tensor, cfg: RopeConfig, out: torch.Tensor 
     if _away(dev, stream):
         return _elsewhere(dev, stream, rope, x, pos, cfg, out)
     if out is None:
-        out = torch.empty_like(x)
+        out = x.new_empty(shape)
     os_ = _rows(out, shape, dt, dev, "rope: out")
     _check(lib.ofb_rope(ctypes.byref(cfg), x.data_ptr(), _TYPE_OF[dt], T, H, d, xs, p, T, out.data_ptr(), os_,
                         _raw_stream(dev.index)))
@@ -358,7 +359,7 @@ def rope_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, seq: torch.Ten
         q_out = None
     else:
         if q_out is None:
-            q_out = torch.empty((T, H, d), dtype=dt, device=dev)
+            q_out = q.new_empty((T, H, d))
         os_ = _rows(q_out, (T, H, d), dt, dev, "rope_append: q_out")
     _check(lib.ofb_rope_append(cache._ref, None if rope is None else ctypes.byref(rope), _TYPE_OF[dt], T, H, _ptr(q), qs,
                                k.data_ptr(), ks, v.data_ptr(), vs, pp, T, sp, ip, np_, _ptr(q_out), os_,
@@ -399,7 +400,7 @@ def attn_decode(cache: KvCache, q: torch.Tensor, lens: torch.Tensor, scale: floa
     elif scratch.device != dev or not scratch.is_contiguous():
         raise OfbError(EINVAL, "attn_decode: scratch must be contiguous beside the cache")
     if out is None:
-        out = torch.empty(shape, dtype=dt, device=dev)
+        out = q.new_empty(shape)
     os_ = _rows(out, shape, dt, dev, "attn_decode: out")
     _check(lib.ofb_attn_decode(cache._ref, q.data_ptr(), _TYPE_OF[dt], qs, H, d ** -0.5 if scale is None else scale, lp, B,
                                max_len, int(accumulate), out.data_ptr(), os_, scratch.data_ptr(), scratch.nbytes,
@@ -431,9 +432,9 @@ def kv_evict(cache: KvCache, lens: torch.Tensor, keep: int, recent: int = 0, max
         raise OfbError(EINVAL, "kv_evict: scratch must be contiguous beside the cache")
     shape = (B, cache.n_kv_heads, keep)
     if kept is None:
-        kept = torch.empty(shape, dtype=torch.int32, device=dev)
+        kept = lens.new_empty(shape)
     if lens_out is None:
-        lens_out = torch.empty_like(lens)
+        lens_out = lens.new_empty(B)
     _check(lib.ofb_kv_evict(cache._ref, lp, B, max_len, keep, recent, _ints(lens_out, (B,), dev, "kv_evict: lens_out"),
                             _ints(kept, shape, dev, "kv_evict: kept"), scratch.data_ptr(), scratch.nbytes,
                             _raw_stream(dev.index)))
