@@ -4,20 +4,26 @@
 // Second launch (programmatic, its CTAs come up as the split kernel's leave): the
 // parts of a head that more than one run holds are joined in the order of the runs,
 //   M = max m_i, out = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i,
-// so the result does not depend on which CTA took which run, nor on when. A CTA
-// takes one head, its warps every eighth part, where a head has many parts, and
-// eight heads of a kv head, a warp each, where it has few.
+// so the result does not depend on which CTA took which run, nor on when. Where a
+// head has many parts, a CTA takes 32 columns of it and a quarter of a warp every
+// 32nd part (one sequence of 131071 entries, 16 heads of 128 in some 150 parts each:
+// 30.7 us in all, with all columns in one CTA 33.1); where it has few, a CTA takes
+// eight heads of a kv head, a warp each.
 //
 // Third launch, with `accumulate`: each entry's probability, summed over the query
 // heads of its kv head in their order, is added to the cache's weight, four
 // entries per thread. It reads the scores the split kernel left (4 bytes per entry
-// and query head, an eighth of the entry's K and V at 8 heads of 128; forming them
-// again would read all of K a second time).
+// and query head, an sixteenth of the entry's K and V at 8 heads of 128; forming them
+// again would read all of K a second time). Of 176 us for 48 ragged sequences, 32 heads
+// over 8 kv heads of 128, the scores' way through HBM takes some 15 and this launch
+// 10. Asking L2 to keep them, whole lines per store, or weights and join in one launch
+// did not make it less.
 #include "attn.cuh"
 
 namespace ofb {
 
 constexpr int AJ_THREADS = 256;  // 8 warps, a row each where a CTA joins 8 rows
+constexpr int AJ_COLUMNS = 32;  // of a CTA that has one head's parts
 constexpr int AJ_CHUNK = 4 * AJ_THREADS;  // entries of one weight CTA
 
 struct AttnJoinArgs {
@@ -42,92 +48,113 @@ __device__ __forceinline__ PartRange part_range(const AttnJoinArgs &j, int b, in
     return r;
 }
 
-// Sums over parts w, w + step, ... of row r, by one warp: lane x4 has columns
-// 4 lane .. and, with more than 128 columns, 128 + 4 lane ..
-struct JoinSum {
+// Sums over parts w, w + step, ... of row r of 4 N columns x on, x + 128 on, for one
+// lane; columns from d on are not there.
+template <int N> struct JoinSum {
     float m, l;
-    float4 o[2];
-    __device__ __forceinline__ void add(const AttnJoinArgs &j, const PartRange &pr, int r, int w, int step, int lane) {
+    float4 o[N];
+    __device__ __forceinline__ void add(const AttnJoinArgs &j, const PartRange &pr, int r, int w, int step, int x) {
         m = -INFINITY, l = 0.0f;
-        o[0] = o[1] = make_float4(0, 0, 0, 0);
+#pragma unroll
+        for (int h = 0; h < N; h++) o[h] = make_float4(0, 0, 0, 0);
         constexpr int UN = 4;
         for (int i0 = w; i0 < pr.n; i0 += UN * step) {
             float2 e[UN];
-            float4 y[UN][2];
+            float4 y[UN][N];
 #pragma unroll
             for (int k = 0; k < UN; k++) {
                 const int i = i0 + k * step;
                 e[k] = make_float2(-INFINITY, 0.0f);
-                y[k][0] = y[k][1] = make_float4(0, 0, 0, 0);
+#pragma unroll
+                for (int h = 0; h < N; h++) y[k][h] = make_float4(0, 0, 0, 0);
                 if (i < pr.n) {
                     const int p = pr.slot(i) * j.rows + r;
                     const float *src = j.a.part_o + (int64_t)p * j.d;
                     e[k] = j.a.part_ml[p];
-                    if (4 * lane < j.d) y[k][0] = *reinterpret_cast<const float4 *>(src + 4 * lane);
-                    if (128 + 4 * lane < j.d) y[k][1] = *reinterpret_cast<const float4 *>(src + 128 + 4 * lane);
+#pragma unroll
+                    for (int h = 0; h < N; h++)
+                        if (128 * h + x < j.d) y[k][h] = *reinterpret_cast<const float4 *>(src + 128 * h + x);
                 }
             }
             float mn = m;
 #pragma unroll
             for (int k = 0; k < UN; k++) mn = fmaxf(mn, e[k].x);
-            const float ref = mn == -INFINITY ? 0.0f : mn, old = exp2_fast(m - ref);
-            m = mn;
-            l *= old;
-#pragma unroll
-            for (int h = 0; h < 2; h++) o[h].x *= old, o[h].y *= old, o[h].z *= old, o[h].w *= old;
+            rescale(mn);
+            const float ref = mn == -INFINITY ? 0.0f : mn;
 #pragma unroll
             for (int k = 0; k < UN; k++) {
                 const float f = exp2_fast(e[k].x - ref);
                 l += f * e[k].y;
 #pragma unroll
-                for (int h = 0; h < 2; h++)
+                for (int h = 0; h < N; h++)
                     o[h].x += f * y[k][h].x, o[h].y += f * y[k][h].y, o[h].z += f * y[k][h].z, o[h].w += f * y[k][h].w;
             }
         }
+    }
+    __device__ __forceinline__ void rescale(float mn) {  // to the maximum mn
+        const float f = exp2_fast(m - (mn == -INFINITY ? 0.0f : mn));
+        m = mn;
+        l *= f;
+#pragma unroll
+        for (int h = 0; h < N; h++) o[h].x *= f, o[h].y *= f, o[h].z *= f, o[h].w *= f;
     }
 };
 
 template <typename IO> __global__ void __launch_bounds__(AJ_THREADS) attn_join_kernel(const __grid_constant__ AttnJoinArgs j) {
     constexpr int W = AJ_THREADS / 32;
-    __shared__ __align__(16) float acc[W][256 + 4];
+    __shared__ __align__(16) float acc[W][AJ_COLUMNS];
     __shared__ float2 ml[W];
     const AttnArgs &a = j.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     pdl_wait();
     pdl_trigger();
-    int b, vh, r;
+    int b, vh, r, x;
     if (j.wide) {
-        b = blockIdx.x / a.H;
-        const int h = blockIdx.x - b * a.H, kvh = h / a.G, g = h - kvh * a.G;
+        const int pieces = j.d / AJ_COLUMNS, u = blockIdx.x / pieces;
+        x = (blockIdx.x - u * pieces) * AJ_COLUMNS + lane % 8 * 4;
+        b = u / a.H;
+        const int h = u - b * a.H, kvh = h / a.G, g = h - kvh * a.G;
         vh = kvh * a.NB + g / j.rows, r = g % j.rows;
     } else {
         const int u = blockIdx.x / (j.rows / W);  // 8 rows per CTA
         b = u / (a.KVH * a.NB), vh = u - b * a.KVH * a.NB, r = (blockIdx.x - u * (j.rows / W)) * W + warp;
+        x = 4 * lane;
     }
     const int kvh = vh / a.NB, g = (vh - kvh * a.NB) * j.rows + r, nt = a.prefix[b + 1] - a.prefix[b] - ATT_PART;
     if (nt < 0) return;
     const PartRange pr = part_range(j, b, vh, nt);
     if (pr.n == 1 || g >= a.G) return;  // (`wide`: the CTA's only head, so all leave)
-    IO *const out = static_cast<IO *>(a.out) + b * a.out_stride + (int64_t)(kvh * a.G + g) * j.d;
-    JoinSum s;
-    s.add(j, pr, r, j.wide ? warp : 0, j.wide ? W : 1, lane);
+    IO *const out = static_cast<IO *>(a.out) + b * a.out_stride + (int64_t)(kvh * a.G + g) * j.d + x;
+    float2 *const joined = a.ml + (int64_t)b * a.H + kvh * a.G + g;  // for the weights
     if (!j.wide) {
-        if (lane == 0) a.ml[(int64_t)b * a.H + kvh * a.G + g] = make_float2(s.m, s.l);
+        JoinSum<2> s;
+        s.add(j, pr, r, 0, 1, x);
+        if (lane == 0) *joined = make_float2(s.m, s.l);
         const float inv = s.l > 0.0f || s.l != s.l ? 1.0f / s.l : 0.0f;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-            const int x = 128 * h + 4 * lane;
-            if (x >= j.d) break;
-            out[x] = from_f32<IO>(s.o[h].x * inv), out[x + 1] = from_f32<IO>(s.o[h].y * inv);
-            out[x + 2] = from_f32<IO>(s.o[h].z * inv), out[x + 3] = from_f32<IO>(s.o[h].w * inv);
+            if (128 * h + x >= j.d) break;
+            out[128 * h] = from_f32<IO>(s.o[h].x * inv), out[128 * h + 1] = from_f32<IO>(s.o[h].y * inv);
+            out[128 * h + 2] = from_f32<IO>(s.o[h].z * inv), out[128 * h + 3] = from_f32<IO>(s.o[h].w * inv);
         }
         return;
     }
-    if (lane == 0) ml[warp] = make_float2(s.m, s.l);
+    // four parts side by side in a warp, joined by shuffles, then the warps
+    JoinSum<1> s;
+    s.add(j, pr, r, warp * 4 + lane / 8, W * 4, x);
 #pragma unroll
-    for (int h = 0; h < 2; h++)
-        if (128 * h + 4 * lane < j.d) *reinterpret_cast<float4 *>(&acc[warp][128 * h + 4 * lane]) = s.o[h];
+    for (int o = 8; o < 32; o <<= 1) {
+        s.rescale(fmaxf(s.m, __shfl_xor_sync(0xffffffffu, s.m, o)));
+        s.l += __shfl_xor_sync(0xffffffffu, s.l, o);
+        s.o[0].x += __shfl_xor_sync(0xffffffffu, s.o[0].x, o);
+        s.o[0].y += __shfl_xor_sync(0xffffffffu, s.o[0].y, o);
+        s.o[0].z += __shfl_xor_sync(0xffffffffu, s.o[0].z, o);
+        s.o[0].w += __shfl_xor_sync(0xffffffffu, s.o[0].w, o);
+    }
+    if (lane == 0) ml[warp] = make_float2(s.m, s.l);
+    if (lane < 8) *reinterpret_cast<float4 *>(&acc[warp][4 * lane]) = s.o[0];
     __syncthreads();
+    if (tid >= AJ_COLUMNS) return;
     float m = -INFINITY, l = 0.0f, v = 0.0f;
 #pragma unroll
     for (int w = 0; w < W; w++) m = fmaxf(m, ml[w].x);
@@ -136,10 +163,10 @@ template <typename IO> __global__ void __launch_bounds__(AJ_THREADS) attn_join_k
     for (int w = 0; w < W; w++) {
         const float f = exp2_fast(ml[w].x - ref);
         l += f * ml[w].y;
-        if (tid < j.d) v += f * acc[w][tid];
+        v += f * acc[w][tid];
     }
-    if (tid < j.d) out[tid] = from_f32<IO>(l > 0.0f || l != l ? v / l : 0.0f);
-    if (tid == 0) a.ml[(int64_t)b * a.H + kvh * a.G + g] = make_float2(m, l);
+    out[tid - x % AJ_COLUMNS] = from_f32<IO>(l > 0.0f || l != l ? v / l : 0.0f);
+    if (x == 0) *joined = make_float2(m, l);
 }
 
 constexpr int AW_HEADS = 128;  // heads whose maximum and sum are in shared memory at a time
@@ -354,7 +381,7 @@ extern "C" int ofb_attn_decode(const ofb_kv_cache *cache, const void *q, int typ
     e = launch_pdl(p.v.run, dim3(p.ctas), dim3(p.v.warps * 32), smem, s, a);
     if (e != cudaSuccess) return cuda_status(e, "ofb_attn_decode launch");
     if (p.ctas == 1 && !accumulate) return OFB_OK;  // every part is whole
-    const dim3 grid((unsigned)(n_seqs * (j.wide ? n_heads : a.KVH * a.NB * (p.rows / (AJ_THREADS / 32))))), block(AJ_THREADS);
+    const dim3 grid((unsigned)(n_seqs * (j.wide ? n_heads * (j.d / AJ_COLUMNS) : a.KVH * a.NB * (p.rows / (AJ_THREADS / 32))))), block(AJ_THREADS);
     e = type == OFB_TYPE_F32              ? launch_pdl(attn_join_kernel<float>, grid, block, 0, s, j)
         : cache->type == OFB_TYPE_BF16 ? launch_pdl(attn_join_kernel<__nv_bfloat16>, grid, block, 0, s, j)
                                        : launch_pdl(attn_join_kernel<__half>, grid, block, 0, s, j);
