@@ -13,7 +13,7 @@
 // Third launch, with `accumulate`: each entry's probability, summed over the query
 // heads of its kv head in their order, is added to the cache's weight, four
 // entries per thread. It reads the scores the split kernel left (4 bytes per entry
-// and query head, an sixteenth of the entry's K and V at 8 heads of 128; forming them
+// and query head, a sixteenth of the entry's K and V at 8 heads of 128; forming them
 // again would read all of K a second time). Of 176 us for 48 ragged sequences, 32 heads
 // over 8 kv heads of 128, the scores' way through HBM takes some 15 and this launch
 // 10. Asking L2 to keep them, whole lines per store, or weights and join in one launch

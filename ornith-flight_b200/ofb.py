@@ -324,8 +324,9 @@ def rope(x: torch.Tensor, pos: torch.Tensor, cfg: RopeConfig, out: torch.Tensor 
     if _away(dev, stream):
         return _elsewhere(dev, stream, rope, x, pos, cfg, out)
     if out is None:
-        out = x.new_empty(shape)
-    os_ = _rows(out, shape, dt, dev, "rope: out")
+        out, os_ = x.new_empty(shape), H * d
+    else:
+        os_ = _rows(out, shape, dt, dev, "rope: out")
     _check(lib.ofb_rope(ctypes.byref(cfg), x.data_ptr(), _TYPE_OF[dt], T, H, d, xs, p, T, out.data_ptr(), os_,
                         _raw_stream(dev.index)))
     return out
@@ -359,8 +360,9 @@ def rope_append(cache: KvCache, k: torch.Tensor, v: torch.Tensor, seq: torch.Ten
         q_out = None
     else:
         if q_out is None:
-            q_out = q.new_empty((T, H, d))
-        os_ = _rows(q_out, (T, H, d), dt, dev, "rope_append: q_out")
+            q_out, os_ = q.new_empty((T, H, d)), H * d
+        else:
+            os_ = _rows(q_out, (T, H, d), dt, dev, "rope_append: q_out")
     _check(lib.ofb_rope_append(cache._ref, None if rope is None else ctypes.byref(rope), _TYPE_OF[dt], T, H, _ptr(q), qs,
                                k.data_ptr(), ks, v.data_ptr(), vs, pp, T, sp, ip, np_, _ptr(q_out), os_,
                                _raw_stream(dev.index)))
@@ -400,8 +402,9 @@ def attn_decode(cache: KvCache, q: torch.Tensor, lens: torch.Tensor, scale: floa
     elif scratch.device != dev or not scratch.is_contiguous():
         raise OfbError(EINVAL, "attn_decode: scratch must be contiguous beside the cache")
     if out is None:
-        out = q.new_empty(shape)
-    os_ = _rows(out, shape, dt, dev, "attn_decode: out")
+        out, os_ = q.new_empty(shape), H * d
+    else:
+        os_ = _rows(out, shape, dt, dev, "attn_decode: out")
     _check(lib.ofb_attn_decode(cache._ref, q.data_ptr(), _TYPE_OF[dt], qs, H, d ** -0.5 if scale is None else scale, lp, B,
                                max_len, int(accumulate), out.data_ptr(), os_, scratch.data_ptr(), scratch.nbytes,
                                _raw_stream(dev.index)))
@@ -433,11 +436,14 @@ def kv_evict(cache: KvCache, lens: torch.Tensor, keep: int, recent: int = 0, max
     shape = (B, cache.n_kv_heads, keep)
     if kept is None:
         kept = lens.new_empty(shape)
+    else:
+        _ints(kept, shape, dev, "kv_evict: kept")
     if lens_out is None:
         lens_out = lens.new_empty(B)
-    _check(lib.ofb_kv_evict(cache._ref, lp, B, max_len, keep, recent, _ints(lens_out, (B,), dev, "kv_evict: lens_out"),
-                            _ints(kept, shape, dev, "kv_evict: kept"), scratch.data_ptr(), scratch.nbytes,
-                            _raw_stream(dev.index)))
+    else:
+        _ints(lens_out, (B,), dev, "kv_evict: lens_out")
+    _check(lib.ofb_kv_evict(cache._ref, lp, B, max_len, keep, recent, lens_out.data_ptr(), kept.data_ptr(),
+                            scratch.data_ptr(), scratch.nbytes, _raw_stream(dev.index)))
     return kept, lens_out
 
 
