@@ -290,8 +290,9 @@ __global__ void __launch_bounds__(AttnShape<D, AttnQuery<D, R, CT, IO>::QB>::THR
         if (a.lens[first.b] > a.max_len && first.vh == 0 && rank == 0 && tid == 0) report(a.errors, OFB_CACHE_ELEN);
         first.len = attn_len(a, first.b);
         first.nt = (first.len + ATT_TILE - 1) / ATT_TILE;
-        first.t = (int)((int64_t)rank * first.nt / C);
-        first.end = (int)((int64_t)(rank + 1) * first.nt / C);
+        const int share = __ffs(C) - 1;  // (C is a power of two)
+        first.t = (int)((int64_t)rank * first.nt >> share);
+        first.end = (int)((int64_t)(rank + 1) * first.nt >> share);
         first.f_end = 1;
     } else {
         // places before each sequence; every CTA forms them for itself

@@ -32,7 +32,7 @@ struct RopeArgs {
     // first kernel: rows of a CTA under way, CTAs that share a group's rows
     int slots, split;
     int n_pages, page_size, n_seqs, max_pages;
-    FastDiv page, rows, per_row;  // by page_size, by H + 2 KVH, by chunk pairs of a row
+    FastDiv page, rows, per_row, pairs;  // by page_size, by H + 2 KVH, by chunk pairs of a row, by rot / 2
     const void *q, *k, *v;
     void *q_out, *ck, *cv;
     int64_t qs, ks, vs, qos, page_stride, pos_stride;
@@ -92,7 +92,7 @@ __device__ __forceinline__ void rope_setup(const RopeArgs &a, int t0, int nt, co
     const uint8_t *axis = a.axis;
     asm("" : "+l"(freq), "+l"(axis));
     for (int i = threadIdx.x; i < nt * pairs; i += RP_THREADS) {
-        const int t = i / pairs, p = i - t * pairs;
+        const int t = a.pairs.div(i), p = i - t * pairs;
         const float2 cs = rope_angle(a.pos[axis[p] * a.pos_stride + t0 + t], freq[p]);
         sh.c[i] = cs.x;
         sh.s[i] = cs.y;
@@ -150,10 +150,12 @@ template <typename IO> struct RopeRaw {
 // slot, slot + slots, ...: it asks for its first three (f32: two) items at once;
 // while they are on their way the last threads find the tokens' places in the cache
 // and the first ones form the cosines, so that the three waits are one. Measured on
-// 8190 tokens with 32 + 2 x 8 heads of 128, bf16: 39.5 us, 5.1 TB/s, where adding a
-// number to as many bytes takes 32 (16383 tokens x 16 heads alone: 24.4 and 21.7).
-// 8 CTAs per SM 39.8, 6 41.2, 4 items at once 43, 2 x 192 threads 42, 3 x 256 41;
-// CTAs that stay and ask for the next group's loads, positions and pages ahead 45.
+// 8190 tokens with 32 + 2 x 8 heads of 128, bf16: 38.7 us, 5.2 TB/s, where adding a
+// number to as many bytes takes 32 (16383 tokens x 16 heads alone: 23.9 and 21.7).
+// A plain division by the pairs where the cosines are formed cost 5% of that, with
+// all CTAs waiting on it: 40.5. Against 39.5 for 7 CTAs per SM then, 8 took 39.8, 6
+// 41.2, 4 items at once 43, 2 x 192 threads 42, 3 x 256 41; CTAs that stay and ask for
+// the next group's loads, positions and pages ahead 45.
 constexpr int RV_THREADS = 128, RV_CTAS = 7;  // CTAs per SM that registers allow
 template <typename IO> constexpr int RV_BATCH = sizeof(IO) == 2 ? 3 : 2;  // items asked for at once
 template <typename IO, typename CT, bool ADJ, bool CACHE>
@@ -198,8 +200,9 @@ __global__ void __launch_bounds__(RV_THREADS, RV_CTAS) rope_vec_kernel(const __g
         const uint64_t *freq = a.turns;  // see rope_setup
         const uint8_t *axis = a.axis;
         asm("" : "+l"(freq), "+l"(axis));
+#pragma unroll 1
         for (int i = tid; i < nt * half; i += RV_THREADS) {
-            const int t = a.tpb == 1 ? 0 : i / half, p = i - t * half;
+            const int t = a.pairs.div(i), p = i - t * half;
             const float2 cs = rope_angle(a.pos[axis[p] * a.pos_stride + t0 + t], freq[p]);
             cosines[i] = cs.x;
             sines[i] = cs.y;
@@ -360,6 +363,7 @@ template <typename IO, typename CT> static cudaError_t rope_launch(RopeArgs &a, 
     a.rows = fast_div(rows);
     a.page = fast_div(a.page_size ? a.page_size : 1);
     a.per_row = fast_div(vec ? a.d / 16 : 1);
+    a.pairs = fast_div(a.rot ? a.rot / 2 : 1);
     a.slots = RV_THREADS / (int)a.per_row.d;
     // few tokens with many rows: several CTAs share a token's rows
     const int groups = (a.T + tpb - 1) / tpb, batches = (tpb * rows + a.slots * RV_BATCH<IO> - 1) / (a.slots * RV_BATCH<IO>);
