@@ -28,7 +28,8 @@ constexpr int AJ_CHUNK = 4 * AJ_THREADS;  // entries of one weight CTA
 
 struct AttnJoinArgs {
     AttnArgs a;
-    int ctas, warps, rows, d; // of the split kernel: CTAs, warps of each, heads per pass; head_dim
+    int warps, rows, d;       // of the split kernel: warps of a CTA, heads per pass (8 or 16); head_dim
+    FastDiv group;            // by G
     int wide, chunks;         // one head per CTA; weight CTAs per (sequence, kv head)
 };
 
@@ -41,7 +42,7 @@ struct PartRange {
 __device__ __forceinline__ PartRange part_range(const AttnJoinArgs &j, int b, int vh, int nt) {
     const int nvh = j.a.KVH * j.a.NB, places = nt + ATT_PART;
     PartRange r;
-    r.sp = AttnSplit::make(j.a.prefix[j.a.B] * nvh, j.ctas, j.warps);
+    r.sp = AttnSplit::make(j.a.prefix[j.a.B] * nvh, j.a.ctas, j.warps);
     r.f0 = j.a.prefix[b] * nvh + vh * places;
     r.c0 = (r.f0 + ATT_PART) / r.sp.run;
     r.n = (r.f0 + places - 1) / r.sp.run - r.c0 + 1;
@@ -106,21 +107,21 @@ template <typename IO> __global__ void __launch_bounds__(AJ_THREADS) attn_join_k
     __shared__ float2 ml[W];
     const AttnArgs &a = j.a;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    pdl_wait();
-    pdl_trigger();
-    int b, vh, r, x;
+    // grid: wide: head, columns, sequence; else eight heads, -, sequence
+    const int b = blockIdx.z, shift = j.rows == 16 ? 4 : 3;
+    int kvh, g, x;
     if (j.wide) {
-        const int pieces = j.d / AJ_COLUMNS, u = blockIdx.x / pieces;
-        x = (blockIdx.x - u * pieces) * AJ_COLUMNS + lane % 8 * 4;
-        b = u / a.H;
-        const int h = u - b * a.H, kvh = h / a.G, g = h - kvh * a.G;
-        vh = kvh * a.NB + g / j.rows, r = g % j.rows;
+        kvh = j.group.div(blockIdx.x), g = (int)blockIdx.x - kvh * a.G;
+        x = blockIdx.y * AJ_COLUMNS + lane % 8 * 4;
     } else {
-        const int u = blockIdx.x / (j.rows / W);  // 8 rows per CTA
-        b = u / (a.KVH * a.NB), vh = u - b * a.KVH * a.NB, r = (blockIdx.x - u * (j.rows / W)) * W + warp;
+        const int vh = blockIdx.x * W >> shift;
+        kvh = a.NB == 1 ? vh : vh / a.NB, g = blockIdx.x * W + warp - (kvh * a.NB << shift);
         x = 4 * lane;
     }
-    const int kvh = vh / a.NB, g = (vh - kvh * a.NB) * j.rows + r, nt = a.prefix[b + 1] - a.prefix[b] - ATT_PART;
+    const int vh = kvh * a.NB + (g >> shift), r = g & (j.rows - 1);
+    pdl_wait();
+    pdl_trigger();
+    const int nt = a.prefix[b + 1] - a.prefix[b] - ATT_PART;
     if (nt < 0) return;
     const PartRange pr = part_range(j, b, vh, nt);
     if (pr.n == 1 || g >= a.G) return;  // (`wide`: the CTA's only head, so all leave)
@@ -348,7 +349,7 @@ extern "C" int ofb_attn_decode(const ofb_kv_cache *cache, const void *q, int typ
     a.page_stride = cache_page_stride(cache), a.q_stride = q_stride, a.out_stride = out_stride;
     a.B = n_seqs, a.KVH = cache->n_kv_heads, a.G = n_heads / a.KVH, a.NB = p.NB, a.H = n_heads;
     a.page_size = cache->page_size, a.max_pages = cache->max_pages, a.n_pages = cache->n_pages, a.max_len = p.max_len;
-    a.page = fast_div(a.page_size), a.halves = a.page_size % 16 == 0;
+    a.page = fast_div(a.page_size), a.ctas = fast_div(p.ctas), a.halves = a.page_size % 16 == 0;
     a.scale = scale * 1.4426950408889634f;
     a.errors = cache->errors;
     a.prefix = reinterpret_cast<int *>(w + p.prefix), a.ml = reinterpret_cast<float2 *>(w + p.ml);
@@ -356,7 +357,7 @@ extern "C" int ofb_attn_decode(const ofb_kv_cache *cache, const void *q, int typ
     a.z = accumulate ? reinterpret_cast<float *>(w + p.z) : nullptr;
     a.z_stride = p.z_stride, a.weight = cache->weight;
     a.quads = a.page_size % 4 == 0 && !misaligned(a.weight, 16);
-    j.ctas = p.ctas, j.warps = p.v.warps, j.rows = p.rows, j.d = cache->head_dim;
+    j.group = fast_div(a.G), j.warps = p.v.warps, j.rows = p.rows, j.d = cache->head_dim;
     // parts of a head, about, when all sequences are of the largest length
     j.wide = p.ctas >= 4 * n_seqs * a.KVH * a.NB;
     j.chunks = (p.max_len + AJ_CHUNK - 1) / AJ_CHUNK;
@@ -381,7 +382,7 @@ extern "C" int ofb_attn_decode(const ofb_kv_cache *cache, const void *q, int typ
     e = launch_pdl(p.v.run, dim3(p.ctas), dim3(p.v.warps * 32), smem, s, a);
     if (e != cudaSuccess) return cuda_status(e, "ofb_attn_decode launch");
     if (p.ctas == 1 && !accumulate) return OFB_OK;  // every part is whole
-    const dim3 grid((unsigned)(n_seqs * (j.wide ? n_heads * (j.d / AJ_COLUMNS) : a.KVH * a.NB * (p.rows / (AJ_THREADS / 32))))), block(AJ_THREADS);
+    const dim3 block(AJ_THREADS), grid = j.wide ? dim3(n_heads, j.d / AJ_COLUMNS, n_seqs) : dim3(a.KVH * a.NB * p.rows / (AJ_THREADS / 32), 1, n_seqs);
     e = type == OFB_TYPE_F32              ? launch_pdl(attn_join_kernel<float>, grid, block, 0, s, j)
         : cache->type == OFB_TYPE_BF16 ? launch_pdl(attn_join_kernel<__nv_bfloat16>, grid, block, 0, s, j)
                                        : launch_pdl(attn_join_kernel<__half>, grid, block, 0, s, j);

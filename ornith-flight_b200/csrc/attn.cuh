@@ -86,6 +86,7 @@ struct AttnArgs {
     float *z;         // [B][H][z_stride] scores in log2, or NULL
     int64_t z_stride;
     float *weight;
+    FastDiv ctas;     // by the number of runs
 };
 
 __device__ __forceinline__ float exp2_fast(float x) {  // 2 steps at most; below 2^-126 it gives 0
@@ -104,8 +105,8 @@ __device__ __forceinline__ int attn_len(const AttnArgs &a, int b) { return min(m
 constexpr int ATT_PART = 8;
 struct AttnSplit {
     int total, run;
-    static __device__ __forceinline__ AttnSplit make(int total, int ctas, int warps) {
-        return {total, max(total / ctas + (total % ctas != 0), warps)};
+    static __device__ __forceinline__ AttnSplit make(int total, const FastDiv &ctas, int warps) {
+        return {total, max(ctas.div(total + (int)ctas.d - 1), warps)};
     }
     __device__ __forceinline__ int first(int id) const { return (int)min((int64_t)id * run, (int64_t)total); }
 };
@@ -326,7 +327,7 @@ __global__ void __launch_bounds__(AttnShape<D, AttnQuery<D, R, CT, IO>::QB>::THR
         for (int b = blockIdx.x; b < a.B; b += gridDim.x)
             if (prefix[b + 1] == prefix[b])
                 for (int i = tid; i < a.H * D; i += THREADS) static_cast<IO *>(a.out)[b * a.out_stride + i] = from_f32<IO>(0.0f);
-        const AttnSplit sp = AttnSplit::make(prefix[a.B] * nvh, (int)gridDim.x, W);
+        const AttnSplit sp = AttnSplit::make(prefix[a.B] * nvh, a.ctas, W);
         f0 = sp.first(blockIdx.x), f1 = sp.first(blockIdx.x + 1);
         if (f0 >= f1) return;
         first = attn_part(prefix, last, a.B, nvh, f0, f1);
