@@ -66,8 +66,8 @@ struct EvictArgs {
     uint32_t *errors;
     int64_t page_stride;
     FastDiv page, row2;  // by page_size; by the 16-byte chunks of a K and a V row
+    FastDiv kvh, slices; // by KVH; by the second launch's CTAs per row
     int KVH, d, page_size, n_pages, max_pages, max_len, keep, recent, chunk;
-    int slices;      // of a row's moves, the second launch's CTAs
     int kept_quads;  // keep is a multiple of 4 and kept 16-byte aligned
     int fused;       // rows are copied by this launch
     int order_kept;  // order numbers fit beside the keys (else they are read again)
@@ -142,6 +142,12 @@ __device__ __forceinline__ void evict_copy(const EvictArgs &a, int u, const Evic
     }
 }
 
+__device__ __forceinline__ uint32_t cluster_index() {  // blockIdx.x over the cluster's size
+    uint32_t i;
+    asm("mov.u32 %0, %%clusterid.x;" : "=r"(i));
+    return i;
+}
+
 // NT threads. QUAD: four consecutive entries lie in one page, 16-byte aligned.
 template <int NT, bool QUAD> __global__ void __launch_bounds__(NT, EV_THREADS / NT) evict_kernel(const __grid_constant__ EvictArgs a) {
     extern __shared__ __align__(16) int hist[];  // [2][EV_BINS], then keys, then order numbers
@@ -158,7 +164,7 @@ template <int NT, bool QUAD> __global__ void __launch_bounds__(NT, EV_THREADS / 
     const int C = (int)cl.num_blocks(), rank = (int)cl.block_rank();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     constexpr int nthr = NT, nwarp = NT / 32;
-    const int u = blockIdx.x / C, b = u / a.KVH, h = u - b * a.KVH;
+    const int u = (int)cluster_index(), b = a.kvh.div(u), h = u - b * a.KVH;
     // sum of x[w] over the warps before this one (x: one value per warp)
     auto warps_before = [&](const int *x) { return __reduce_add_sync(0xffffffffu, lane < warp ? x[lane] : 0); };
     auto sync_all = [&]() {
@@ -548,12 +554,12 @@ template <int NT, bool QUAD> __global__ void __launch_bounds__(NT, EV_THREADS / 
 // took 10 to 15% longer: what counts is rows under way at once.)
 constexpr int EV_MOVE_THREADS = 128;
 __global__ void __launch_bounds__(EV_MOVE_THREADS) evict_move_kernel(const __grid_constant__ EvictArgs a) {
+    const int u = a.slices.div(blockIdx.x), s = (int)(blockIdx.x - u * a.slices.d), lane = threadIdx.x & 31, b = a.kvh.div(u);
+    constexpr int EACH = EV_SLICE / (EV_MOVE_THREADS / 32);
+    const int m0 = s * EV_SLICE + (threadIdx.x >> 5) * EACH, k = min(m0 + lane, a.keep - 1);
     pdl_wait();
     pdl_trigger();
-    const int u = blockIdx.x / a.slices, s = blockIdx.x - u * a.slices, lane = threadIdx.x & 31, b = u / a.KVH;
-    constexpr int EACH = EV_SLICE / (EV_MOVE_THREADS / 32);
     // the lists are asked for beside the count: places behind the last move are not used
-    const int m0 = s * EV_SLICE + (threadIdx.x >> 5) * EACH, k = min(m0 + lane, a.keep - 1);
     const int32_t *list = a.lists + (int64_t)u * 2 * a.keep;
     const int moves = a.counts[u];
     EvictMove mv;
@@ -652,8 +658,9 @@ extern "C" int ofb_kv_evict(const ofb_kv_cache *cache, const int32_t *lens, int 
     const int most = bound <= keep ? 0 : bound - keep < keep ? bound - keep : keep;  // moves of a row
     a.kept_quads = keep % 4 == 0 && !misaligned(kept, 16);
     a.fused = most <= EV_FUSED;
-    a.slices = (most + EV_SLICE - 1) / EV_SLICE;
-    if (!a.fused && rows * a.slices > INT32_MAX) { set_error("ofb_kv_evict: too many moves"); return OFB_ETOOLARGE; }
+    const int slices = (most + EV_SLICE - 1) / EV_SLICE;
+    a.slices = fast_div(slices > 1 ? slices : 1), a.kvh = fast_div(a.KVH);
+    if (!a.fused && rows * slices > INT32_MAX) { set_error("ofb_kv_evict: too many moves"); return OFB_ETOOLARGE; }
     int C, threads = 256;
     evict_shape((int)rows, bound, C, threads);
     a.chunk = ((bound + C - 1) / C + 3) / 4 * 4;  // runs of the CTAs start at a multiple of 4
@@ -676,6 +683,6 @@ extern "C" int ofb_kv_evict(const ofb_kv_cache *cache, const int32_t *lens, int 
     if (e != cudaSuccess) return cuda_status(e, "ofb_kv_evict smem attribute");
     e = launch_pdl_cluster(kernel, dim3((unsigned)(rows * C)), dim3(threads), C, smem, static_cast<cudaStream_t>(stream), a);
     if (e == cudaSuccess && !a.fused)
-        e = launch_pdl(evict_move_kernel, dim3((unsigned)(rows * a.slices)), dim3(EV_MOVE_THREADS), 0, static_cast<cudaStream_t>(stream), a);
+        e = launch_pdl(evict_move_kernel, dim3((unsigned)(rows * slices)), dim3(EV_MOVE_THREADS), 0, static_cast<cudaStream_t>(stream), a);
     return e == cudaSuccess ? OFB_OK : cuda_status(e, "ofb_kv_evict launch");
 }
