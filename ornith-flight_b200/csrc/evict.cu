@@ -176,6 +176,18 @@ template <int NT, bool QUAD> __global__ void __launch_bounds__(NT, EV_THREADS / 
     pdl_wait();
     pdl_trigger();
 
+    // page numbers of the first entries, asked for beside the length, and then always
+    // those of the next ones (2 rows of 1040 8.55 -> 8.3 us, 24 of 131072 70.9 -> 70.5)
+    constexpr int V = QUAD ? 4 : 1, UN = QUAD ? 3 : 8;  // entries read together, groups in flight
+    const int32_t *table = a.table + (int64_t)b * a.max_pages;
+    const int start = rank * a.chunk;
+    int page[UN];
+    auto look_up = [&](int base, int end) {
+#pragma unroll
+        for (int k = 0; k < UN; k++)
+            if (base + k * nthr * V < end) page[k] = table[a.page.div(start + base + k * nthr * V)];
+    };
+    look_up(tid * V, min(a.chunk, a.max_len - start));
     const int raw = a.lens[b], n = min(max(raw, 0), a.max_len), K = a.keep, n_out = min(n, K);
     if (rank == 0 && tid == 0) {
         if (raw > a.max_len) report(a.errors, OFB_CACHE_ELEN);
@@ -188,29 +200,24 @@ template <int NT, bool QUAD> __global__ void __launch_bounds__(NT, EV_THREADS / 
         if (rank == 0 && tid == 0) a.counts[u] = 0;
         return;
     }
-    const int32_t *table = a.table + (int64_t)b * a.max_pages;
     // row of entry i in page p (-1: no such page) among all rows [n_pages][KVH][page_size]
     auto row_of = [&](int i, int p) {
         if (p < 0 || p >= a.n_pages) return -1;
         return (p * a.KVH + h) * a.page_size + (i - a.page.div(i) * a.page_size);
     };
-    const int i0 = min(rank * a.chunk, n), i1 = min(i0 + a.chunk, n), m = i1 - i0;
+    const int i0 = min(start, n), i1 = min(i0 + a.chunk, n), m = i1 - i0;
 
     __syncthreads();
     constexpr uint32_t ZERO = 0x80000000u, INF = 0xff800000u;  // keys of 0 and of infinity
-    constexpr int V = QUAD ? 4 : 1, UN = QUAD ? 3 : 8;         // entries read together, groups in flight
     int top = INT32_MIN;
     uint32_t low = 0xffffffffu, high = 0u;
     for (int base = tid * V; base < m; base += UN * nthr * V) {
         int e[UN], o[UN][V];
         float w[UN][V];
 #pragma unroll
-        for (int k = 0; k < UN; k++)
-            if (base + k * nthr * V < m) e[k] = table[a.page.div(i0 + base + k * nthr * V)];
-#pragma unroll
         for (int k = 0; k < UN; k++) {
             const int i = base + k * nthr * V;
-            e[k] = i < m ? row_of(i0 + i, e[k]) : -1;
+            e[k] = i < m ? row_of(i0 + i, page[k]) : -1;
             if (e[k] < 0) continue;
             if constexpr (QUAD) {  // (what lies behind the last entry is read with it, and not used)
                 *reinterpret_cast<float4 *>(w[k]) = *reinterpret_cast<const float4 *>(a.weight + e[k]);
@@ -220,6 +227,7 @@ template <int NT, bool QUAD> __global__ void __launch_bounds__(NT, EV_THREADS / 
                 if (a.recent) o[k][0] = a.order[e[k]];
             }
         }
+        look_up(base + UN * nthr * V, m);
 #pragma unroll
         for (int k = 0; k < UN; k++) {
             const int i = base + k * nthr * V;
