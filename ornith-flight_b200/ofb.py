@@ -307,7 +307,8 @@ class KvCache:
 
     def device_errors(self) -> int:
         """CACHE_E* bits that calls on this cache have met since the last call
-        (0: none). Waits for the device."""
+        (0: none). Waits for the current stream; work on the cache on other
+        streams has to be waited for before."""
         bits = int(self.errors.item())
         self.errors.zero_()
         return bits

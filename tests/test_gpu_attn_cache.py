@@ -178,6 +178,21 @@ def test_attention(ofb, cuda, cache, kv, G, d, page, lens, acc, io):
     assert c.handle.device_errors() == 0
 
 
+@pytest.mark.parametrize("io", ["f32", "own"])
+@pytest.mark.parametrize("d,G,page,cache", [(64, 3, 16, "bf16"), (96, 12, 20, "f16"), (128, 20, 64, "bf16"), (192, 9, 5, "f16"), (256, 4, 32, "bf16")])
+def test_attention_joins_many_parts(ofb, cuda, d, G, page, cache, io):
+    # one long sequence among short ones: its parts lie in most of the runs
+    lens = [7, 30011, 0, 2600]
+    io = cache if io == "own" else io
+    c = Cache(ofb, lens, 1, d, page, cache, seed=G, meta=True)
+    q = (torch.randn(len(lens), G, d, generator=torch.Generator().manual_seed(d)) * 2).to(DT[io]).to(cuda)
+    before = c.weight.clone()
+    check_attention(c, q, ofb.attn_decode(c.handle, q, c.dlens, accumulate=True), io, d ** -0.5, before)
+    one = Cache(ofb, lens[1:2], 2, d, page, cache, seed=G + 1)
+    q = q[:1].repeat(1, 2, 1)
+    check_attention(one, q, ofb.attn_decode(one.handle, q, one.dlens), io, d ** -0.5)
+
+
 def test_attention_many_sequences(ofb, cuda):
     rng = np.random.default_rng(3)
     lens = rng.integers(0, 90, size=1100).tolist()
