@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(AJ_THREADS) attn_weight_kernel(const __grid_co
 
 // Tiles per warp up to which a sequence is left to a cluster: 2 heads of 16 over one
 // sequence of 1500 entries (two tiles) 7.9 us, as runs and a join 8.6; of 2500 10.9
-// and 9.3. CTAs of one warp, up to 4 tiles: 64 x 8 kv heads of 100 entries with
+// and 9.2. CTAs of one warp, up to 4 tiles: 64 x 8 kv heads of 100 entries with
 // weights 18.0 us against 21.7, 95 x 3 of 15 entries (256) 12.4 against 27.7.
 constexpr int ATT_SHORT = 3, ATT_ONE_WARP = 4;
 

@@ -25,7 +25,7 @@
 //    the CTA and one exchange over the cluster.
 // 4. The k-th hole and the k-th spare meet in the scratch and rows are copied,
 //    4 KB in flight per warp: by the same cluster where few rows can move, else
-//    by a second launch whose CTAs take 64 moves each, since one (sequence, kv
+//    by a second launch whose CTAs take 16 or 32 moves each, since one (sequence, kv
 //    head) has many more than another.
 //
 // A CTA's steps wait on each other, so what counts is that all CTAs run at
@@ -42,10 +42,16 @@ constexpr int EV_THREADS = 1024;  // at most
 constexpr int EV_WARPS = EV_THREADS / 32;
 constexpr int EV_CLUSTER = 8;   // CTAs of a cluster at most
 constexpr int EV_BINS = 1024;
-constexpr int EV_SLICE = 64;    // moves of one CTA of the second launch
-// moves per row that may be, up to which there is no second launch: 2 rows of 1100
-// entries down to 1024 take 10.4 us without and 11.4 with it, of 1536 16.2 and 12.2
-constexpr int EV_FUSED = 128;
+// moves of one CTA of the second launch: 32, or 16 where so short ones have room at
+// once, EV_ROOM per SM (8 rows of 32000, 4000 moves each: 24.6 us with 32, 26.1 with
+// 16, 27.1 with 64; 2 rows of 2000, 250 moves each: 11.2, 10.8 and 12.2; 512 rows of up
+// to 512 moves: 40.9, 45.4 and 41.0; 24 rows of 8192: 71.4, 76.3 and 70.8)
+constexpr int EV_SLICE = 32, EV_ROOM = 8;
+// moves per row that may be, up to which there is no second launch: 48 with up to
+// EV_FEW rows, whose clusters leave most of the GPU idle, else 128 (8 rows of 1072
+// entries down to 1024 take 9.6 us without and 9.8 with it, of 4160 to 4096 14.4 and
+// 13.1; 128 rows of 1152 to 1024 11.9 and 13.6)
+constexpr int EV_FUSED_FEW = 48, EV_FUSED = 128, EV_FEW = 64;
 // entries per CTA from which a cluster is worth its barriers: 2 rows of 8000 take
 // 17.2 us with one CTA each and 20.1 with seven, of 16000 19.3 with three and 22.1
 // with one
@@ -67,6 +73,7 @@ struct EvictArgs {
     int64_t page_stride;
     FastDiv page, row2;  // by page_size; by the 16-byte chunks of a K and a V row
     FastDiv kvh, slices; // by KVH; by the second launch's CTAs per row
+    int slice;           // moves of such a CTA
     int KVH, d, page_size, n_pages, max_pages, max_len, keep, recent, chunk;
     int kept_quads;  // keep is a multiple of 4 and kept 16-byte aligned
     int fused;       // rows are copied by this launch
@@ -557,14 +564,14 @@ template <int NT, bool QUAD> __global__ void __launch_bounds__(NT, EV_THREADS / 
     }
 }
 
-// The second launch: CTA (row, slice) makes moves EV_SLICE * slice and on.
+// The second launch: CTA (row, s) makes moves slice * s and on.
 // (Warps that go round over slices, looking the next ones up while they copy,
 // took 10 to 15% longer: what counts is rows under way at once.)
 constexpr int EV_MOVE_THREADS = 128;
 __global__ void __launch_bounds__(EV_MOVE_THREADS) evict_move_kernel(const __grid_constant__ EvictArgs a) {
     const int u = a.slices.div(blockIdx.x), s = (int)(blockIdx.x - u * a.slices.d), lane = threadIdx.x & 31, b = a.kvh.div(u);
-    constexpr int EACH = EV_SLICE / (EV_MOVE_THREADS / 32);
-    const int m0 = s * EV_SLICE + (threadIdx.x >> 5) * EACH, k = min(m0 + lane, a.keep - 1);
+    const int each = a.slice / (EV_MOVE_THREADS / 32);
+    const int m0 = s * a.slice + (threadIdx.x >> 5) * each, k = min(m0 + lane, a.keep - 1);
     pdl_wait();
     pdl_trigger();
     // the lists are asked for beside the count: places behind the last move are not used
@@ -573,7 +580,7 @@ __global__ void __launch_bounds__(EV_MOVE_THREADS) evict_move_kernel(const __gri
     EvictMove mv;
     mv.hole = list[k], mv.spare = list[a.keep + k];
     if (m0 >= moves) return;
-    const int cnt = min(EACH, moves - m0);
+    const int cnt = min(each, moves - m0);
     mv.pages(a, b, lane < cnt);
     mv.rows(a, u - b * a.KVH);
     evict_copy(a, u, mv, cnt, lane);
@@ -665,8 +672,9 @@ extern "C" int ofb_kv_evict(const ofb_kv_cache *cache, const int32_t *lens, int 
     a.counts = a.lists + rows * 2 * keep;
     const int most = bound <= keep ? 0 : bound - keep < keep ? bound - keep : keep;  // moves of a row
     a.kept_quads = keep % 4 == 0 && !misaligned(kept, 16);
-    a.fused = most <= EV_FUSED;
-    const int slices = (most + EV_SLICE - 1) / EV_SLICE;
+    a.fused = most <= (rows <= EV_FEW ? EV_FUSED_FEW : EV_FUSED);
+    a.slice = rows * ((most + EV_SLICE / 2 - 1) / (EV_SLICE / 2)) <= EV_ROOM * sm_count() ? EV_SLICE / 2 : EV_SLICE;
+    const int slices = (most + a.slice - 1) / a.slice;
     a.slices = fast_div(slices > 1 ? slices : 1), a.kvh = fast_div(a.KVH);
     if (!a.fused && rows * slices > INT32_MAX) { set_error("ofb_kv_evict: too many moves"); return OFB_ETOOLARGE; }
     int C, threads = 256;

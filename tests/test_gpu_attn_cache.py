@@ -335,6 +335,13 @@ def test_eviction(ofb, cuda, cache, kv, d, page, lens, keep, recent):
     assert c.handle.device_errors() == 0
 
 
+@pytest.mark.parametrize("seqs,more", [(1, 47), (2, 48), (2, 49), (33, 48), (33, 49), (33, 128), (33, 129), (40, 600)])
+def test_eviction_copies_in_either_launch(ofb, cuda, seqs, more):
+    # few and many rows, with moves up to and past where a second launch makes them
+    lens = [700 + more - i % 5 for i in range(seqs)]
+    check_eviction(ofb, Cache(ofb, lens, 2, 64, 16, "f16", seed=more, reach=700 + more, meta=True), 700, 30, max_len=700 + more)
+
+
 def test_eviction_ties_nan_and_zeros(ofb, cuda):
     # equal weights go to the lower place, across the CTAs of a cluster; NaN is lightest, -0 is 0
     c = Cache(ofb, [9000, 9000, 300], 2, 64, 16, meta=True)
