@@ -663,7 +663,7 @@ __global__ void __launch_bounds__(AttnShape<D, AttnQuery<D, R, CT, IO>::QB>::THR
                 dst[2] = from_f32<IO>(acc.z * inv), dst[3] = from_f32<IO>(acc.w * inv);
                 if (x == 0) {
                     if (CLUSTER) cml[r] = make_float2(ref, inv * PSCALE);
-                    else a.ml[(int64_t)p.b * a.H + head] = make_float2(mm, ll);
+                    if (!CLUSTER || a.NB > 1) a.ml[(int64_t)p.b * a.H + head] = make_float2(mm, ll);
                 }
             } else {
                 const float u = 1.0f / PSCALE;
@@ -700,16 +700,19 @@ __global__ void __launch_bounds__(AttnShape<D, AttnQuery<D, R, CT, IO>::QB>::THR
                 dst[0] = from_f32<IO>(acc.x * inv), dst[1] = from_f32<IO>(acc.y * inv);
                 dst[2] = from_f32<IO>(acc.z * inv), dst[3] = from_f32<IO>(acc.w * inv);
             }
-            if (a.z) {  // one pass per kv head here: this CTA's entries are its own
+            // weights: with one pass per kv head this CTA's entries are its own; with more
+            // a launch of its own adds them (attn.cu)
+            if (a.z) {
                 if (C > 1 && tid < rows) {
                     float mm = -INFINITY, ll = 0.0f;
                     for (int c = 0; c < C; c++) mm = fmaxf(mm, all_ml[c][tid].x);
                     const float ref = mm == -INFINITY ? 0.0f : mm;
                     for (int c = 0; c < C; c++) ll += exp2_fast(all_ml[c][tid].x - ref) * all_ml[c][tid].y;
                     cml[tid] = make_float2(ref, ll > 0.0f || ll != ll ? 1.0f / ll : 0.0f);
+                    if (a.NB > 1 && rank == 0) a.ml[(int64_t)p.b * a.H + kvh * a.G + h0 + tid] = make_float2(mm, ll);
                 }
                 __syncthreads();
-                const int i1 = min(p.end * ATT_TILE, p.len);
+                const int i1 = a.NB > 1 ? 0 : min(p.end * ATT_TILE, p.len);
                 for (int i = p.t * ATT_TILE + tid; i < i1; i += THREADS) {
                     const float *z = a.z + ((int64_t)p.b * a.H + kvh * a.G) * a.z_stride + i;
                     float add = 0.0f;

@@ -193,6 +193,16 @@ def test_attention_joins_many_parts(ofb, cuda, d, G, page, cache, io):
     check_attention(one, q, ofb.attn_decode(one.handle, q, one.dlens), io, d ** -0.5)
 
 
+@pytest.mark.parametrize("kv,G,d,lens", [(1, 16, 256, [300]), (2, 20, 128, [100, 0, 31, 1]), (3, 16, 256, [9, 13] * 40),
+                                         (1, 40, 64, [700]), (2, 24, 192, [60] * 90)])
+def test_attention_weights_of_short_sequences_in_passes(ofb, cuda, kv, G, d, lens):
+    # more query heads per kv head than a pass has: clusters of one and more CTAs, CTAs of one warp
+    c = Cache(ofb, lens, kv, d, 16, "bf16", seed=G, meta=True)
+    q = torch.randn(len(lens), kv * G, d, generator=torch.Generator().manual_seed(d)).to(cuda)
+    before = c.weight.clone()
+    check_attention(c, q, ofb.attn_decode(c.handle, q, c.dlens, accumulate=True), "f32", d ** -0.5, before)
+
+
 def test_attention_many_sequences(ofb, cuda):
     rng = np.random.default_rng(3)
     lens = rng.integers(0, 90, size=1100).tolist()
