@@ -10,7 +10,8 @@
 // 30.7 us in all, with all columns in one CTA 33.1); where it has few, a CTA takes
 // eight heads of a kv head, a warp each.
 //
-// Third launch, with `accumulate`: each entry's probability, summed over the query
+// Third launch, with `accumulate` (the second behind clusters of several passes; with
+// one pass they do it themselves): each entry's probability, summed over the query
 // heads of its kv head in their order, is added to the cache's weight, four
 // entries per thread. It reads the scores the split kernel left (4 bytes per entry
 // and query head, a sixteenth of the entry's K and V at 8 heads of 128; forming them
