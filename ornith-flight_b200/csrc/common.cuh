@@ -107,11 +107,13 @@ __device__ __forceinline__ uint16_t ld_u16(const uint8_t *p) {
 
 // Raises a kernel's dynamic shared-memory limit to `bytes` on the current
 // device (function attributes are per device); `cache` remembers, per
-// device, the largest value already set.
+// device, the largest value already set. `fixed`: bytes of the kernel's static
+// arrays at most. They count against the 48 KB that need no raised limit, and
+// against all that a CTA can have, but are not part of the limit that is set.
 template <typename... KArgs>
-inline cudaError_t ensure_dyn_smem(void (*kernel)(KArgs...), size_t bytes, size_t (&cache)[64]) {
+inline cudaError_t ensure_dyn_smem(void (*kernel)(KArgs...), size_t bytes, size_t (&cache)[64], size_t fixed = 0) {
     const int dev = current_device();
-    if (bytes <= 48 * 1024 || bytes <= cache[dev]) return cudaSuccess;
+    if (bytes + fixed <= 48 * 1024 || bytes <= cache[dev]) return cudaSuccess;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     if (e == cudaSuccess) cache[dev] = bytes;
     return e;

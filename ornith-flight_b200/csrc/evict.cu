@@ -681,7 +681,8 @@ extern "C" int ofb_kv_evict(const ofb_kv_cache *cache, const int32_t *lens, int 
     evict_shape((int)rows, bound, C, threads);
     a.chunk = ((bound + C - 1) / C + 3) / 4 * 4;  // runs of the CTAs start at a multiple of 4
     a.row2 = fast_div(2 * (a.d / 8));
-    // order numbers stay in shared memory where that leaves room for the SM's other CTAs
+    // order numbers stay in shared memory where that leaves room for the SM's other CTAs (one
+    // CTA of 1024 threads: 227328 bytes and the static arrays, the 227 KB that a CTA can have)
     size_t smem = (size_t)(2 * EV_BINS + 2 * a.chunk) * 4;
     a.order_kept = recent > 0 && (smem + EV_STATIC + 1024) * (1024 / threads) <= 228 * 1024;
     if (!a.order_kept) smem = (size_t)(2 * EV_BINS + a.chunk) * 4;
@@ -694,8 +695,7 @@ extern "C" int ofb_kv_evict(const ofb_kv_cache *cache, const int32_t *lens, int 
                         : vi == 4 ? evict_kernel<1024, false>
                                   : evict_kernel<1024, true>;
     static size_t attr[6][64];
-    // with room for the kernel's static arrays, which count against the default limit too
-    cudaError_t e = ensure_dyn_smem(kernel, smem + EV_STATIC, attr[vi]);
+    cudaError_t e = ensure_dyn_smem(kernel, smem, attr[vi], EV_STATIC);
     if (e != cudaSuccess) return cuda_status(e, "ofb_kv_evict smem attribute");
     e = launch_pdl_cluster(kernel, dim3((unsigned)(rows * C)), dim3(threads), C, smem, static_cast<cudaStream_t>(stream), a);
     if (e == cudaSuccess && !a.fused)
