@@ -16,6 +16,7 @@ void set_error(const char *fmt, ...) {
 }
 
 int cuda_status(cudaError_t e, const char *what) {
+    cudaGetLastError();  // reported here: the runtime would give it to the next launch check, too
     set_error("%s: %s (%s)", what, cudaGetErrorName(e), cudaGetErrorString(e));
     return e == cudaErrorMemoryAllocation ? OFB_ENOMEM : OFB_ECUDA;
 }
