@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <stdint.h>
 
+#include <mutex>
+
 #include "ornith_moe.h"
 
 #define OFB_STR2(x) #x
@@ -113,9 +115,12 @@ __device__ __forceinline__ uint16_t ld_u16(const uint8_t *p) {
 template <typename... KArgs>
 inline cudaError_t ensure_dyn_smem(void (*kernel)(KArgs...), size_t bytes, size_t (&cache)[64], size_t fixed = 0) {
     const int dev = current_device();
-    if (bytes + fixed <= 48 * 1024 || bytes <= cache[dev]) return cudaSuccess;
+    if (bytes + fixed <= 48 * 1024 || bytes <= __atomic_load_n(&cache[dev], __ATOMIC_ACQUIRE)) return cudaSuccess;
+    static std::mutex mu;
+    std::lock_guard<std::mutex> lock(mu);
+    if (bytes <= cache[dev]) return cudaSuccess;
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    if (e == cudaSuccess) cache[dev] = bytes;
+    if (e == cudaSuccess) __atomic_store_n(&cache[dev], bytes, __ATOMIC_RELEASE);
     return e;
 }
 

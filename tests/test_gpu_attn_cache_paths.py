@@ -1,5 +1,7 @@
 """The attention cache's launches by size: calls at either side of each rule that
 chooses a launch, each of which says which one it is for."""
+from concurrent.futures import ThreadPoolExecutor
+
 import pytest
 import torch
 
@@ -40,3 +42,35 @@ def test_eviction_by_the_tables_reach(ofb, cuda):
     # no max_len: the table's reach bounds the lengths, here 81920 whatever they are
     c = GpuCache(ofb, [3000] * 5, 8, 64, 64, reach=81920)
     check_eviction(ofb, c, 1024, 64)
+
+
+# ---- host threads --------------------------------------------------------------------
+
+def test_threads_with_calls_of_different_sizes(ofb, cuda):
+    # each raises the kernels' shared-memory limits to what its sizes need, at the same time
+    def work(lens, keep):
+        c = GpuCache(ofb, lens, 2, 64, 16, seed=keep)
+        q = torch.randn(len(lens), 4, 64, device=cuda)
+        state = [t.clone() for t in (c.k, c.v, c.weight, c.order)]
+
+        def step():
+            for t, s in zip((c.k, c.v, c.weight, c.order), state):
+                t.copy_(s)
+            out = ofb.attn_decode(c.handle, q, c.dlens)
+            return [out, *ofb.kv_evict(c.handle, c.dlens, keep=keep, recent=10), c.k.clone(), c.order.clone()]
+        return step
+
+    works = [work([20000, 40], 700), work([9000] * 3, 800), work([300] * 400, 100), work([50] * 900 + [500], 40)]
+    want = [w() for w in works]
+    torch.cuda.synchronize()
+
+    def loop(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(8):
+                got = works[i]()
+                torch.cuda.current_stream().synchronize()
+                bits = lambda t: t.contiguous().view(torch.uint8)  # noqa: E731
+                assert all(torch.equal(bits(a), bits(b)) for a, b in zip(got, want[i]))
+
+    with ThreadPoolExecutor(len(works)) as pool:
+        list(pool.map(loop, range(len(works))))

@@ -25,3 +25,7 @@ def run_check(tmp_path, name):
 
 def test_a_reported_failure_is_not_reported_again(tmp_path):
     run_check(tmp_path, "last_error_check")
+
+
+def test_threads_never_lower_a_shared_memory_limit(tmp_path):
+    run_check(tmp_path, "smem_limit_check")
