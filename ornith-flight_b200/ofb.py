@@ -264,6 +264,8 @@ def _elsewhere(device: torch.device, stream, call, *args, **kw):
     """call(...) with `device` and `stream` current."""
     if device.type != "cuda":
         raise OfbError(EINVAL, "tensors must be on a CUDA device")
+    if stream is not None and stream.device != device:
+        raise OfbError(EINVAL, f"the stream is on {stream.device}, the tensors are on {device}")
     with torch.cuda.device(device), torch.cuda.stream(stream):
         return call(*args, **kw)
 
