@@ -257,7 +257,8 @@ def _rows(t: torch.Tensor, shape, dtype, device, name: str) -> int:
     return row
 
 
-_get_device, _raw_stream = torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream
+# (None in a torch built without CUDA, which has no tensors that get that far)
+_get_device, _raw_stream = (getattr(torch._C, name, None) for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"))
 
 
 def _elsewhere(device: torch.device, stream, call, *args, **kw):
