@@ -1,13 +1,32 @@
 """For the tests of the attention cache's paths: which launch a call's sizes lead
 to (restated from the dispatch rules), caches built on the GPU, and 64-bit
 restatements that run there, for sizes at which host loops would take too long."""
+import re
+
 import numpy as np
 import torch
 
-from attn_cache_ref import DT
+from attn_cache_ref import DT, HALF_STEP, attend_tol
 
 
 # ---- which launch a call takes ---------------------------------------------------
+
+def launches(call, tmp_path):
+    """(mangled kernel name, CTAs, threads of a CTA, dynamic shared memory) of each
+    launch of call(), which is captured into a graph and not run."""
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    graph.enable_debug_mode()
+    with torch.cuda.graph(graph):
+        call()
+    graph.debug_dump(str(tmp_path / "graph.dot"))
+    text = (tmp_path / "graph.dot").read_text()
+    found = re.findall(r"\(topoId: (\d+)\) \| (\w+)\\<\\<\\<(.*?)\\>\\>\\>", text)
+    out = []
+    for _, name, shape in sorted(found, key=lambda f: -int(f[0])):
+        *grid, block, smem = [int(x) for x in re.findall(r"\d+", shape)]
+        out.append((name, tuple(grid), block, smem))
+    return out
+
 
 def evict_path(rows, bound, keep, recent, sms=148):
     """(CTAs of a cluster, threads of a CTA, entries of a CTA, whether order
@@ -117,4 +136,32 @@ def check_eviction(ofb, c, keep, recent, max_len=0):
     assert new.tolist() == [min(n, keep) for n in lens]
     for x in names:
         assert torch.equal(bits(getattr(c, x)), want[x]), x
+    assert c.handle.device_errors() == 0
+
+
+def check_attention(c, q, got, io, scale, weight_before=None):
+    """One attn_decode call's output, and weights, against softmax in 64 bits; the
+    bounds are those of the tests on small caches."""
+    H, d = q.shape[1:]
+    G = H // c.kv
+    for b, n in enumerate(c.lens):
+        if not n:
+            assert (got[b] == 0).all()
+            continue
+        k, v = (c.rows(x, b, n).double().transpose(0, 1) for x in "kv")  # [kv, n, d]
+        x = q[b].double().view(c.kv, G, d)
+        p = torch.softmax(scale * (x @ k.mT), -1)
+        want, p = p @ v, p.sum(1)
+        size = abs(scale) * (x.abs() @ k.abs().mT).amax(-1, keepdim=True)
+        tol = attend_tol(size, d)
+        bound = (tol + (2.0 ** -17 if io == "bf16" else 0)) * v.abs().max() + HALF_STEP[io] * want.abs() + 2.0 ** -25 * (io == "f16")
+        err = (got[b].double().view(want.shape) - want).abs()
+        assert (err <= bound).all(), f"sequence {b} of {n}: off by {err.max()}, bound {bound.max()}"
+        if weight_before is not None:
+            pg, s = c.at(b, n)
+            old, new = weight_before[pg, :, s].double().T, c.weight[pg, :, s].double().T
+            slack = tol.amax(1) * p + 2.0 ** -23 * (old.abs() + p)
+            assert ((new - old - p).abs() <= slack).all(), f"weights of sequence {b}"
+    if weight_before is not None:
+        assert torch.equal(c.weight.view(torch.int32)[~c.live], weight_before.view(torch.int32)[~c.live])
     assert c.handle.device_errors() == 0
