@@ -252,8 +252,8 @@ int ofb_sample(const float *logits, int vocab, float temperature, float r, float
  * table entries behind them may hold anything, and what is in memory behind
  * the last entry is neither used nor changed. A page number outside
  * [0, n_pages) is never followed: such an entry counts as masked (attention),
- * is dropped (append), or as the lightest (eviction), and OFB_CACHE_EPAGE is
- * set. No page may belong to two sequences of one call that write it. */
+ * is dropped (append), or as the lightest (eviction; one that would move into
+ * its place is lost), and OFB_CACHE_EPAGE is set. No page may belong to two sequences of one call that write it. */
 #define OFB_CACHE_EPAGE 1u  /* a page number outside [0, n_pages) */
 #define OFB_CACHE_ELEN 2u   /* a length above the call's max_len or the table's reach: cut down to it */
 #define OFB_CACHE_EINDEX 4u /* append: a sequence or place outside the table: the row was dropped */
@@ -335,8 +335,16 @@ int ofb_rope_append(const ofb_kv_cache *cache, const ofb_rope_config *rope, int 
  * reach) and sizes the scratch. q and out: type OFB_TYPE_F32 or the cache's,
  * row b at b*q_stride (b*out_stride), heads consecutive; they must not overlap.
  * accumulate 1: cache->weight of entry n of kv head g grows by the sum of p_n
- * over g's query heads. Softmax, sums and weights are f32 and queries and
- * probabilities are not rounded to the cache's type. scratch:
+ * over g's query heads. Softmax, sums and weights are f32. Neither queries nor
+ * probabilities are rounded to the cache's type; they go in as two or three
+ * numbers of it: f32 queries with 24 bits over bf16 and 22 over fp16,
+ * probabilities with 24 bits over bf16 where the output is f32, 16 where it is
+ * bf16, and 22 over fp16. A NaN or an infinity among the attended entries stays
+ * where it belongs (a key's: its kv head's query heads; a value's: its column of
+ * them; a query's: its head), but since numbers are multiplied in parts, an
+ * infinite key or value may give NaN where the formula gives an infinity or
+ * leaves the entry without weight. Where no entry has a score above -infinity the
+ * output is zeros. scratch:
  * ofb_attn_scratch_size() bytes of device memory, 16-byte aligned, needing no
  * initialisation; calls whose GPU work may overlap (other streams, graphs
  * replayed side by side) need scratch of their own. */

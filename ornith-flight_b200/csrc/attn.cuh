@@ -29,8 +29,8 @@
 // distributed shared memory, which saves the second launch.
 //
 // Measured: 24 sequences of 8 to 40 thousand entries, 2 kv heads of 256, fp16
-// (1.11 GB): 182 us, 6.1 TB/s; a plain sum over as many bytes takes 183. The copies
-// alone, without the products, take 178.
+// (1.11 GB): 180 to 190 us, 5.8 to 6.1 TB/s; a plain sum over as many bytes takes 183.
+// The copies alone, without the products, take 178.
 //
 // The products run on mma.sync m16n8k16 (bf16 or fp16, f32 sums): 16 rows of A
 // by 8 entries or 8 output columns. Neither an f32 query nor a probability is
@@ -42,9 +42,12 @@
 //     fp16 hi + low of 2^14 p (22 bits).
 // Up to 8 query heads of a kv head fill 8 rows; the other 8 rows take the next
 // part of the same numbers, so that two parts cost one product. 9 to 16 heads
-// (R = 16) fill all rows, with a product per part; more take several passes over
-// K and V, and so do 9 to 16 f32 heads of 192 or 256, whose queries and sums are
-// more than the registers hold.
+// (R = 16) fill all rows, with a product per part; more take several passes, a part
+// of the work each, which read K and V again: ceil(G / 16), or ceil(G / 8) with f32
+// heads of 192 or 256, of which 16 have more queries and sums than one warp's registers
+// hold. 24 sequences of 8 to 40 thousand entries in bf16: 2 x 8 f32 heads of 256 203 us,
+// 2 x 16 417; 1 x 16 bf16 heads of 128 60 us, 1 x 128 324. (Warps of a CTA that share
+// tiles and take a pass each have not been tried.)
 // A number's parts end in the same thread, which adds them in f32. With f32 output
 // each tile's product starts at zero and is added to the running sum by an FFMA,
 // since the tensor core's own accumulation cuts off where an addition rounds; with
@@ -135,6 +138,8 @@ template <int D, int QB> struct AttnShape {
     // tile
     static __host__ __device__ constexpr int ring(int w) { return w * S * TILE_BYTES; }
     static __host__ __device__ constexpr int head(int w) { return ring(w) + (W + 1) * 16 * 8 + QB; }
+    // (head_dim 64: beside more than 869 sequences' an SM has room for one CTA, not two; 1400
+    // sequences of 100 to 300 entries, 2 kv heads: 103 us, 860 43)
     static constexpr int smem(int B) { return head(W) + (B + 1) * 4 + (B + 3) / 4 * 4; }
     static_assert(CTAS <= ATT_MAX_CTAS, "parts in the scratch");
     static_assert(TILE_BYTES >= 16 * (D + 4) * 4, "a warp's sums must fit one ring slot");

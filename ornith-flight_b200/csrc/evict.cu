@@ -57,7 +57,7 @@ constexpr int EV_FUSED_FEW = 48, EV_FUSED = 128, EV_FEW = 64;
 // with one
 constexpr int EV_RUN = 4096;
 constexpr int EV_CAND = 256;    // entries ranked directly (at most one per thread)
-constexpr int EV_STATIC = 5120;  // bytes of the kernel's static arrays, rounded up
+constexpr int EV_STATIC = 5120;  // the kernel's static arrays (4416 bytes), rounded up
 constexpr int EV_KEYS = 49152;  // keys a CTA holds at most: OFB_EVICT_MAX_LEN / EV_CLUSTER
 static_assert(EV_KEYS < 1 << 16, "counts of a CTA's holes and spares share a word");
 static_assert(OFB_EVICT_MAX_LEN == EV_CLUSTER * EV_KEYS, "eviction length limit");

@@ -231,7 +231,9 @@ def sample(logits: torch.Tensor, temperature: float, r: float, stream=None) -> i
 # ---- attention cache ----------------------------------------------------------
 # Each call runs on the device of its tensors, on `stream` or that device's
 # current stream. Tensors of other types, shapes, strides or devices than the
-# call takes raise OfbError (EINVAL) before anything is launched.
+# call takes, and a stream of another device, raise OfbError (EINVAL) before
+# anything is launched. The calls are for inference: autograd does not see them,
+# so a result has no gradient, whether or not its inputs require one.
 
 _TYPE_OF = {torch.float32: TYPE_F32, torch.bfloat16: TYPE_BF16, torch.float16: TYPE_F16}
 
