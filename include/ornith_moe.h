@@ -253,7 +253,8 @@ int ofb_sample(const float *logits, int vocab, float temperature, float r, float
  * the last entry is neither used nor changed. A page number outside
  * [0, n_pages) is never followed: such an entry counts as masked (attention),
  * is dropped (append), or as the lightest (eviction; one that would move into
- * its place is lost), and OFB_CACHE_EPAGE is set. No page may belong to two sequences of one call that write it. */
+ * its place is lost), and OFB_CACHE_EPAGE is set. No page may belong to two
+ * sequences of one call that write it. */
 #define OFB_CACHE_EPAGE 1u  /* a page number outside [0, n_pages) */
 #define OFB_CACHE_ELEN 2u   /* a length above the call's max_len or the table's reach: cut down to it */
 #define OFB_CACHE_EINDEX 4u /* append: a sequence or place outside the table: the row was dropped */
