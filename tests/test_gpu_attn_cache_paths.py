@@ -9,7 +9,7 @@ import torch
 from attn_cache_paths import GpuCache, check_attention, check_eviction, evict_path, launches
 from attn_cache_ref import DT
 
-pytestmark = [pytest.mark.gpu, pytest.mark.filterwarnings("ignore:DEBUG. calling cudaGraphDebugDotPrint")]
+pytestmark = [pytest.mark.gpu, pytest.mark.filterwarnings("ignore:DEBUG. ")]
 
 
 def one_long(seqs, bound, short=700):
